@@ -6,3 +6,5 @@
 #include "attention.cu"
 #include "peer.cu"
 #include "vae.cu"
+#include "rotary.cu"
+#include "resnorm.cu"

@@ -1,0 +1,601 @@
+// The gated residual between two norms, forward and backward, one pass over the rows each:
+//   m = post-norm(y) (none, rms or layer), u = post_w m
+//   x' = x + alpha gate[item] u
+//   n = pre-norm(x') (rms or layer), h = pre_w n (1 + scale[item]) + shift[item]
+// with the normalised rows n = (t - mean) r (rms: mean = 0), r = 1 / sqrt(mean((t - mean)^2) + eps).
+// Backward, from dh and the gradient dx' that reaches x' from behind:
+//   g = dh (1 + scale) pre_w,  G = dx' + r (g - mean(g) - n mean(g n))     (rms: without mean(g))
+//   dx = G,  du = alpha gate G,  g = du post_w,  dy = r_y (g - mean(g) - m mean(g m))
+//   dgate = alpha sum_item G u,  dscale = sum_item dh n pre_w,  dshift = sum_item dh,
+//   dpost_w = sum du m,  dpre_w = sum dh (1 + scale) n
+// The statistics are computed again from y and x' (a row is in registers anyway), so the forward saves
+// nothing.
+//
+// Both passes are bound by HBM. A row is held in registers by T = C / V threads (V = 8 columns a
+// thread, or 1 where the columns or alignments are odd); the row's sums are warp shuffles and one
+// exchange through shared memory a round. The backward's column sums stay in registers over the rows
+// of a block, each block writes one partial row of sums and a second kernel adds the partials in a
+// fixed order: no atomics, the same inputs give the same bits.
+
+#include "internal.h"
+#include "sm100.cuh"
+
+namespace anima {
+namespace resnorm {
+
+constexpr int kNone = 0, kRms = 1, kLayer = 2;
+constexpr int kThreads = 256;
+constexpr int kMaxCols = 4096;  // 16 columns a thread: the backward's five sums of each fit its registers
+constexpr int kMaxSums = 5;
+
+struct Params {
+  const void* x;   // forward: x; backward: x'
+  const void* y;
+  const void* dh;  // backward
+  const void* dx;  // backward: the gradient that reaches x' from behind, or NULL
+  void* o0;        // forward: x'; backward: dx
+  void* o1;        // forward: h;  backward: dy
+  long long ldx, ldy, lddh, lddx, ldo0, ldo1;
+  int dtx, dty, dth;  // x, x', dx share a type, so do y and dy, and h and dh
+  int rows, C, L;     // L rows an item
+  int post, pre;
+  float alpha, eps;
+  const float *gate, *scale, *shift, *post_w, *pre_w;
+  long long ldgate, ldscale, ldshift;
+  int layer_threads;  // T
+  // backward: the partial sums [item][part][k][C] and which sum is where (-1: not asked for)
+  float* part;
+  int parts, part_rows, sums;
+  int s_gate, s_postw, s_prew, s_scale, s_shift;
+};
+
+__device__ __forceinline__ float lo16(uint32_t w, int dt) {
+  return dt == ANIMA_BF16 ? __uint_as_float(w << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(w)));
+}
+__device__ __forceinline__ float hi16(uint32_t w, int dt) {
+  return dt == ANIMA_BF16 ? __uint_as_float(w & 0xFFFF0000u)
+                          : __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)));
+}
+
+// V elements as they lie in memory: 8 of 32 bits take both vectors, 8 of 16 bits the first.
+template <int V>
+struct Raw {
+  uint4 a, b;
+};
+template <>
+struct Raw<1> {
+  uint32_t a;
+};
+
+template <int V>
+__device__ __forceinline__ void load_raw(Raw<V>& r, const void* p, int dt, size_t at) {
+  if constexpr (V == 8) {
+    if (dt == ANIMA_F32) {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at);
+      r.a = q[0];  // plain loads: an output may be its input
+      r.b = q[1];
+    } else {
+      r.a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+    }
+  } else {
+    r.a = dt == ANIMA_F32 ? static_cast<const uint32_t*>(p)[at]
+                          : static_cast<uint32_t>(static_cast<const uint16_t*>(p)[at]);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void unpack(const Raw<V>& r, int dt, float (&v)[V]) {
+  if constexpr (V == 8) {
+    const uint32_t a[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+    if (dt == ANIMA_F32) {
+      const uint32_t b[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = __uint_as_float(a[i]);
+        v[4 + i] = __uint_as_float(b[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = lo16(a[i], dt);
+        v[2 * i + 1] = hi16(a[i], dt);
+      }
+    }
+  } else {
+    v[0] = dt == ANIMA_F32 ? __uint_as_float(r.a) : lo16(r.a, dt);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int dt) {
+  if (dt == ANIMA_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int V>
+__device__ __forceinline__ void store(void* p, int dt, size_t at, const float (&v)[V]) {
+  if constexpr (V == 8) {
+    if (dt == ANIMA_F32) {
+      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+      q[0] = make_float4(v[0], v[1], v[2], v[3]);
+      q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
+          make_uint4(pack16(v[0], v[1], dt), pack16(v[2], v[3], dt), pack16(v[4], v[5], dt), pack16(v[6], v[7], dt));
+    }
+  } else {
+    if (dt == ANIMA_F32)
+      static_cast<float*>(p)[at] = v[0];
+    else
+      static_cast<uint16_t*>(p)[at] = static_cast<uint16_t>(pack16(v[0], 0.f, dt));
+  }
+}
+
+// fp32 parameters of the row's columns (modulations, norm weights); `none` where there are none
+template <int V>
+__device__ __forceinline__ void param(const float* p, size_t at, float none, float (&v)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = none;
+  } else if constexpr (V == 8) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p + at)), b = __ldg(reinterpret_cast<const float4*>(p + at) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    v[0] = __ldg(p + at);
+  }
+}
+
+// Sums of K values over the T threads of a row, to all of them. `buf` alternates between calls, so one
+// barrier a call is enough: a value is read before its thread can reach the barrier after next.
+template <int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* red, int& buf) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], s);
+  const int W = blockDim.x >> 5;
+  if (W == 1) return;
+  float* slot = red + (buf * blockDim.y + threadIdx.y) * (W * 2);
+  buf ^= 1;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) slot[(threadIdx.x >> 5) * 2 + k] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = 0.f;
+    for (int w = 0; w < W; ++w) v[k] += slot[w * 2 + k];
+  }
+}
+constexpr int kRedFloats = 2 * 2 * (kThreads / 32);  // [2 buffers][rows][warps][2 values]
+
+// A thread's columns: NV vectors of V, T V apart.
+template <int V, int NV>
+struct Cols {
+  int c0, step, C;
+  __device__ __forceinline__ Cols(const Params& p) : c0(threadIdx.x * V), step(blockDim.x * V), C(p.C) {}
+  __device__ __forceinline__ int at(int k) const { return c0 + k * step; }
+  __device__ __forceinline__ bool in(int k) const { return at(k) < C; }  // V divides C
+};
+
+// In place: t -> its normalised row; returns r. Columns past C hold 0 and do not count.
+template <int V, int NV>
+__device__ __forceinline__ float normalise(float (&t)[NV][V], const Cols<V, NV>& cols, int kind, float inv_c, float eps,
+                                           float* red, int& buf) {
+  if (kind == kLayer) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[0] += t[k][i];
+    row_sum(s, red, buf);
+    const float mean = s[0] * inv_c;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (cols.in(k)) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[k][i] -= mean;
+      }
+  }
+  float q[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[0] = fmaf(t[k][i], t[k][i], q[0]);
+  row_sum(q, red, buf);
+  const float r = 1.0f / sqrtf(fmaf(q[0], inv_c, eps));
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[k][i] *= r;
+  return r;
+}
+
+template <int V, int NV>
+__device__ __forceinline__ void load_row(float (&t)[NV][V], const Cols<V, NV>& cols, const void* p, int dt, size_t base,
+                                         bool live) {
+  Raw<V> raw[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (live && cols.in(k)) load_raw<V>(raw[k], p, dt, base + cols.at(k));
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (live && cols.in(k)) {
+      unpack<V>(raw[k], dt, t[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) t[k][i] = 0.f;
+    }
+  }
+}
+
+template <int V, int NV>
+__global__ void __launch_bounds__(kThreads) residual_norm_kernel(const Params p) {
+  __shared__ float red[kRedFloats];
+  int buf = 0;
+  const Cols<V, NV> cols(p);
+  const int row = blockIdx.x * blockDim.y + threadIdx.y;
+  const bool live = row < p.rows;
+  const size_t r = live ? row : 0;
+  const float inv_c = 1.0f / static_cast<float>(p.C);
+  float y[NV][V], x[NV][V];
+  load_row<V, NV>(y, cols, p.y, p.dty, r * p.ldy, live);
+  load_row<V, NV>(x, cols, p.x, p.dtx, r * p.ldx, live);
+  if (p.post != kNone) normalise<V, NV>(y, cols, p.post, inv_c, p.eps, red, buf);
+  const size_t item = r / p.L;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (!cols.in(k)) continue;
+    float g[V], w[V];
+    param<V>(p.gate, item * p.ldgate + cols.at(k), 1.f, g);
+    param<V>(p.post_w, cols.at(k), 1.f, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[k][i] = fmaf(p.alpha * g[i], y[k][i] * w[i], x[k][i]);
+    if (live) store<V>(p.o0, p.dtx, r * p.ldo0 + cols.at(k), x[k]);
+  }
+  normalise<V, NV>(x, cols, p.pre, inv_c, p.eps, red, buf);
+  if (!live) return;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (!cols.in(k)) continue;
+    float a[V], b[V], w[V];
+    param<V>(p.scale, item * p.ldscale + cols.at(k), 0.f, a);
+    param<V>(p.shift, item * p.ldshift + cols.at(k), 0.f, b);
+    param<V>(p.pre_w, cols.at(k), 1.f, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[k][i] = fmaf(x[k][i] * w[i], 1.0f + a[i], b[i]);
+    store<V>(p.o1, p.dth, r * p.ldo1 + cols.at(k), x[k]);
+  }
+}
+
+// g -> r (g - mean(g) - n mean(g n)), the gradient through normalise()
+template <int V, int NV>
+__device__ __forceinline__ void normalise_back(float (&g)[NV][V], const float (&n)[NV][V], const Cols<V, NV>& cols,
+                                               int kind, float r, float inv_c, float* red, int& buf) {
+  float s[2] = {0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[0] += g[k][i];
+      s[1] = fmaf(g[k][i], n[k][i], s[1]);
+    }
+  row_sum(s, red, buf);
+  const float mg = kind == kLayer ? s[0] * inv_c : 0.f, mgn = s[1] * inv_c;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[k][i] = r * (g[k][i] - mg - n[k][i] * mgn);
+}
+
+// One block a part: part_rows rows of one item, blockDim.y at a time.
+template <int V, int NV>
+__global__ void __launch_bounds__(kThreads, NV * V <= 8 ? 2 : 1) residual_norm_grad_kernel(const Params p) {
+  __shared__ float red[kRedFloats];
+  int buf = 0;
+  const Cols<V, NV> cols(p);
+  const int item = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const int first = part * p.part_rows, last = min(p.L, first + p.part_rows);
+  const float inv_c = 1.0f / static_cast<float>(p.C);
+  float sum[kMaxSums][NV][V];
+#pragma unroll
+  for (int s = 0; s < kMaxSums; ++s)
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[s][k][i] = 0.f;
+  for (int l0 = first; l0 < last; l0 += blockDim.y) {
+    const int l = l0 + threadIdx.y;
+    const bool live = l < last;
+    const size_t r = static_cast<size_t>(item) * p.L + (live ? l : first);
+    float x[NV][V], y[NV][V], dh[NV][V], dx[NV][V];
+    load_row<V, NV>(x, cols, p.x, p.dtx, r * p.ldx, live);
+    load_row<V, NV>(dh, cols, p.dh, p.dth, r * p.lddh, live);
+    load_row<V, NV>(y, cols, p.y, p.dty, r * p.ldy, live);
+    load_row<V, NV>(dx, cols, p.dx, p.dtx, r * p.lddx, live && p.dx);
+    const float rx = normalise<V, NV>(x, cols, p.pre, inv_c, p.eps, red, buf);
+    const float ry = p.post != kNone ? normalise<V, NV>(y, cols, p.post, inv_c, p.eps, red, buf) : 1.f;
+    float w[V], a[V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (!live || !cols.in(k)) continue;
+      param<V>(p.scale, static_cast<size_t>(item) * p.ldscale + cols.at(k), 0.f, a);
+      param<V>(p.pre_w, cols.at(k), 1.f, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float t = dh[k][i] * x[k][i];
+        sum[0][k][i] += dh[k][i];
+        sum[1][k][i] = fmaf(t, w[i], sum[1][k][i]);
+        sum[2][k][i] = fmaf(t, 1.0f + a[i], sum[2][k][i]);
+        dh[k][i] *= (1.0f + a[i]) * w[i];
+      }
+    }
+    normalise_back<V, NV>(dh, x, cols, p.pre, rx, inv_c, red, buf);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (!live || !cols.in(k)) continue;
+      float g[V];
+      param<V>(p.gate, static_cast<size_t>(item) * p.ldgate + cols.at(k), 1.f, g);
+      param<V>(p.post_w, cols.at(k), 1.f, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) dx[k][i] += dh[k][i];
+      store<V>(p.o0, p.dtx, r * p.ldo0 + cols.at(k), dx[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float t = p.alpha * dx[k][i] * y[k][i];
+        sum[3][k][i] = fmaf(t, w[i], sum[3][k][i]);
+        sum[4][k][i] = fmaf(t, g[i], sum[4][k][i]);
+        dx[k][i] *= p.alpha * g[i] * w[i];
+      }
+    }
+    if (p.post != kNone) normalise_back<V, NV>(dx, y, cols, p.post, ry, inv_c, red, buf);
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (cols.in(k)) store<V>(p.o1, p.dty, r * p.ldo1 + cols.at(k), dx[k]);
+    }
+  }
+  if (!p.sums) return;
+  const int where[kMaxSums] = {p.s_shift, p.s_scale, p.s_prew, p.s_gate, p.s_postw};
+  float* out = p.part + (static_cast<size_t>(blockIdx.x) * blockDim.y + threadIdx.y) * p.sums * p.C;
+#pragma unroll
+  for (int s = 0; s < kMaxSums; ++s) {
+    if (where[s] < 0) continue;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (cols.in(k)) store<V>(out, ANIMA_F32, static_cast<size_t>(where[s]) * p.C + cols.at(k), sum[s][k]);
+  }
+}
+
+struct SumParams {
+  const float* part;  // [items][parts][sums][C]
+  int items, parts, sums, C;
+  float* out[kMaxSums];
+  int per_item[kMaxSums];  // out [items][C], else [C] over all items
+};
+
+// out = the partial rows added in order. A block takes 32 columns of one output row; its 8 warps each
+// add every 8th partial, then the first adds the eight.
+__global__ void __launch_bounds__(256) partial_sum_kernel(const SumParams p) {
+  __shared__ float red[8][32];
+  const int s = blockIdx.z, item = blockIdx.y;
+  if (!p.per_item[s] && item) return;
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  const int n = p.per_item[s] ? p.parts : p.parts * p.items;
+  const float* base = p.part + (static_cast<size_t>(item) * p.parts * p.sums + s) * p.C;
+  float t = 0.f;
+  if (c < p.C)
+    for (int i = threadIdx.y; i < n; i += 8) t += base[static_cast<size_t>(i) * p.sums * p.C + c];
+  red[threadIdx.y][threadIdx.x] = t;
+  __syncthreads();
+  if (threadIdx.y || c >= p.C) return;
+  t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x];
+  p.out[s][static_cast<size_t>(item) * p.C + c] = t;
+}
+
+struct Shape {
+  int V, NV, T, Y;  // columns a vector, vectors a thread, threads a row, rows a block
+};
+
+Shape shape_of(int C, bool vec) {
+  Shape s;
+  s.V = vec && C % 8 == 0 ? 8 : 1;
+  const int n = C / s.V;
+  s.NV = 1;
+  while (static_cast<long long>(s.NV) * kThreads < n) s.NV *= 2;
+  if (s.V == 1) s.NV = s.NV <= 8 ? 8 : 16;
+  s.T = ((n + s.NV - 1) / s.NV + 31) / 32 * 32;
+  s.Y = kThreads / s.T;
+  return s;
+}
+
+// Rows of one item that a block of the backward pass takes: about two blocks an SM over all items.
+void parts_of(const Shape& s, int items, int L, int sms, int& parts, int& part_rows) {
+  const int want = (2 * sms + items - 1) / items;
+  const int most = (L + s.Y - 1) / s.Y;
+  parts = want < most ? want : most;
+  part_rows = ((L + parts - 1) / parts + s.Y - 1) / s.Y * s.Y;
+  parts = (L + part_rows - 1) / part_rows;
+}
+
+int count_sums(const anima_residual_norm_args* a) {
+  return (a->dshift != nullptr) + (a->dscale != nullptr) + (a->dpre_w != nullptr) + (a->dgate != nullptr) +
+         (a->dpost_w != nullptr);
+}
+
+int check(const char* fn, const anima_residual_norm_args* a, bool grad) {
+  ANIMA_REQUIRE(a->rows >= 0 && a->cols > 0 && a->cols <= kMaxCols, "%s: %d rows of %d columns (at most %d)", fn,
+                a->rows, a->cols, kMaxCols);
+  ANIMA_REQUIRE(a->rows_per_item > 0 && a->rows % a->rows_per_item == 0, "%s: %d rows are not items of %d rows", fn,
+                a->rows, a->rows_per_item);
+  for (const int dt : {a->x_dtype, a->y_dtype, a->h_dtype})
+    ANIMA_REQUIRE(dt == ANIMA_F32 || dt == ANIMA_BF16 || dt == ANIMA_F16, "%s: dtype %d", fn, dt);
+  ANIMA_REQUIRE(a->post >= kNone && a->post <= kLayer, "%s: post norm %d (0 none, 1 rms, 2 layer)", fn, a->post);
+  ANIMA_REQUIRE(a->pre == kRms || a->pre == kLayer, "%s: pre norm %d (1 rms, 2 layer)", fn, a->pre);
+  ANIMA_REQUIRE(a->eps >= 0.f, "%s: eps %g", fn, a->eps);
+  ANIMA_REQUIRE(!a->post_w || a->post != kNone, "%s: post_w without a post norm", fn);
+  if (a->rows == 0) return ANIMA_OK;
+  ANIMA_REQUIRE(a->x_out && a->y, "%s: NULL data pointer", fn);
+  ANIMA_REQUIRE(a->ldx_out >= a->cols && a->ldy >= a->cols, "%s: a row stride is below %d columns", fn, a->cols);
+  for (const long long ld : {a->gate ? a->ld_gate : 0LL, a->scale ? a->ld_scale : 0LL, a->shift ? a->ld_shift : 0LL})
+    ANIMA_REQUIRE(ld >= 0, "%s: negative stride of a modulation", fn);
+  if (!grad) {
+    ANIMA_REQUIRE(a->x && a->h && a->ldx >= a->cols && a->ldh >= a->cols, "%s: x or h is NULL or its stride too small",
+                  fn);
+    return ANIMA_OK;
+  }
+  ANIMA_REQUIRE(a->dh && a->dx && a->dy, "%s: dh, dx or dy is NULL", fn);
+  ANIMA_REQUIRE(a->lddh >= a->cols && a->lddx >= a->cols && a->lddy >= a->cols &&
+                    (!a->dx_out || a->lddx_out >= a->cols),
+                "%s: a row stride is below %d columns", fn, a->cols);
+  ANIMA_REQUIRE((!a->dgate || a->gate) && (!a->dscale || a->scale) && (!a->dshift || a->shift) &&
+                    (!a->dpost_w || a->post_w) && (!a->dpre_w || a->pre_w),
+                "%s: a gradient is asked for whose parameter is NULL", fn);
+  return ANIMA_OK;
+}
+
+bool aligned(const void* p, int dt, long long ld) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * (dt == ANIMA_F32 ? 4 : 2)) % 16 == 0);
+}
+
+// Whether every tensor can be read and written in 16-byte vectors of a row.
+bool vectors_ok(const anima_residual_norm_args* a, bool grad) {
+  const int f = ANIMA_F32;
+  bool ok = aligned(a->y, a->y_dtype, a->ldy) && aligned(a->x_out, a->x_dtype, a->ldx_out) &&
+            aligned(a->gate, f, a->ld_gate) && aligned(a->scale, f, a->ld_scale) && aligned(a->shift, f, a->ld_shift) &&
+            aligned(a->post_w, f, 0) && aligned(a->pre_w, f, 0);
+  if (!grad) return ok && aligned(a->x, a->x_dtype, a->ldx) && aligned(a->h, a->h_dtype, a->ldh);
+  return ok && aligned(a->dh, a->h_dtype, a->lddh) && aligned(a->dx_out, a->x_dtype, a->lddx_out) &&
+         aligned(a->dx, a->x_dtype, a->lddx) && aligned(a->dy, a->y_dtype, a->lddy) && aligned(a->workspace, f, 0);
+}
+
+void fill(Params& p, const anima_residual_norm_args* a) {
+  p.y = a->y;
+  p.ldy = a->ldy;
+  p.dtx = a->x_dtype;
+  p.dty = a->y_dtype;
+  p.dth = a->h_dtype;
+  p.rows = a->rows;
+  p.C = a->cols;
+  p.L = a->rows_per_item;
+  p.post = a->post;
+  p.pre = a->pre;
+  p.alpha = a->alpha;
+  p.eps = a->eps;
+  p.gate = a->gate;
+  p.scale = a->scale;
+  p.shift = a->shift;
+  p.post_w = a->post_w;
+  p.pre_w = a->pre_w;
+  p.ldgate = a->ld_gate;
+  p.ldscale = a->ld_scale;
+  p.ldshift = a->ld_shift;
+}
+
+using Kernel = void (*)(const Params);
+
+}  // namespace resnorm
+}  // namespace anima
+
+extern "C" int anima_residual_norm(anima_ctx* ctx, const anima_residual_norm_args* a) {
+  using namespace anima::resnorm;
+  ANIMA_REQUIRE(ctx && a, "anima_residual_norm: NULL argument");
+  ANIMA_ON_DEVICE(ctx);
+  int st = check("anima_residual_norm", a, false);
+  if (st || a->rows == 0) return st;
+  const Shape s = shape_of(a->cols, vectors_ok(a, false));
+  Params p{};
+  fill(p, a);
+  p.x = a->x;
+  p.ldx = a->ldx;
+  p.o0 = a->x_out;
+  p.ldo0 = a->ldx_out;
+  p.o1 = a->h;
+  p.ldo1 = a->ldh;
+  const Kernel fn = s.V == 8 ? (s.NV == 1 ? residual_norm_kernel<8, 1> : residual_norm_kernel<8, 2>)
+                             : (s.NV == 8 ? residual_norm_kernel<1, 8> : residual_norm_kernel<1, 16>);
+  ProfScope prof(ctx, "residual_norm", 0, static_cast<double>(a->rows) * a->cols * 12);
+  fn<<<(a->rows + s.Y - 1) / s.Y, dim3(s.T, s.Y), 0, ctx->stream>>>(p);
+  return check_launch("residual_norm_kernel");
+}
+
+extern "C" int anima_residual_norm_backward_workspace(anima_ctx* ctx, const anima_residual_norm_args* a, size_t* bytes) {
+  using namespace anima::resnorm;
+  ANIMA_REQUIRE(ctx && a && bytes, "anima_residual_norm_backward_workspace: NULL argument");
+  *bytes = 0;
+  int st = check("anima_residual_norm_backward_workspace", a, true);
+  if (st || a->rows == 0) return st;
+  // the larger of the two shapes, so that the answer does not depend on alignments
+  for (const bool vec : {false, true}) {
+    const Shape s = shape_of(a->cols, vec);
+    int parts, part_rows;
+    parts_of(s, a->rows / a->rows_per_item, a->rows_per_item, ctx->num_sms, parts, part_rows);
+    const size_t n = static_cast<size_t>(a->rows / a->rows_per_item) * parts * s.Y * count_sums(a) * a->cols * 4;
+    if (n > *bytes) *bytes = n;
+  }
+  return ANIMA_OK;
+}
+
+extern "C" int anima_residual_norm_backward(anima_ctx* ctx, const anima_residual_norm_args* a) {
+  using namespace anima::resnorm;
+  ANIMA_REQUIRE(ctx && a, "anima_residual_norm_backward: NULL argument");
+  ANIMA_ON_DEVICE(ctx);
+  int st = check("anima_residual_norm_backward", a, true);
+  if (st || a->rows == 0) return st;
+  const int items = a->rows / a->rows_per_item;
+  const Shape s = shape_of(a->cols, vectors_ok(a, true));
+  Params p{};
+  fill(p, a);
+  p.x = a->x_out;
+  p.ldx = a->ldx_out;
+  p.dh = a->dh;
+  p.lddh = a->lddh;
+  p.dx = a->dx_out;
+  p.lddx = a->lddx_out;
+  p.o0 = a->dx;
+  p.ldo0 = a->lddx;
+  p.o1 = a->dy;
+  p.ldo1 = a->lddy;
+  parts_of(s, items, a->rows_per_item, ctx->num_sms, p.parts, p.part_rows);
+  p.sums = count_sums(a);
+  const size_t need = static_cast<size_t>(items) * p.parts * s.Y * p.sums * a->cols * 4;
+  ANIMA_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need),
+                "anima_residual_norm_backward: a workspace of %zu bytes is needed, %zu are given", need,
+                a->workspace ? a->workspace_bytes : 0);
+  p.part = static_cast<float*>(a->workspace);
+  SumParams sp{};
+  int k = 0;
+  auto slot = [&](float* out, bool per_item) {
+    if (!out) return -1;
+    sp.out[k] = out;
+    sp.per_item[k] = per_item;
+    return k++;
+  };
+  p.s_shift = slot(a->dshift, true);
+  p.s_scale = slot(a->dscale, true);
+  p.s_gate = slot(a->dgate, true);
+  p.s_prew = slot(a->dpre_w, false);
+  p.s_postw = slot(a->dpost_w, false);
+  const Kernel fn = s.V == 8 ? (s.NV == 1 ? residual_norm_grad_kernel<8, 1> : residual_norm_grad_kernel<8, 2>)
+                             : (s.NV == 8 ? residual_norm_grad_kernel<1, 8> : residual_norm_grad_kernel<1, 16>);
+  ANIMA_REQUIRE(static_cast<long long>(items) * p.parts < (1LL << 31) && items <= 65535,
+                "anima_residual_norm_backward: %d items are too many", items);
+  ProfScope prof(ctx, "residual_norm.grad", 0, static_cast<double>(a->rows) * a->cols * 20);
+  fn<<<items * p.parts, dim3(s.T, s.Y), 0, ctx->stream>>>(p);
+  st = check_launch("residual_norm_grad_kernel");
+  if (st || p.sums == 0) return st;
+  sp.part = p.part;
+  sp.items = items;
+  sp.parts = p.parts * s.Y;
+  sp.sums = p.sums;
+  sp.C = a->cols;
+  partial_sum_kernel<<<dim3((a->cols + 31) / 32, items, p.sums), dim3(32, 8), 0, ctx->stream>>>(sp);
+  return check_launch("partial_sum_kernel");
+}

@@ -34,7 +34,8 @@ EXPORTS = [
     "anima_attention", "anima_attention_noalloc", "anima_elementwise", "anima_zero", "anima_patchify", "anima_unpatchify",
     "anima_timestep_embedding", "anima_euler_step", "anima_lincomb", "anima_selftest_wait_timeout",
     "anima_ctx_set_attention_split", "anima_ipc_alloc", "anima_ipc_open", "anima_ipc_close", "anima_ipc_free",
-    "anima_peer_barrier", "anima_conv3x3", "anima_channel_norm",
+    "anima_peer_barrier", "anima_conv3x3", "anima_channel_norm", "anima_rotary", "anima_residual_norm",
+    "anima_residual_norm_backward_workspace", "anima_residual_norm_backward",
 ]
 
 
@@ -83,6 +84,28 @@ class AttentionArgs(C.Structure):
                 ("key_len", C.c_void_p), ("scale", C.c_float), ("group", C.c_int), ("causal", C.c_int)]
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("rows", C.c_int), ("D", C.c_int), ("R", C.c_int),
+                ("q", C.c_void_p), ("ldq", C.c_longlong), ("Hq", C.c_int), ("out_q", C.c_void_p), ("ldoq", C.c_longlong),
+                ("k", C.c_void_p), ("ldk", C.c_longlong), ("Hk", C.c_int), ("out_k", C.c_void_p), ("ldok", C.c_longlong),
+                ("inv_freq", C.c_void_p), ("mscale", C.c_float), ("positions", C.c_void_p), ("offset", C.c_longlong),
+                ("rows_per_item", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int)]
+
+
+class ResidualNormArgs(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("rows_per_item", C.c_int),
+                ("x_dtype", C.c_int), ("y_dtype", C.c_int), ("h_dtype", C.c_int), ("post", C.c_int), ("pre", C.c_int),
+                ("alpha", C.c_float), ("eps", C.c_float),
+                ("x", C.c_void_p), ("ldx", C.c_longlong), ("y", C.c_void_p), ("ldy", C.c_longlong),
+                ("x_out", C.c_void_p), ("ldx_out", C.c_longlong), ("h", C.c_void_p), ("ldh", C.c_longlong),
+                ("gate", C.c_void_p), ("ld_gate", C.c_longlong), ("scale", C.c_void_p), ("ld_scale", C.c_longlong),
+                ("shift", C.c_void_p), ("ld_shift", C.c_longlong), ("post_w", C.c_void_p), ("pre_w", C.c_void_p),
+                ("dh", C.c_void_p), ("lddh", C.c_longlong), ("dx_out", C.c_void_p), ("lddx_out", C.c_longlong),
+                ("dx", C.c_void_p), ("lddx", C.c_longlong), ("dy", C.c_void_p), ("lddy", C.c_longlong),
+                ("dgate", C.c_void_p), ("dscale", C.c_void_p), ("dshift", C.c_void_p), ("dpost_w", C.c_void_p),
+                ("dpre_w", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -127,6 +150,10 @@ def load_library(path: str = LIB_PATH):
             "anima_peer_barrier": [vp, C.POINTER(PeerGroup)],
             "anima_conv3x3": [vp, vp, i, i, i, C.POINTER(Weight), i, vp, i],
             "anima_channel_norm": [vp, vp, ll, i, vp, i, vp],
+            "anima_rotary": [vp, C.POINTER(RotaryArgs)],
+            "anima_residual_norm": [vp, C.POINTER(ResidualNormArgs)],
+            "anima_residual_norm_backward_workspace": [vp, C.POINTER(ResidualNormArgs), C.POINTER(sz)],
+            "anima_residual_norm_backward": [vp, C.POINTER(ResidualNormArgs)],
         }
         for name, args in sig.items():
             fn = getattr(lib, name)
@@ -155,7 +182,7 @@ LAUNCHING = set(EXPORTS) - {"anima_ctx_create", "anima_ctx_destroy", "anima_ctx_
                             "anima_last_error", "anima_alloc", "anima_free", "anima_upload", "anima_download",
                             "anima_profile_report", "anima_version", "anima_zero", "anima_selftest_wait_timeout",
                             "anima_ctx_set_attention_split", "anima_ipc_alloc", "anima_ipc_open", "anima_ipc_close",
-                            "anima_ipc_free"}
+                            "anima_ipc_free", "anima_residual_norm_backward_workspace"}
 
 
 class KernelTimer:

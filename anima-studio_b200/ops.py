@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -64,6 +65,30 @@ def _dt(t: torch.Tensor) -> int:
 def _contig_rows(t: torch.Tensor):
     if t.dim() != 2 or t.stride(1) != 1:
         raise dev.AnimaError(1, "expected a 2-D tensor with contiguous rows")
+
+
+def _rows(fn: str, name: str, t: torch.Tensor, rows: int, cols: int, dtype=None, device=None, exact: bool = False):
+    """Refuse what is not `rows` contiguous rows of at least (exact: just) `cols` columns of a kernel type."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or (exact and t.shape[1] != cols):
+        raise dev.AnimaError(1, f"{fn}: {name} is {tuple(t.shape)}, expected [{rows}, {cols}]")
+    if cols and t.stride(1) != 1 and t.shape[1] > 1 or (rows > 1 and t.stride(0) < 0):
+        raise dev.AnimaError(1, f"{fn}: {name} needs contiguous rows (strides {t.stride()})")
+    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
+        raise dev.AnimaError(1, f"{fn}: {name} is {t.dtype}" + (f", expected {dtype}" if dtype is not None else ""))
+    if device is not None and t.device != device:
+        raise dev.AnimaError(1, f"{fn}: {name} is on {t.device}, expected {device}")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of what _rows has let pass (a single row's stride says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(fn: str, name: str, t: torch.Tensor, n: int, dtype, device):
+    """Refuse what is not a dense vector of n elements of `dtype` on `device`."""
+    if t.dim() != 1 or t.numel() != n or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+        raise dev.AnimaError(1, f"{fn}: {name} has to be a dense {dtype} [{n}] on {device}, is {t.dtype} "
+                                f"{tuple(t.shape)} on {t.device}")
 
 
 # ----------------------------------------------------------------------------- rotation / norms
@@ -142,6 +167,193 @@ def rope(x: torch.Tensor, cs: torch.Tensor, L: int, H: int, D: int, row_stride: 
     """In-place split-half RoPE on x viewed as [L, H, D] (ops.js:148-152)."""
     rows = cs.numel() // D
     ctx_for(x).call("anima_rope", ptr(x), _dt(x), L, H, D, row_stride or H * D, col_off, ptr(cs), rows)
+
+
+def rotary_freqs(dim: int, theta: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+                 original_len: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 device="cuda") -> tuple[torch.Tensor, float]:
+    """Inverse frequencies (fp64 [dim / 2]) and output factor for rotary(): theta^(-2i / dim), and for
+    contexts `factor` times the trained original_len
+      "linear"  every frequency divided by factor;
+      "ntk"     theta raised to theta * factor^(dim / (dim - 2)): the slowest pair is stretched by
+                factor, the fastest not at all;
+      "yarn"    pairs that turn more than beta_fast times within original_len stay, those below
+                beta_slow turns are divided by factor, a linear ramp over the turns between; outputs
+                multiplied by 0.1 ln(factor) + 1.
+    No reference counterpart: its RoPE is a table of fixed theta (common.js:26-52)."""
+    if dim < 2 or dim % 2 or not theta > 0 or not factor > 0:
+        raise dev.AnimaError(1, f"rotary_freqs: dim {dim} (even, at least 2), theta {theta}, factor {factor}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise dev.AnimaError(1, f"rotary_freqs: scaling {scaling!r} (None, 'linear', 'ntk' or 'yarn')")
+    if scaling == "ntk" and dim > 2:
+        theta = theta * factor ** (dim / (dim - 2))
+    inv = theta ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    mscale = 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        if not beta_fast > beta_slow or original_len <= 0:
+            raise dev.AnimaError(1, f"rotary_freqs: beta_fast {beta_fast} has to exceed beta_slow {beta_slow}, "
+                                    f"original_len {original_len} be positive")
+        turns = original_len * inv / (2.0 * math.pi)
+        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
+        inv = inv * keep + inv / factor * (1.0 - keep)
+        mscale = 0.1 * math.log(factor) + 1.0
+    return inv.to(device), mscale
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, *, Hq: int, D: int, Hk: int = 0,
+           positions: torch.Tensor | None = None, offset: int = 0, rows_per_item: int | None = None,
+           mscale: float = 1.0, interleaved: bool = False, inverse: bool = False, out_q: torch.Tensor | None = None,
+           out_k: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions on q [rows, >= Hq D] and k [rows, >= Hk D] (or None) in one launch, angles from
+    positions and frequencies (rope() is the table form). The first 2 len(inv_freq) dims of each head
+    are turned and multiplied by mscale (rotary_freqs gives both), in pairs (i, i + R/2), or
+    (2i, 2i + 1) when interleaved; the other dims are copied. Row r stands at positions[r] (int32), or
+    at offset + r % rows_per_item (default: all rows are one item). inverse: the transposed rotation,
+    for gradients. Returns (out_q, out_k), new tensors unless given; out_q may be q itself."""
+    _rows("rotary", "q", q, q.shape[0], Hq * D)
+    rows = q.shape[0]
+    if out_q is None:
+        out_q = torch.empty(rows, Hq * D, dtype=q.dtype, device=q.device)
+    _rows("rotary", "out_q", out_q, rows, Hq * D, q.dtype, q.device)
+    a = dev.RotaryArgs(dtype=_dt(q), rows=rows, D=D, R=2 * inv_freq.numel(), q=q.data_ptr(), ldq=_ld(q), Hq=Hq,
+                       out_q=out_q.data_ptr(), ldoq=_ld(out_q), inv_freq=inv_freq.data_ptr(), mscale=mscale,
+                       offset=offset, rows_per_item=rows_per_item or max(rows, 1), interleaved=interleaved,
+                       inverse=inverse)
+    if k is not None:
+        if out_k is None:
+            out_k = torch.empty(rows, Hk * D, dtype=q.dtype, device=q.device)
+        _rows("rotary", "k", k, rows, Hk * D, q.dtype, q.device)
+        _rows("rotary", "out_k", out_k, rows, Hk * D, q.dtype, q.device)
+        a.k, a.ldk, a.Hk, a.out_k, a.ldok = k.data_ptr(), _ld(k), Hk, out_k.data_ptr(), _ld(out_k)
+    elif Hk or out_k is not None:
+        raise dev.AnimaError(1, "rotary: Hk or out_k without k")
+    _vector("rotary", "inv_freq", inv_freq, inv_freq.numel(), torch.float64, q.device)
+    if positions is not None:
+        _vector("rotary", "positions", positions, rows, torch.int32, q.device)
+        a.positions = positions.data_ptr()
+    ctx_for(q).call("anima_rotary", C.byref(a))
+    return out_q, out_k
+
+
+NORM_KIND = {None: 0, "rms": 1, "layer": 2}
+
+
+def _residual_norm_args(fn, x, y, alpha, gate, post, post_w, pre, pre_w, scale, shift, eps, rows_per_item):
+    """The arguments that the forward and the backward share; x: the residual stream's tensor."""
+    if post not in NORM_KIND or pre not in ("rms", "layer"):
+        raise dev.AnimaError(1, f"{fn}: post {post!r} (None, 'rms' or 'layer'), pre {pre!r} ('rms' or 'layer')")
+    if x.dim() != 2:
+        raise dev.AnimaError(1, f"{fn}: x has to be a 2-D tensor of rows")
+    rows, cols = x.shape
+    _rows(fn, "y", y, rows, cols, None, x.device, exact=True)
+    L = rows_per_item or max(rows, 1)
+    a = dev.ResidualNormArgs(rows=rows, cols=cols, rows_per_item=L, x_dtype=_dt(x), y_dtype=_dt(y), post=NORM_KIND[post],
+                             pre=NORM_KIND[pre], alpha=alpha, eps=eps, y=y.data_ptr(), ldy=_ld(y))
+    items = rows // L
+    for name, m in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if m is None:
+            continue
+        if m.dim() == 1:
+            _vector(fn, name, m, cols, torch.float32, x.device)
+            if items > 1:
+                raise dev.AnimaError(1, f"{fn}: {name} [{cols}] for {items} items of rows (a [items, cols] tensor)")
+            ld = cols
+        else:
+            _rows(fn, name, m, items, cols, torch.float32, x.device, exact=True)
+            ld = _ld(m)
+        setattr(a, name, m.data_ptr())
+        setattr(a, "ld_" + name, ld)
+    for name, w in (("post_w", post_w), ("pre_w", pre_w)):
+        if w is not None:
+            _vector(fn, name, w, cols, torch.float32, x.device)
+            setattr(a, name, w.data_ptr())
+    return a
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, *, alpha: float = 1.0, gate: torch.Tensor | None = None,
+                  post: str | None = None, post_w: torch.Tensor | None = None, pre: str = "layer",
+                  pre_w: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                  shift: torch.Tensor | None = None, eps: float = 1e-6, rows_per_item: int | None = None, out_dtype=None,
+                  x_out: torch.Tensor | None = None, h: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The step from one sublayer to the next in one pass: u = post(y) * post_w, x_out = x + alpha *
+    gate * u, h = pre(x_out) * pre_w * (1 + scale) + shift; returns (x_out, h). x, y [rows, cols], each
+    fp32, bf16 or fp16; post: None, "rms" or "layer"; pre: "rms" or "layer"; gate, scale, shift: fp32
+    [items, cols] (rows may be strided: slices of a modulation tensor) or [cols] for one item, row r
+    taking those of item r // rows_per_item; post_w, pre_w: fp32 [cols]. h has out_dtype (default
+    x's). x_out may be x itself. The reference runs the gate and the adaLN norm apart (dit.js:261-314)."""
+    fn = "residual_norm"
+    a = _residual_norm_args(fn, x, y, alpha, gate, post, post_w, pre, pre_w, scale, shift, eps, rows_per_item)
+    _rows(fn, "x", x, a.rows, a.cols)
+    if x_out is None:
+        x_out = torch.empty(a.rows, a.cols, dtype=x.dtype, device=x.device)
+    if h is None:
+        h = torch.empty(a.rows, a.cols, dtype=out_dtype or x.dtype, device=x.device)
+    elif out_dtype not in (None, h.dtype):
+        raise dev.AnimaError(1, f"{fn}: h is {h.dtype}, out_dtype {out_dtype}")
+    _rows(fn, "x_out", x_out, a.rows, a.cols, x.dtype, x.device, exact=True)
+    _rows(fn, "h", h, a.rows, a.cols, None, x.device, exact=True)
+    a.h_dtype = _dt(h)
+    a.x, a.ldx, a.x_out, a.ldx_out = x.data_ptr(), _ld(x), x_out.data_ptr(), _ld(x_out)
+    a.h, a.ldh = h.data_ptr(), _ld(h)
+    ctx_for(x).call("anima_residual_norm", C.byref(a))
+    return x_out, h
+
+
+class ResidualNormGrads(NamedTuple):
+    """Gradients of residual_norm's inputs; None where the parameter is None. dgate, dscale and dshift
+    have one row per item (the caller sums them where it gave several items one vector)."""
+
+    dx: torch.Tensor
+    dy: torch.Tensor
+    dgate: torch.Tensor | None
+    dpost_w: torch.Tensor | None
+    dpre_w: torch.Tensor | None
+    dscale: torch.Tensor | None
+    dshift: torch.Tensor | None
+
+
+def residual_norm_backward(dh: torch.Tensor, dx_out: torch.Tensor | None, x_out: torch.Tensor, y: torch.Tensor, *,
+                           alpha: float = 1.0, gate: torch.Tensor | None = None, post: str | None = None,
+                           post_w: torch.Tensor | None = None, pre: str = "layer", pre_w: torch.Tensor | None = None,
+                           scale: torch.Tensor | None = None, shift: torch.Tensor | None = None, eps: float = 1e-6,
+                           rows_per_item: int | None = None, dx: torch.Tensor | None = None,
+                           dy: torch.Tensor | None = None) -> ResidualNormGrads:
+    """The backward pass of residual_norm: dh is the gradient of h, dx_out the gradient that reaches
+    x_out from behind (None: none), x_out and y are as the forward left and had them, the rest are the
+    forward's arguments. dx (x's type) may be dx_out itself, dy (y's type) y itself. Statistics are
+    computed again in fp32 from y and the stored x_out; column sums are in fp32 and of fixed order."""
+    fn = "residual_norm_backward"
+    a = _residual_norm_args(fn, x_out, y, alpha, gate, post, post_w, pre, pre_w, scale, shift, eps, rows_per_item)
+    rows, cols, dv = a.rows, a.cols, x_out.device
+    _rows(fn, "x_out", x_out, rows, cols)
+    _rows(fn, "dh", dh, rows, cols, None, dv, exact=True)
+    dx = torch.empty(rows, cols, dtype=x_out.dtype, device=dv) if dx is None else dx
+    dy = torch.empty(rows, cols, dtype=y.dtype, device=dv) if dy is None else dy
+    _rows(fn, "dx", dx, rows, cols, x_out.dtype, dv, exact=True)
+    _rows(fn, "dy", dy, rows, cols, y.dtype, dv, exact=True)
+    a.x_out, a.ldx_out, a.h_dtype = x_out.data_ptr(), _ld(x_out), _dt(dh)
+    a.dh, a.lddh, a.dx, a.lddx, a.dy, a.lddy = (dh.data_ptr(), _ld(dh), dx.data_ptr(), _ld(dx), dy.data_ptr(),
+                                                _ld(dy))
+    if dx_out is not None:
+        _rows(fn, "dx_out", dx_out, rows, cols, x_out.dtype, dv, exact=True)
+        a.dx_out, a.lddx_out = dx_out.data_ptr(), _ld(dx_out)
+    grads = {}
+    for name, t in (("gate", gate), ("post_w", post_w), ("pre_w", pre_w), ("scale", scale), ("shift", shift)):
+        g = None
+        if t is not None:
+            g = (torch.empty if rows else torch.zeros)(t.shape, dtype=torch.float32, device=dv)
+            setattr(a, "d" + name, g.data_ptr())
+        grads["d" + name] = g
+    ctx = ctx_for(x_out)
+    need = C.c_size_t()
+    dev.check(ctx.lib.anima_residual_norm_backward_workspace(ctx.h, C.byref(a), C.byref(need)))
+    if need.value:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dv)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+    ctx.call("anima_residual_norm_backward", C.byref(a), kernels=2 if need.value else 1)
+    return ResidualNormGrads(dx, dy, **grads)
 
 
 def elementwise(op: str, a: torch.Tensor, b: torch.Tensor | None = None, out: torch.Tensor | None = None):

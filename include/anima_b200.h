@@ -219,6 +219,69 @@ int anima_qk_norm_rope(anima_ctx* ctx, void* qkv, int dtype, int L, int H, int D
 /* ops.rope (ops.js:148-152, kernels.js:336-357), in place on x viewed as [L, H, D] at colOff. */
 int anima_rope(anima_ctx* ctx, void* x, int dtype, int L, int H, int D, int row_stride, int col_off,
                const float* rope, int rope_rows);
+/* Rotary positions on q and k in one call, from positions and frequencies instead of a table
+ * (anima_rope is the table form). Of each head's D dims the first R are turned, in pairs (i, i + R/2),
+ * or (2i, 2i + 1) when interleaved; the rest is copied. Pair i at position p turns by
+ * p * inv_freq[i], computed in 64 bits, and is multiplied by mscale (1, or the factor that a scheme for
+ * long contexts asks for); inverse != 0 turns back, which maps the gradient of the outputs to that of
+ * the inputs. p = positions[row], or offset + row % rows_per_item where positions is NULL. An output may
+ * be its input (same pointer and stride); otherwise they must not overlap. Either side may have 0 heads. */
+typedef struct {
+  int dtype;               /* F32, BF16 or F16, of q, k and their outputs */
+  int rows, D, R;
+  const void* q; long long ldq; int Hq;
+  void* out_q; long long ldoq;
+  const void* k; long long ldk; int Hk;
+  void* out_k; long long ldok;
+  const double* inv_freq;  /* [R / 2] */
+  float mscale;
+  const int* positions;    /* [rows] or NULL */
+  long long offset;
+  int rows_per_item;
+  int interleaved, inverse;
+} anima_rotary_args;
+int anima_rotary(anima_ctx* ctx, const anima_rotary_args* a);
+
+/* The step between two sublayers in one pass over the rows: post-norm of the block's output y, gate and
+ * residual scale, the residual add, and the next block's pre-norm with its modulation:
+ *   u = post_norm(y) * post_w;  x_out = x + alpha * gate[item] * u;
+ *   h = pre_norm(x_out) * pre_w * (1 + scale[item]) + shift[item]
+ * with item = row / rows_per_item, norms over the row in fp32 (h is computed from x_out before it is
+ * rounded). Every fp32 parameter (gate, scale, shift [items, cols] with their row strides; post_w, pre_w
+ * [cols]) may be NULL: 1, 0, 0, 1, 1. x_out may be x. At most 4096 columns.
+ * The backward call takes dh, the gradient of h, and dx_out, the gradient that reaches x_out from
+ * behind (NULL: none), with x_out and y as the forward left and had them, and writes dx and dy and
+ * whichever of the parameters' gradients are not NULL (dgate, dscale, dshift [items, cols] dense;
+ * dpost_w, dpre_w [cols]; fp32; sums of fixed order, so the same inputs give the same bits). dx may be
+ * dx_out, dy may be y. Its workspace (device memory of the caller, 16-byte aligned, free again when
+ * the call's work is done) has to hold anima_residual_norm_backward_workspace bytes for the same args.
+ * With 0 rows nothing is written. */
+typedef struct {
+  int rows, cols, rows_per_item;
+  int x_dtype, y_dtype, h_dtype; /* F32, BF16 or F16: of x, x_out and their gradients; y, dy; h, dh */
+  int post, pre;                 /* 0 none (post only), 1 rms, 2 layer */
+  float alpha, eps;
+  const void* x; long long ldx;  /* forward only */
+  const void* y; long long ldy;
+  void* x_out; long long ldx_out; /* written by the forward, read by the backward */
+  void* h; long long ldh;         /* forward only */
+  const float* gate; long long ld_gate;
+  const float* scale; long long ld_scale;
+  const float* shift; long long ld_shift;
+  const float* post_w;
+  const float* pre_w;
+  /* backward only */
+  const void* dh; long long lddh;
+  const void* dx_out; long long lddx_out;
+  void* dx; long long lddx;
+  void* dy; long long lddy;
+  float *dgate, *dscale, *dshift, *dpost_w, *dpre_w;
+  void* workspace; size_t workspace_bytes;
+} anima_residual_norm_args;
+int anima_residual_norm(anima_ctx* ctx, const anima_residual_norm_args* a);
+int anima_residual_norm_backward_workspace(anima_ctx* ctx, const anima_residual_norm_args* a, size_t* bytes);
+int anima_residual_norm_backward(anima_ctx* ctx, const anima_residual_norm_args* a);
+
 /* ops.attention (ops.js:166-208, kernels.js:147-299): multi-head attention with fp32 softmax.
  * head_dim 128 with bf16/fp16 q/k/v (the DiT's attentions; the Qwen3 text encoder's, causal with
  * grouped k/v heads): the tcgen05 flash kernel. fp32 q/k/v with one wide head (head_dim a multiple

@@ -1,0 +1,127 @@
+"""CPU tests of the trained block's operators: frequencies, refusals, the C structs' layout."""
+
+import ctypes
+import math
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+from tests.conftest import ROOT, pkg
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return pkg("ops")
+
+
+@pytest.fixture(scope="module")
+def err():
+    return pkg("device").AnimaError
+
+
+def test_structs_match_the_c_header(tmp_path):
+    dev = pkg("device")
+    structs = {"anima_rotary_args": dev.RotaryArgs, "anima_residual_norm_args": dev.ResidualNormArgs}
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "anima_b200.h"', "int main(void) {"]
+    for cname, cls in structs.items():
+        lines.append(f'  printf("{cname} sizeof %zu\\n", sizeof({cname}));')
+        lines += [f'  printf("{cname} {f} %zu\\n", offsetof({cname}, {f}));' for f, *_ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    subprocess.run([cc, "-std=c11", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split("\n")
+    got = {(a, b): int(c) for a, b, c in (ln.split() for ln in out if ln)}
+    for cname, cls in structs.items():
+        assert got[(cname, "sizeof")] == ctypes.sizeof(cls), cname
+        for f, *_ in cls._fields_:
+            assert got[(cname, f)] == getattr(cls, f).offset, (cname, f)
+
+
+# ----------------------------------------------------------------------------- frequencies
+
+def test_rotary_freqs(ops):
+    plain, m = ops.rotary_freqs(128, 1e6, device="cpu")
+    assert m == 1.0 and plain.dtype == torch.float64
+    for i in (0, 1, 63):
+        assert math.isclose(plain[i].item(), 1e6 ** (-2 * i / 128), rel_tol=1e-14)
+    lin, _ = ops.rotary_freqs(128, 1e6, scaling="linear", factor=4.0, device="cpu")
+    assert torch.equal(lin, plain / 4)
+    ntk, _ = ops.rotary_freqs(128, 1e6, scaling="ntk", factor=4.0, device="cpu")
+    assert ntk[0] == 1.0 and math.isclose((plain[63] / ntk[63]).item(), 4.0, rel_tol=1e-12)
+    yarn, m = ops.rotary_freqs(128, 1e4, scaling="yarn", factor=8.0, original_len=4096, device="cpu")
+    plain, _ = ops.rotary_freqs(128, 1e4, device="cpu")
+    assert math.isclose(m, 0.1 * math.log(8.0) + 1.0)
+    turns = 4096 * plain / (2 * math.pi)
+    assert torch.equal(yarn[turns >= 32], plain[turns >= 32])
+    torch.testing.assert_close(yarn[turns <= 1], plain[turns <= 1] / 8, rtol=1e-14, atol=0)
+    mid = (turns > 1) & (turns < 32)
+    assert mid.any() and bool(((yarn < plain) & (yarn > plain / 8))[mid].all())
+
+
+@pytest.mark.parametrize("kw", [dict(dim=0), dict(dim=7), dict(dim=8, theta=0.0), dict(dim=8, factor=-1.0),
+                                dict(dim=8, scaling="cubic"), dict(dim=8, scaling="yarn", beta_fast=1.0),
+                                dict(dim=8, scaling="yarn", original_len=0)])
+def test_rotary_freqs_refuses(ops, err, kw):
+    with pytest.raises(err):
+        ops.rotary_freqs(device="cpu", **kw)
+
+
+# ----------------------------------------------------------------------------- refusals
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=t(5, 63)), dict(q=t(320)), dict(q=t(64, 5).T), dict(q=t(5, 64, dtype=torch.float64)),
+    dict(k=t(4, 32)), dict(k=t(5, 31)), dict(k=t(5, 32, dtype=torch.bfloat16)), dict(k=None),
+    dict(positions=t(5, dtype=torch.int64)), dict(positions=t(4, dtype=torch.int32)),
+    dict(positions=torch.zeros(10, dtype=torch.int32)[::2]), dict(inv_freq=t(8)),
+    dict(inv_freq=t(2, 4, dtype=torch.float64)), dict(out_q=t(5, 64, dtype=torch.float16)), dict(out_q=t(6, 64)),
+    dict(out_k=t(5, 16)),
+])
+def test_rotary_refuses(ops, err, change):
+    kw = dict(q=t(5, 64), k=t(5, 32), inv_freq=t(8, dtype=torch.float64), Hq=4, Hk=2, D=16)
+    with pytest.raises(err) as e:
+        ops.rotary(**{**kw, **change})
+    assert e.value.status == 1
+
+
+def test_no_cpu_path(ops, err):
+    with pytest.raises(err) as e:
+        ops.rotary(t(5, 64), t(5, 32), t(8, dtype=torch.float64), Hq=4, Hk=2, D=16)
+    assert e.value.status == -1
+    with pytest.raises(err) as e:
+        ops.residual_norm(t(6, 16), t(6, 16))
+    assert e.value.status == -1
+
+
+NORM_BAD = [
+    dict(y=t(5, 16)), dict(y=t(6, 15)), dict(y=t(16, 6).T), dict(y=t(6, 16, dtype=torch.float64)), dict(post="max"),
+    dict(pre=None), dict(gate=t(16)), dict(gate=t(3, 16)), dict(scale=t(2, 15)), dict(shift=t(2, 16, dtype=torch.float16)),
+    dict(pre_w=t(15)), dict(post_w=t(2, 8), post="rms"),
+]
+
+
+@pytest.mark.parametrize("change", NORM_BAD + [dict(x=t(6, 16, 1)), dict(x_out=t(6, 16, dtype=torch.float16)),
+                                               dict(h=t(5, 16)), dict(h=t(6, 16), out_dtype=torch.float16)])
+def test_residual_norm_refuses(ops, err, change):
+    kw = dict(x=t(6, 16), y=t(6, 16), rows_per_item=3, gate=t(2, 16))
+    with pytest.raises(err) as e:
+        ops.residual_norm(**{**kw, **change})
+    assert e.value.status == 1
+
+
+@pytest.mark.parametrize("change", NORM_BAD + [dict(dh=t(6, 15)), dict(dx_out=t(6, 16, dtype=torch.float16)),
+                                               dict(dx=t(5, 16)), dict(dy=t(6, 16, dtype=torch.bfloat16))])
+def test_residual_norm_backward_refuses(ops, err, change):
+    kw = dict(dh=t(6, 16), dx_out=t(6, 16), x_out=t(6, 16), y=t(6, 16), rows_per_item=3, gate=t(2, 16))
+    with pytest.raises(err) as e:
+        ops.residual_norm_backward(**{**kw, **change})
+    assert e.value.status == 1
