@@ -8,3 +8,4 @@
 #include "vae.cu"
 #include "rotary.cu"
 #include "resnorm.cu"
+#include "attention_grad.cu"

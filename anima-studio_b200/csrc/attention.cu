@@ -33,11 +33,11 @@ namespace anima {
 namespace attn {
 
 constexpr int TILE = 128;     // query rows per tile and keys per block
-constexpr int HD = 128;       // head dim
 constexpr int THREADS = 576;
 constexpr int SOFTMAX_WARPS = 16;
 constexpr int ATOM = 16384;   // one SWIZZLE_128B atom column: 128 rows x 128 bytes
-constexpr int TILE_BYTES = 2 * ATOM;
+constexpr int TILE_BYTES = 2 * ATOM;  // a tile's slot: head_dim 128; at 64 half of it is used
+constexpr int MAX_HD = 128;
 // shared memory: Q_A | Q_B | K[2] | V[2] | barriers
 constexpr int OFF_Q = 0;
 constexpr int OFF_K = OFF_Q + 2 * TILE_BYTES;
@@ -64,6 +64,8 @@ struct Params {
   int persist;       // whole units, CTA c taking units c, c + grid, ... (grid = SM count)
   int group;         // q heads per k/v head (k/v head = h / group)
   int causal;        // key j visible to query i only when j <= i
+  int zero_tail;     // key_len given: V's rows past it are zeroed before P V (0 x NaN is not 0)
+  float* lse;        // [batch][heads][Lq] ln of each row's sum of exponentials, or NULL
   float* ws;         // [units][PART_FLOATS] partial softmax states of split units
   unsigned* flags;   // [units] tail part written (cleared by the head part)
 };
@@ -136,8 +138,8 @@ struct Seg {
 constexpr int kWhole = 0, kHeadPart = 1, kTailPart = 2;
 // workspace slot: O of both tiles as float4 [tile][half][16 column quads][128 rows], then the max
 // and the row sum [tile][half][128 rows] each
-constexpr int PART_FLOATS = 2 * TILE * HD + 2 * 2 * 2 * TILE;
-constexpr int PART_M = 2 * TILE * HD;
+constexpr int PART_FLOATS = 2 * TILE * MAX_HD + 2 * 2 * 2 * TILE;
+constexpr int PART_M = 2 * TILE * MAX_HD;
 constexpr int PART_L = PART_M + 2 * 2 * TILE;
 
 __device__ __forceinline__ Seg segment_at(const Params& p, long long g, long long end) {
@@ -196,11 +198,19 @@ __device__ __forceinline__ void st_release_u32(unsigned* q, unsigned v) {
   asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(q), "r"(v) : "memory");
 }
 
+// Row statistic of the backward pass: ln sum_j exp(scale q.k_j), from the maximum m (log2 units) and
+// the row sum l relative to it; -inf where the row saw no key.
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
 // 18 warps are allocated registers as 20: 96 x 32 x 20 = 61440 of the SM's 65536
-template <bool BF16>
+template <bool BF16, int HD>
 __global__ void __launch_bounds__(THREADS, 1)
     attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  static_assert(HD == 64 || HD == 128, "one or two 64-column atoms a row");
+  constexpr int ATOMS = HD / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
@@ -268,11 +278,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int q0 = qp * 2 * TILE;
         const int qc = p.q_col + h * HD, kc = p.k_col + (h / p.group) * HD, vc = p.v_col + (h / p.group) * HD;
         if (qn > 0 && !mbar_wait(q_empty, (qn - 1) & 1, abort_flag, kErrTimeoutEmpty)) break;
-        mbar_arrive_expect_tx(q_full, 2 * TILE_BYTES);
-        tma_load_3d(smem + OFF_Q, &tm_q, q_full, qc, q0, b);
-        tma_load_3d(smem + OFF_Q + ATOM, &tm_q, q_full, qc + 64, q0, b);
-        tma_load_3d(smem + OFF_Q + TILE_BYTES, &tm_q, q_full, qc, q0 + TILE, b);
-        tma_load_3d(smem + OFF_Q + TILE_BYTES + ATOM, &tm_q, q_full, qc + 64, q0 + TILE, b);
+        mbar_arrive_expect_tx(q_full, 2 * ATOMS * ATOM);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int t = 0; t < ATOMS; ++t)
+            tma_load_3d(smem + OFF_Q + x * TILE_BYTES + t * ATOM, &tm_q, q_full, qc + 64 * t, q0 + x * TILE, b);
         arm(0, qn & 1);
         ++qn;
         for (int j = 0; j < nb; ++j) {
@@ -280,14 +291,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int st = G & 1;
           const uint32_t ph = (G >> 1) & 1;
           if (!mbar_wait(&k_empty[st], ph ^ 1, abort_flag, kErrTimeoutEmpty)) break;
-          mbar_arrive_expect_tx(&k_full[st], TILE_BYTES);
-          tma_load_3d(smem + OFF_K + st * TILE_BYTES, &tm_k, &k_full[st], kc, kb * TILE, kvb);
-          tma_load_3d(smem + OFF_K + st * TILE_BYTES + ATOM, &tm_k, &k_full[st], kc + 64, kb * TILE, kvb);
+          mbar_arrive_expect_tx(&k_full[st], ATOMS * ATOM);
+#pragma unroll
+          for (int t = 0; t < ATOMS; ++t)
+            tma_load_3d(smem + OFF_K + st * TILE_BYTES + t * ATOM, &tm_k, &k_full[st], kc + 64 * t, kb * TILE, kvb);
           arm(1 + st, ph);
           if (!mbar_wait(&v_empty[st], ph ^ 1, abort_flag, kErrTimeoutEmpty)) break;
-          mbar_arrive_expect_tx(&v_full[st], TILE_BYTES);
-          tma_load_3d(smem + OFF_V + st * TILE_BYTES, &tm_v, &v_full[st], vc, kb * TILE, kvb);
-          tma_load_3d(smem + OFF_V + st * TILE_BYTES + ATOM, &tm_v, &v_full[st], vc + 64, kb * TILE, kvb);
+          mbar_arrive_expect_tx(&v_full[st], ATOMS * ATOM);
+#pragma unroll
+          for (int t = 0; t < ATOMS; ++t)
+            tma_load_3d(smem + OFF_V + st * TILE_BYTES + t * ATOM, &tm_v, &v_full[st], vc + 64 * t, kb * TILE, kvb);
           arm(3 + st, ph);
         }
         gb += nb;
@@ -402,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + x * 128 + 64 * hf;  // fp32 scores of this half
     const uint32_t p_addr = tmem + lane_addr + x * 128 + 32 * hf;  // its 64 probabilities, 2 per column
-    const uint32_t o_addr = tmem + lane_addr + 256 + x * 128 + 64 * hf;
+    const uint32_t o_addr = tmem + lane_addr + 256 + x * 128 + (HD / 2) * hf;  // its half of O's columns
     float* red = reinterpret_cast<float*>(smem + OFF_RED);      // [parity][tile][half][row]
     float* red_l = reinterpret_cast<float*>(smem + OFF_RED_L);  // [tile][half][row]
     const int bar_id = 1 + x * 4 + quad;                        // named barrier of the two warps of a row
@@ -424,7 +437,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int h = bh % p.heads, b = bh / p.heads;
         qrow = qp * 2 * TILE + x * TILE + row;
         return static_cast<size_t>(b) * p.o_bstride + static_cast<size_t>(qrow) * p.ldo + static_cast<size_t>(h) * HD +
-               64 * hf;
+               (HD / 2) * hf;
+      };
+      auto put_lse = [&](int qrow, float v) {  // one of a row's two warps
+        if (p.lse && hf == 0 && qrow < p.Lq) p.lse[static_cast<size_t>(segs[si].x / p.q_pairs) * p.Lq + qrow] = v;
       };
       if (nb <= 0) {
         int qrow;
@@ -433,8 +449,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (qrow < p.Lq) {
           const int esz = p.out_dtype == ANIMA_F32 ? 4 : 2;
           uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + obase * esz);
-          for (int t = 0; t < 64 * esz / 16; ++t) dst[t] = make_uint4(0, 0, 0, 0);
+          for (int t = 0; t < (HD / 2) * esz / 16; ++t) dst[t] = make_uint4(0, 0, 0, 0);
         }
+        put_lse(qrow, -INFINITY);
         continue;
       }
       float m_used = -INFINITY;  // max the probabilities (and O, l) are relative to
@@ -523,13 +540,29 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < ATOMS; ++c) {
             uint32_t orr[32];
             tmem_ld32(o_addr + 32 * c, orr);
             tmem_ld_wait(orr);
 #pragma unroll
             for (int t = 0; t < 32; ++t) orr[t] = __float_as_uint(__uint_as_float(orr[t]) * alpha);
             tmem_st32(o_addr + 32 * c, orr);
+          }
+        }
+        if (p.zero_tail && masked) {
+          // the block that key_len ends in: what lies behind may be anything, and the tensor core
+          // multiplies it by P = 0. Each tile's warps clear all of V's hidden rows before their P V.
+          const int left = min(p.Lk, p.key_len[p.kv_bcast ? 0 : segs[si].x / p.q_pairs / p.heads]) - (kb0 + j) * TILE;
+          if (left < TILE) {
+            if (!warp_wait(&v_full[jp], (G >> 1) & 1, abort_flag, kErrTimeoutFull)) {
+              ok = false;
+              continue;
+            }
+            const int n = (TILE - left) * 8;  // 16-byte pieces of an atom's rows
+            for (int t = (warp & 7) * 32 + lane; t < n * ATOMS; t += 256)
+              *reinterpret_cast<uint4*>(smem + OFF_V + jp * TILE_BYTES + (t / n) * ATOM + left * 128 + (t % n) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
           }
         }
         tmem_st_wait();
@@ -556,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         float* slot = p.ws + static_cast<size_t>(blockIdx.x) * PART_FLOATS;
         float4* po = reinterpret_cast<float4*>(slot) + (x * 2 + hf) * 16 * TILE + row;
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < ATOMS; ++c) {
           uint32_t orr[32];
           tmem_ld32(o_addr + 32 * c, orr);
           tmem_ld_wait(orr);
@@ -573,6 +606,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         continue;
       }
       float fa = 1.f, fb = 0.f, inv = l_row > 0.f ? 1.0f / l_row : 0.f;
+      float m_row = m_used, l_all = l_row;
       const float4* pb = nullptr;
       if (kind == kTailPart) {
         // wait (bounded) for the head part's partial from the previous CTA, then merge
@@ -608,12 +642,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         fb = ex2(mb - m);
         const float lt = l_row * fa + lb * fb;
         inv = lt > 0.f ? 1.0f / lt : 0.f;
+        m_row = m;
+        l_all = lt;
         pb = reinterpret_cast<const float4*>(slot) + (x * 2 + hf) * 16 * TILE + row;
       }
       int qrow;
       const size_t obase = out_base(qrow);
+      put_lse(qrow, row_lse(m_row, l_all));
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < ATOMS; ++c) {
         uint32_t orr[32];
         tmem_ld32(o_addr + 32 * c, orr);
         tmem_ld_wait(orr);
@@ -945,9 +982,24 @@ int text_attention(anima_ctx* ctx, const anima_attention_args* a, int group) {
   return check_launch("text_attention_kernel");
 }
 
-// static_ws: the stream-K workspace comes from the module's static device array (no allocation)
-// instead of the context's lazily allocated one.
-int attention_launch(anima_ctx* ctx, const anima_attention_args* a, bool static_ws) {
+// Where the stream-K workspace comes from: the context's (allocated on first use), the module's static
+// device array (no allocation), or the caller, whose flags are cleared before the launch.
+struct Scratch {
+  bool static_ws = false;
+  bool callers = false;
+  void* ws = nullptr;
+  size_t bytes = 0;
+};
+constexpr size_t callers_flag_bytes(int sms) {
+  return (static_cast<size_t>(sms) * attn::SOFTMAX_WARPS * sizeof(unsigned) + 255) / 256 * 256;
+}
+constexpr size_t callers_bytes(int sms) {
+  return callers_flag_bytes(sms) + static_cast<size_t>(sms) * attn::PART_FLOATS * sizeof(float);
+}
+
+// lse: row statistics wanted (then head_dim 64 takes the tensor cores too, and nothing else runs).
+int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratch& scratch, float* lse) {
+  const bool static_ws = scratch.static_ws;
   ANIMA_REQUIRE(ctx && a, "anima_attention: NULL argument");
   ANIMA_ON_DEVICE(ctx);
   ANIMA_REQUIRE(a->out_dtype == ANIMA_F32 || a->out_dtype == ANIMA_BF16 || a->out_dtype == ANIMA_F16,
@@ -955,8 +1007,12 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, bool static_
   ANIMA_REQUIRE(a->batch > 0 && a->heads > 0 && a->Lq > 0 && a->Lk > 0, "anima_attention: empty problem");
   ANIMA_REQUIRE(a->q && a->k && a->v && a->out, "anima_attention: NULL data pointer");
   const int group = a->group > 1 ? a->group : 1;
-  if (attention_planes_ok(a)) return attention_planes(ctx, a);  // the VAE's wide single head
-  if (a->head_dim != attn::HD || a->dtype == ANIMA_F32 || a->heads % group != 0) {
+  if (lse) {
+    ANIMA_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "anima_attention_lse: head_dim %d (64 or 128)", a->head_dim);
+    ANIMA_REQUIRE(a->heads % group == 0, "anima_attention_lse: %d heads do not form groups of %d", a->heads, group);
+  }
+  if (!lse && attention_planes_ok(a)) return attention_planes(ctx, a);  // the VAE's wide single head
+  if (!lse && (a->head_dim != 128 || a->dtype == ANIMA_F32 || a->heads % group != 0)) {
     ANIMA_REQUIRE(a->dtype == ANIMA_F32 || a->dtype == ANIMA_BF16 || a->dtype == ANIMA_F16,
                   "anima_attention: q/k/v dtype %d", a->dtype);
     return text_attention(ctx, a, group);  // no workspace either way
@@ -978,6 +1034,8 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, bool static_
   const int kv_batch = kv_bcast ? 1 : a->batch;
   ANIMA_REQUIRE(a->ldo >= static_cast<long long>(a->heads) * a->head_dim && a->ldo % 8 == 0,
                 "anima_attention: bad output stride");
+  ANIMA_REQUIRE(reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && (a->batch == 1 || a->o_bstride % 8 == 0),
+                "anima_attention: the output has to be 16-byte aligned, its batch stride a multiple of 8");
 
   // 3D maps (cols, rows, batch) over each operand; the box is 64 columns x 128 rows.
   CUtensorMap tq, tk, tv;
@@ -1017,6 +1075,8 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, bool static_
   p.o_bstride = a->batch > 1 ? a->o_bstride : 0;
   p.out_dtype = a->out_dtype;
   p.key_len = a->key_len;
+  p.zero_tail = a->key_len ? 1 : 0;
+  p.lse = lse;
   p.kv_bcast = kv_bcast ? 1 : 0;
   p.group = group;
   p.causal = a->causal ? 1 : 0;
@@ -1029,7 +1089,15 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, bool static_
   p.ublk = (a->Lk + attn::TILE - 1) / attn::TILE;
   long long grid = units;
   if (attn::use_stream_k(ctx, a, units, p.ublk)) {
-    if (static_ws) {
+    if (scratch.callers) {
+      ANIMA_REQUIRE(scratch.ws && scratch.bytes >= callers_bytes(ctx->num_sms) &&
+                        reinterpret_cast<uintptr_t>(scratch.ws) % 256 == 0,
+                    "anima_attention_lse: a workspace of %zu bytes (256-byte aligned) is needed, %zu are given",
+                    callers_bytes(ctx->num_sms), scratch.ws ? scratch.bytes : 0);
+      ANIMA_CUDA(cudaMemsetAsync(scratch.ws, 0, callers_flag_bytes(ctx->num_sms), ctx->stream));
+      p.flags = static_cast<unsigned*>(scratch.ws);
+      p.ws = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch.ws) + callers_flag_bytes(ctx->num_sms));
+    } else if (static_ws) {
       int st = attn::static_scratch(ctx);
       if (st) return st;
       p.flags = static_cast<unsigned*>(ctx->attn_static_ws);
@@ -1052,8 +1120,9 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, bool static_
                  4.0 * a->batch * a->heads * static_cast<double>(a->Lq) * a->Lk * a->head_dim, 0);
   using Kfn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const attn::Params);
   const int kind = a->dtype == ANIMA_BF16 ? 1 : 0;
-  const Kfn fns[2] = {attn::attention_kernel<false>, attn::attention_kernel<true>};
-  const Kfn fn = fns[kind];
+  const Kfn fns[2][2] = {{attn::attention_kernel<false, 128>, attn::attention_kernel<true, 128>},
+                         {attn::attention_kernel<false, 64>, attn::attention_kernel<true, 64>}};
+  const Kfn fn = fns[a->head_dim == 64][kind];
   {
     int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), attn::SMEM_BYTES);
     if (st) return st;
@@ -1065,9 +1134,31 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, bool static_
 }  // namespace
 
 extern "C" int anima_attention(anima_ctx* ctx, const anima_attention_args* a) {
-  return attention_launch(ctx, a, false);
+  return attention_launch(ctx, a, Scratch{}, nullptr);
 }
 
 extern "C" int anima_attention_noalloc(anima_ctx* ctx, const anima_attention_args* a) {
-  return attention_launch(ctx, a, true);
+  Scratch s;
+  s.static_ws = true;
+  return attention_launch(ctx, a, s, nullptr);
+}
+
+extern "C" int anima_attention_lse_workspace(anima_ctx* ctx, const anima_attention_args* a, size_t* bytes) {
+  ANIMA_REQUIRE(ctx && a && bytes, "anima_attention_lse_workspace: NULL argument");
+  ANIMA_REQUIRE(a->batch > 0 && a->heads > 0 && a->Lq > 0 && a->Lk > 0, "anima_attention_lse_workspace: empty problem");
+  const long long pairs = (a->Lq + 2LL * attn::TILE - 1) / (2 * attn::TILE);
+  *bytes = attn::use_stream_k(ctx, a, pairs * a->heads * a->batch, (a->Lk + attn::TILE - 1) / attn::TILE)
+               ? callers_bytes(ctx->num_sms)
+               : 0;
+  return ANIMA_OK;
+}
+
+extern "C" int anima_attention_lse(anima_ctx* ctx, const anima_attention_args* a, float* lse, void* workspace,
+                                   size_t workspace_bytes) {
+  ANIMA_REQUIRE(lse, "anima_attention_lse: lse is NULL");
+  Scratch s;
+  s.callers = true;
+  s.ws = workspace;
+  s.bytes = workspace_bytes;
+  return attention_launch(ctx, a, s, lse);
 }

@@ -1,0 +1,970 @@
+// The backward pass of attention on tcgen05 (kind::f16), head_dim 64 and 128, bf16 and fp16: recomputes
+// the probabilities from q, k and the forward's row statistic lse, and writes dq, dk, dv.
+//
+//   S = scale Q K^T, P = exp(S - lse), dP = dO V^T, delta = rowsum(dO O), dS = P (dP - delta)
+//   dV = P^T dO, dK = scale dS^T Q, dQ = scale dS K
+//
+// Two kinds of work units, in one launch. A k/v unit holds 128 keys of one k/v head and walks the
+// query blocks that see them (of every q head of the group, and of every batch item that shares the
+// K/V), with dV and dK in tensor memory. A q unit holds 128 queries of one head and walks its key
+// blocks, with dQ in tensor memory. S and dP are so computed twice, 7 products for the 5 that the
+// gradients need; in return nothing is added up in memory between units, so there are no atomics and
+// the same inputs give the same bits.
+//
+// 320 threads: warps 0-7 turn S and dP into P and dS (warp w: the 32 tensor-memory lanes of quadrant
+// w % 4, column half w / 4), warp 8 loads tiles by TMA, warp 9 allocates tensor memory and issues the
+// products. A k/v unit computes the transposed S^T = K Q^T and dP^T = V dO^T (lanes = keys), so that
+// P^T and dS^T, rounded to 16 bits and written back over S^T and dP^T, are the A operand of
+// dV += P^T dO and dK += dS^T Q straight from tensor memory, with the Q and dO tiles that are in
+// shared memory anyway as their MN-major B operand. Issue order per block:
+//   dV(i) S(i+1) [dS(i) written] dK(i) dP(i+1)
+// so the exponentials of block i + 1 overlap dK(i) and dP(i+1), and the products dS(i) overlap dV(i)
+// and S(i+1). A q unit has S twice in tensor memory: dQ(i) dP(i+1) S(i+2).
+// Tensor memory, k/v unit: S^T [0,128) dP^T [128,256) dV [256,256+D) dK [256+D,256+2D);
+// q unit: S [0,128) and [384,512), dP [128,256), dQ [256,256+D).
+//
+// Roundings. P and dS round to the operands' type before their products (fp32 sums). In fp16 both are
+// moved into its range by powers of two that are undone in fp32: P <= 1 by 2^14; dS by a factor from
+// the bound |dS| <= 2 max|dO_i| max|V_j| of the k/v head, so that gradients of any size keep their
+// digits. bf16 has fp32's range and needs neither.
+//
+// Masks: a query row that sees no key has lse = -inf, P = 0 and no gradient. Keys past key_len get
+// dK = dV = 0 whatever they hold: P and dS are selected, not multiplied, to 0, and a q unit clears
+// their rows of K in shared memory (0 x NaN is not 0).
+
+#include "internal.h"
+#include "sm100.cuh"
+
+namespace anima {
+namespace agrad {
+
+using attn::arrive_one_lane;
+using attn::ATOM;
+using attn::ex2;
+using attn::pack2;
+using attn::TILE;
+using attn::warp_wait;
+
+constexpr int THREADS = 320;
+constexpr int MATH_WARPS = 8;
+constexpr int TILE_BYTES = 2 * ATOM;  // a tile's slot: 128 rows of 128 16-bit columns (64: half of it is used)
+// shared memory: the unit's two tiles | ring of up to 3 first tiles | ring of 2 second tiles | row
+// statistics of the ring's stages | barriers. A k/v unit: K, V | Q | dO; a q unit: Q, dO | K | V.
+constexpr int OFF_X = 0;
+constexpr int OFF_Y0 = OFF_X + 2 * TILE_BYTES;
+constexpr int Y0_STAGES = 3;
+constexpr int OFF_Y1 = OFF_Y0 + Y0_STAGES * TILE_BYTES;
+constexpr int Y1_STAGES = 2;
+// a k/v unit needs only two stages of Q: the third's place holds the statistics
+constexpr int KV_Y0_STAGES = 2;
+constexpr int OFF_STAT = OFF_Y0 + KV_Y0_STAGES * TILE_BYTES;  // [2 stages][nlse2 | ndelta][128]
+constexpr int OFF_BAR = OFF_Y1 + Y1_STAGES * TILE_BYTES;
+constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
+static_assert(SMEM_BYTES <= 232448, "fits a block's shared memory");
+constexpr float kP16Shift = 14.0f;  // fp16: P is held as 2^14 P
+
+struct Params {
+  int B, H, group, Lq, Lk, Lqp;  // Lqp: Lq rounded up to whole tiles
+  int kv_batch;                  // 1 where the items share one K/V
+  int q_col, k_col, v_col;
+  int causal;
+  const int* key_len;
+  float scale, scale_log2;
+  const float* nlse2;   // [B][H][Lqp] -lse log2(e) (fp16: + 14), -inf for rows without a key
+  const float* ndelta;  // [B][H][Lqp] -delta
+  const unsigned* top;  // fp16: [kv_batch][Hk][2] largest |dO_i|^2 and |V_j|^2, as bits
+  void *dq, *dk, *dv;
+  long long lddq, lddk, lddv, dq_bs, dk_bs, dv_bs;
+  int grad_dtype;
+  int kv_units, q_units, nkb, nqb, kv_splits, q_splits;
+  float* kv_part;  // [split][unit][dv | dk][D / 4][128] float4, where kv_splits > 1
+  float* q_part;   // [split][unit][D / 4][128] float4
+};
+
+// The keys of an item that count.
+__device__ __forceinline__ int keys_of(const Params& p, int kvb) {
+  return p.key_len ? max(0, min(p.Lk, p.key_len[kvb])) : p.Lk;
+}
+
+// The power of two that moves this k/v head's dS into fp16 (its bound to 2^15 at most).
+__device__ __forceinline__ float ds_scale(const Params& p, int kv_head) {
+  const float bound = 2.f * sqrtf(__uint_as_float(p.top[2 * kv_head])) * sqrtf(__uint_as_float(p.top[2 * kv_head + 1]));
+  if (!(bound > 0.f) || bound == INFINITY) return 1.f;
+  const int e = min(max(14 - ilogbf(bound), -100), 100);
+  return ldexpf(1.f, e);
+}
+
+struct Bars {
+  uint64_t *x_full, *y0_full, *y1_full, *y0_empty, *y1_empty, *s_full, *dp_full, *p_full, *ds_full, *acc_done, *drain;
+};
+constexpr int kBars = 1 + 3 + 2 + 3 + 2 + 2 + 1 + 1 + 1 + 1 + 1;
+
+// What a block does: a k/v unit or a q unit, and its range of iterations.
+struct Work {
+  bool kv;
+  int unit, split;
+  int blk;         // key block of a k/v unit, query block of a q unit
+  int b, h;        // k/v unit: K/V item and k/v head; q unit: item and q head
+  int lo, n;       // first iteration and their number
+  int per_head;    // k/v unit: iterations (query blocks) of one q head
+};
+
+__device__ __forceinline__ Work work_of(const Params& p) {
+  Work w;
+  int id = blockIdx.x;
+  const int kv_ctas = p.kv_units * p.kv_splits;
+  w.kv = id < kv_ctas;
+  int total;
+  if (w.kv) {
+    w.unit = id / p.kv_splits;
+    w.split = id - w.unit * p.kv_splits;
+    const int heads = p.kv_units / p.nkb;  // (K/V item, k/v head) pairs
+    // causal: early key blocks are seen by most queries, so they go first; else head by head
+    const int bh = p.causal ? w.unit % heads : w.unit / p.nkb;
+    w.blk = p.causal ? w.unit / heads : w.unit % p.nkb;
+    const int Hk = p.H / p.group;
+    w.b = bh / Hk;
+    w.h = bh - w.b * Hk;
+    const int q0 = p.causal ? w.blk : 0;
+    w.per_head = w.blk * TILE < keys_of(p, w.b) ? max(0, p.nqb - q0) : 0;
+    total = w.per_head * p.group * (p.B / p.kv_batch);
+    w.lo = static_cast<int>(static_cast<long long>(total) * w.split / p.kv_splits);
+    w.n = static_cast<int>(static_cast<long long>(total) * (w.split + 1) / p.kv_splits) - w.lo;
+  } else {
+    id -= kv_ctas;
+    w.unit = id / p.q_splits;
+    w.split = id - w.unit * p.q_splits;
+    const int heads = p.B * p.H;
+    const int bh = p.causal ? w.unit % heads : w.unit / p.nqb;
+    w.blk = p.causal ? p.nqb - 1 - w.unit / heads : w.unit % p.nqb;
+    w.b = bh / p.H;
+    w.h = bh - w.b * p.H;
+    total = (keys_of(p, p.kv_batch > 1 ? w.b : 0) + TILE - 1) / TILE;
+    if (p.causal) total = min(total, w.blk + 1);
+    w.lo = total * w.split / p.q_splits;
+    w.n = total * (w.split + 1) / p.q_splits - w.lo;
+    w.per_head = 0;
+  }
+  return w;
+}
+
+// Iteration i of a k/v unit: the item, q head and query block.
+__device__ __forceinline__ void kv_iteration(const Params& p, const Work& w, int i, int& b, int& h, int& qb) {
+  const int it = w.lo + i;
+  const int hh = it / w.per_head;  // (item, head of the group)
+  qb = it - hh * w.per_head + (p.causal ? w.blk : 0);
+  const int g = hh % p.group;
+  b = p.kv_batch > 1 ? w.b : hh / p.group;
+  h = w.h * p.group + g;
+}
+
+// 16-bit values of a column half h lie at the half's own columns, so neither of a row's two warps
+// overwrites what the other still reads: k-step k (16 of the 128 inner indices, 8 columns) of the A operand.
+__device__ __forceinline__ uint32_t half_cols(int k) { return (k >> 2) * 64 + (k & 3) * 8; }
+
+// Row `row` of the unit's tile, columns [c0, c0 + 32): to the gradient, or to a partial sum.
+__device__ __forceinline__ void put32(void* out, int dtype, size_t at, const uint32_t (&r)[32], float f) {
+  if (dtype == ANIMA_F32) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      d[t] = make_float4(__uint_as_float(r[4 * t]) * f, __uint_as_float(r[4 * t + 1]) * f,
+                         __uint_as_float(r[4 * t + 2]) * f, __uint_as_float(r[4 * t + 3]) * f);
+  } else {
+    uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+    const bool bf = dtype == ANIMA_BF16;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = __uint_as_float(r[8 * t + 2 * e]) * f, b = __uint_as_float(r[8 * t + 2 * e + 1]) * f;
+        w[e] = bf ? pack2<true>(a, b) : pack2<false>(a, b);
+      }
+      d[t] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <bool BF16, int HD>
+__global__ void __launch_bounds__(THREADS, 1)
+    attention_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                          const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                          const Params p) {
+  constexpr int ATOMS = HD / 64;
+  constexpr int BYTES = ATOMS * ATOM;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
+  const Bars bar{bars, bars + 1, bars + 4, bars + 6, bars + 9, bars + 11, bars + 13, bars + 14, bars + 15, bars + 16,
+                 bars + 17};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kProducerWarp = MATH_WARPS, kMmaWarp = MATH_WARPS + 1;
+  const Work w = work_of(p);
+  const int y0_stages = w.kv ? KV_Y0_STAGES : Y0_STAGES;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBars; ++i) {
+      const bool math = bars + i == bar.p_full || bars + i == bar.ds_full;
+      mbar_init(bars + i, math ? MATH_WARPS : 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t t_s = tmem, t_dp = tmem + 128, t_acc = tmem + 256, t_acc2 = tmem + 256 + HD, t_s1 = tmem + 384;
+
+  if (warp == kProducerWarp) {
+    if (lane == 0 && w.n > 0) {
+      // what is in flight: for each full barrier, armed and the parity of its last arm
+      uint32_t armed = 0;
+      auto arm = [&](int i, uint32_t ph) { armed = (armed & ~(3u << (2 * i))) | ((2u | ph) << (2 * i)); };
+      auto load = [&](int off, const CUtensorMap* tm, uint64_t* fb, int col, int row, int item) {
+#pragma unroll
+        for (int t = 0; t < ATOMS; ++t) tma_load_3d(smem + off + t * ATOM, tm, fb, col + 64 * t, row, item);
+      };
+      const int kvb = p.kv_batch > 1 ? w.b : 0;
+      const int hk = w.kv ? w.h : w.h / p.group;
+      const int kc = p.k_col + hk * HD, vc = p.v_col + hk * HD;
+      mbar_arrive_expect_tx(bar.x_full, 2 * BYTES);
+      if (w.kv) {
+        load(OFF_X, &tm_k, bar.x_full, kc, w.blk * TILE, kvb);
+        load(OFF_X + TILE_BYTES, &tm_v, bar.x_full, vc, w.blk * TILE, kvb);
+      } else {
+        load(OFF_X, &tm_q, bar.x_full, p.q_col + w.h * HD, w.blk * TILE, w.b);
+        load(OFF_X + TILE_BYTES, &tm_do, bar.x_full, w.h * HD, w.blk * TILE, w.b);
+      }
+      arm(0, 0);
+      int s0 = 0, s1 = 0;
+      uint32_t ph0 = 0, ph1 = 0;
+      for (int i = 0; i < w.n; ++i) {
+        int b = 0, h = 0, qb = 0;
+        if (w.kv) kv_iteration(p, w, i, b, h, qb);
+        const size_t stat = (static_cast<size_t>(b) * p.H + h) * p.Lqp + static_cast<size_t>(qb) * TILE;
+        float* st = reinterpret_cast<float*>(smem + OFF_STAT);
+        if (!mbar_wait(&bar.y0_empty[s0], ph0 ^ 1, abort_flag, kErrTimeoutEmpty)) break;
+        if (w.kv) {
+          // the statistics come and go with Q: its place is freed last, after dK(i) and so after dS(i)
+          mbar_arrive_expect_tx(&bar.y0_full[s0], BYTES + 2 * TILE * 4);
+          load(OFF_Y0 + s0 * TILE_BYTES, &tm_q, &bar.y0_full[s0], p.q_col + h * HD, qb * TILE, b);
+          bulk_load_1d(st + s0 * 2 * TILE, p.nlse2 + stat, TILE * 4, &bar.y0_full[s0]);
+          bulk_load_1d(st + s0 * 2 * TILE + TILE, p.ndelta + stat, TILE * 4, &bar.y0_full[s0]);
+        } else {
+          mbar_arrive_expect_tx(&bar.y0_full[s0], BYTES);
+          load(OFF_Y0 + s0 * TILE_BYTES, &tm_k, &bar.y0_full[s0], kc, (w.lo + i) * TILE, kvb);
+        }
+        arm(1 + s0, ph0);
+        if (!mbar_wait(&bar.y1_empty[s1], ph1 ^ 1, abort_flag, kErrTimeoutEmpty)) break;
+        if (w.kv) {
+          mbar_arrive_expect_tx(&bar.y1_full[s1], BYTES);
+          load(OFF_Y1 + s1 * TILE_BYTES, &tm_do, &bar.y1_full[s1], h * HD, qb * TILE, b);
+        } else {
+          mbar_arrive_expect_tx(&bar.y1_full[s1], BYTES);
+          load(OFF_Y1 + s1 * TILE_BYTES, &tm_v, &bar.y1_full[s1], vc, (w.lo + i) * TILE, kvb);
+        }
+        arm(4 + s1, ph1);
+        if (++s0 == y0_stages) s0 = 0, ph0 ^= 1;
+        if (++s1 == Y1_STAGES) s1 = 0, ph1 ^= 1;
+      }
+      if (*abort_flag) {
+        // let every copy this thread started land before the block exits
+        for (int i = 0; i < 6; ++i) {
+          const uint32_t a = (armed >> (2 * i)) & 3u;
+          if (!(a & 2u)) continue;
+          const unsigned long long t0 = globaltimer();
+          while (!mbar_test(smem_u32(bars + i), a & 1u)) {
+            if (globaltimer() - t0 > kWaitTimeoutNs) {
+              flag_error(kErrTimeoutDrain);
+              break;
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0 && w.n > 0) {
+      const uint32_t id_s = idesc_f16(TILE, TILE, BF16, false);
+      const uint32_t id_acc = idesc_f16(TILE, HD, BF16, true);
+      const uint32_t sx = smem_u32(smem + OFF_X), sy0 = smem_u32(smem + OFF_Y0), sy1 = smem_u32(smem + OFF_Y1);
+      // d = A B^T over the head's dims, both tiles K-major in shared memory
+      auto dims_product = [&](uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = (k >> 2) * ATOM + (k & 3) * 32;
+          umma_f16(d, sdesc_sw128(a + off, 16, 1024), sdesc_sw128(b + off, 16, 1024), id_s, k > 0 ? 1u : 0u);
+        }
+      };
+      // d (+)= A B, A 128 x 128 16-bit in tensor memory, B's rows the inner index
+      auto rows_product = [&](uint32_t d, uint32_t a, uint32_t b, bool first) {
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k)
+          umma_f16_ts(d, a + half_cols(k), sdesc_sw128(b + k * 16 * 128, ATOM, 1024), id_acc,
+                      (!first || k > 0) ? 1u : 0u);
+      };
+      auto full = [&](uint64_t* fb, uint32_t ph) { return mbar_wait(fb, ph, abort_flag, kErrTimeoutFull); };
+      bool ok = full(bar.x_full, 0) && full(&bar.y0_full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        dims_product(t_s, sx, sy0);
+        umma_commit(&bar.s_full[0]);
+        ok = full(&bar.y1_full[0], 0);
+      }
+      if (ok) {
+        dims_product(t_dp, sx + TILE_BYTES, sy1);
+        umma_commit(bar.dp_full);
+      }
+      if (w.kv) {
+        int s = 0;  // stage of block i (both rings have two)
+        uint32_t ph = 0;
+        for (int i = 0; ok && i < w.n; ++i) {
+          const int s1 = s ^ 1;
+          const uint32_t ph1 = s1 ? ph : ph ^ 1;
+          const bool more = i + 1 < w.n;
+          if (!(ok = full(bar.p_full, i & 1))) break;
+          tc_fence_after();
+          rows_product(t_acc, t_s, sy1 + s * TILE_BYTES, i == 0);  // dV
+          umma_commit(&bar.y1_empty[s]);
+          if (more) {
+            if (!(ok = full(&bar.y0_full[s1], ph1))) break;
+            dims_product(t_s, sx, sy0 + s1 * TILE_BYTES);
+            umma_commit(&bar.s_full[0]);
+          }
+          if (!(ok = full(bar.ds_full, i & 1))) break;
+          tc_fence_after();
+          rows_product(t_acc2, t_dp, sy0 + s * TILE_BYTES, i == 0);  // dK
+          umma_commit(&bar.y0_empty[s]);
+          if (more) {
+            if (!(ok = full(&bar.y1_full[s1], ph1))) break;
+            dims_product(t_dp, sx + TILE_BYTES, sy1 + s1 * TILE_BYTES);
+            umma_commit(bar.dp_full);
+          }
+          s = s1;
+          ph = ph1;
+        }
+      } else {
+        int r0 = 0, n0 = 1;  // ring places of K: block i, the next S
+        uint32_t pn0 = 0;    // the phase of the next S's place
+        auto next_s = [&](int j) {
+          if (!full(&bar.y0_full[n0], pn0)) return false;
+          dims_product(j & 1 ? t_s1 : t_s, sx, sy0 + n0 * TILE_BYTES);
+          umma_commit(&bar.s_full[j & 1]);
+          if (++n0 == Y0_STAGES) n0 = 0, pn0 ^= 1;
+          return true;
+        };
+        if (ok) umma_commit(&bar.y1_empty[0]);
+        if (ok && w.n > 1) ok = next_s(1);
+        for (int i = 0; ok && i < w.n; ++i) {
+          if (!(ok = full(bar.ds_full, i & 1))) break;
+          tc_fence_after();
+          rows_product(t_acc, t_dp, sy0 + r0 * TILE_BYTES, i == 0);  // dQ
+          umma_commit(&bar.y0_empty[r0]);
+          if (++r0 == Y0_STAGES) r0 = 0;
+          if (i + 1 < w.n) {
+            const int s1 = (i + 1) & 1;
+            if (!(ok = full(&bar.y1_full[s1], ((i + 1) >> 1) & 1))) break;
+            dims_product(t_dp, sx + TILE_BYTES, sy1 + s1 * TILE_BYTES);
+            umma_commit(bar.dp_full);
+            umma_commit(&bar.y1_empty[s1]);
+          }
+          if (i + 2 < w.n && !(ok = next_s(i + 2))) break;
+        }
+      }
+      if (ok) {
+        umma_commit(bar.acc_done);
+      } else {
+        // every product this thread issued completes before the block frees tensor memory
+        umma_commit(bar.drain);
+        const unsigned long long t0 = globaltimer();
+        while (!mbar_test(smem_u32(bar.drain), 0)) {
+          if (globaltimer() - t0 > kWaitTimeoutNs) {
+            flag_error(kErrTimeoutDrain);
+            break;
+          }
+        }
+      }
+    }
+  } else {
+    const int hf = warp >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    const f2 sc2 = dup2(p.scale_log2);
+    const int kv_len = keys_of(p, p.kv_batch > 1 ? w.b : 0);
+    float cds = 1.f;  // fp16: dS is held as c dS
+    if (!BF16) cds = ds_scale(p, (p.kv_batch > 1 ? w.b : 0) * (p.H / p.group) + (w.kv ? w.h : w.h / p.group));
+    const f2 c2 = dup2(BF16 ? 1.f : cds * exp2f(-kP16Shift));  // P arrives as 2^14 P
+    bool ok = true;
+    float pr[64];  // this half row of P
+    for (int i = 0; i < w.n; ++i) {
+      if (w.kv) {
+        int b, h, qb;
+        kv_iteration(p, w, i, b, h, qb);
+        const int s = i & 1;
+        const uint32_t ph = (i >> 1) & 1;
+        const float* nlse2 = reinterpret_cast<const float*>(smem + OFF_STAT) + s * 2 * TILE + 64 * hf;
+        const float* ndelta = nlse2 + TILE;
+        // lanes are keys: a hidden key's whole row, and on the diagonal block queries before the key
+        const bool diag = p.causal && qb == w.blk;
+        const bool masked = diag || w.blk * TILE + TILE > kv_len;
+        const int first = w.blk * TILE + row >= kv_len ? TILE : (diag ? row : 0);  // first query that sees it
+        if (!(ok = warp_wait(&bar.y0_full[s], ph, abort_flag, kErrTimeoutFull) &&
+                   warp_wait(bar.s_full, i & 1, abort_flag, kErrTimeoutFull)))
+          break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32];
+          tmem_ld32(t_s + lane_addr + 64 * hf + 32 * c, r);
+          tmem_ld_wait(r);
+          uint32_t pk[16];
+#pragma unroll
+          for (int t = 0; t < 32; t += 4) {
+            const float4 l = *reinterpret_cast<const float4*>(nlse2 + 32 * c + t);
+            const f2 a0 = fma2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, make_float2(l.x, l.y));
+            const f2 a1 =
+                fma2(make_float2(__uint_as_float(r[t + 2]), __uint_as_float(r[t + 3])), sc2, make_float2(l.z, l.w));
+            float e[4] = {ex2(a0.x), ex2(a0.y), ex2(a1.x), ex2(a1.y)};
+            if (masked) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (64 * hf + 32 * c + t + u < first) e[u] = 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) pr[32 * c + t + u] = e[u];
+            pk[t / 2] = pack2<BF16>(e[0], e[1]);
+            pk[t / 2 + 1] = pack2<BF16>(e[2], e[3]);
+          }
+          tmem_st16(t_s + lane_addr + 64 * hf + 16 * c, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        arrive_one_lane(bar.p_full);
+        if (!(ok = warp_wait(bar.dp_full, i & 1, abort_flag, kErrTimeoutFull))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32];
+          tmem_ld32(t_dp + lane_addr + 64 * hf + 32 * c, r);
+          tmem_ld_wait(r);
+          uint32_t pk[16];
+#pragma unroll
+          for (int t = 0; t < 32; t += 4) {
+            const float4 d = *reinterpret_cast<const float4*>(ndelta + 32 * c + t);
+            f2 g0 = add2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), make_float2(d.x, d.y));
+            f2 g1 = add2(make_float2(__uint_as_float(r[t + 2]), __uint_as_float(r[t + 3])), make_float2(d.z, d.w));
+            f2 p0 = make_float2(pr[32 * c + t], pr[32 * c + t + 1]), p1 = make_float2(pr[32 * c + t + 2], pr[32 * c + t + 3]);
+            if (!BF16) p0 = mul2(p0, c2), p1 = mul2(p1, c2);
+            g0 = mul2(g0, p0);
+            g1 = mul2(g1, p1);
+            if (masked) {  // 0 whatever dP is
+              const int q = 64 * hf + 32 * c + t;
+              if (q < first) g0.x = 0.f;
+              if (q + 1 < first) g0.y = 0.f;
+              if (q + 2 < first) g1.x = 0.f;
+              if (q + 3 < first) g1.y = 0.f;
+            }
+            pk[t / 2] = pack2<BF16>(g0.x, g0.y);
+            pk[t / 2 + 1] = pack2<BF16>(g1.x, g1.y);
+          }
+          tmem_st16(t_dp + lane_addr + 64 * hf + 16 * c, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        arrive_one_lane(bar.ds_full);
+      } else {
+        const int kb = w.lo + i;
+        const size_t at = (static_cast<size_t>(w.b) * p.H + w.h) * p.Lqp + static_cast<size_t>(w.blk) * TILE + row;
+        const f2 nlse2 = dup2(p.nlse2[at]), ndelta = dup2(p.ndelta[at]);
+        // lanes are queries: the row's visible keys of this block end at `end`
+        const int left = kv_len - kb * TILE;
+        const bool masked = left < TILE || (p.causal && kb == w.blk);
+        const int end = p.causal && kb == w.blk ? min(left, row + 1) : left;
+        const uint32_t ts = (i & 1 ? t_s1 : t_s) + lane_addr + 64 * hf;
+        if (!(ok = warp_wait(&bar.s_full[i & 1], (i >> 1) & 1, abort_flag, kErrTimeoutFull))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32];
+          tmem_ld32(ts + 32 * c, r);
+          tmem_ld_wait(r);
+#pragma unroll
+          for (int t = 0; t < 32; t += 2) {
+            const f2 a = fma2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, nlse2);
+            pr[32 * c + t] = ex2(a.x);
+            pr[32 * c + t + 1] = ex2(a.y);
+          }
+        }
+        if (!(ok = warp_wait(bar.dp_full, i & 1, abort_flag, kErrTimeoutFull))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t r[32];
+          tmem_ld32(t_dp + lane_addr + 64 * hf + 32 * c, r);
+          tmem_ld_wait(r);
+          uint32_t pk[16];
+#pragma unroll
+          for (int t = 0; t < 32; t += 2) {
+            f2 g = add2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), ndelta);
+            f2 pp = make_float2(pr[32 * c + t], pr[32 * c + t + 1]);
+            if (!BF16) pp = mul2(pp, c2);
+            g = mul2(g, pp);
+            if (masked) {  // 0 whatever S and dP are
+              if (64 * hf + 32 * c + t >= end) g.x = 0.f;
+              if (64 * hf + 32 * c + t + 1 >= end) g.y = 0.f;
+            }
+            pk[t / 2] = pack2<BF16>(g.x, g.y);
+          }
+          tmem_st16(t_dp + lane_addr + 64 * hf + 16 * c, pk);
+        }
+        if (left < TILE && p.key_len) {
+          // K's rows behind key_len may hold anything, and dS K multiplies them by 0
+          const int s0 = i % Y0_STAGES;
+          if (!(ok = warp_wait(&bar.y0_full[s0], (i / Y0_STAGES) & 1, abort_flag, kErrTimeoutFull))) break;
+          const int n = (TILE - left) * 8;  // 16-byte pieces of an atom's rows
+          for (int t = threadIdx.x; t < n * ATOMS; t += MATH_WARPS * 32)
+            *reinterpret_cast<uint4*>(smem + OFF_Y0 + s0 * TILE_BYTES + (t / n) * ATOM + left * 128 + (t % n) * 16) =
+                make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        arrive_one_lane(bar.ds_full);
+      }
+    }
+    if (ok && w.n > 0) ok = warp_wait(bar.acc_done, 0, abort_flag, kErrTimeoutAcc);
+    if (ok) {
+      tc_fence_after();
+      const bool split = (w.kv ? p.kv_splits : p.q_splits) > 1;
+      const int r = w.blk * TILE + row;
+      const int accs = w.kv ? 2 : 1;  // dV, dK
+#pragma unroll 1
+      for (int a = 0; a < accs; ++a) {
+#pragma unroll 1
+        for (int c = 0; c < ATOMS; ++c) {
+          uint32_t v[32];
+          if (w.n > 0) {
+            tmem_ld32((a ? t_acc2 : t_acc) + lane_addr + (HD / 2) * hf + 32 * c, v);
+            tmem_ld_wait(v);
+          } else {
+#pragma unroll
+            for (int t = 0; t < 32; ++t) v[t] = 0u;
+          }
+          float f;
+          if (w.kv && a == 0)
+            f = BF16 ? 1.f : exp2f(-kP16Shift);
+          else
+            f = BF16 ? p.scale : p.scale / cds;
+          const int c0 = (HD / 2) * hf + 32 * c;
+          if (split) {
+            const size_t slot = w.kv ? (static_cast<size_t>(w.split) * p.kv_units + w.unit) * 2 + a
+                                     : static_cast<size_t>(w.split) * p.q_units + w.unit;
+            float4* d = reinterpret_cast<float4*>(w.kv ? p.kv_part : p.q_part) + (slot * (HD / 4) + c0 / 4) * TILE + row;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              d[t * TILE] = make_float4(__uint_as_float(v[4 * t]) * f, __uint_as_float(v[4 * t + 1]) * f,
+                                        __uint_as_float(v[4 * t + 2]) * f, __uint_as_float(v[4 * t + 3]) * f);
+          } else if (w.kv) {
+            if (r < p.Lk) {
+              void* out = a ? p.dk : p.dv;
+              const size_t at = a ? w.b * p.dk_bs + r * p.lddk : w.b * p.dv_bs + r * p.lddv;
+              put32(out, p.grad_dtype, at + static_cast<size_t>(w.h) * HD + c0, v, f);
+            }
+          } else if (r < p.Lq) {
+            put32(p.dq, p.grad_dtype, w.b * p.dq_bs + r * p.lddq + static_cast<size_t>(w.h) * HD + c0, v, f);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ before and after it
+
+// delta and the scaled row statistic of every (item, head, query), padded to whole tiles with rows
+// that no key sees; D / 8 threads a row and head, 16 bytes each. In fp16 also the largest |dO_i|^2.
+// Bound by reading out and dout once.
+struct PrepParams {
+  const void* out;
+  const void* dout;
+  const float* lse;
+  long long ldo, o_bs, lddo, do_bs;
+  int out_dtype, B, H, group, Lq, Lqp, kv_batch;
+  float shift;  // 14 in fp16
+  float *nlse2, *ndelta;
+  unsigned* top;
+};
+
+__device__ __forceinline__ void load8(const void* p, int dtype, size_t at, float (&v)[8]) {
+  if (dtype == ANIMA_F32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    return;
+  }
+  const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = resnorm::lo16(w[i], dtype);
+    v[2 * i + 1] = resnorm::hi16(w[i], dtype);
+  }
+}
+
+template <bool BF16, int HD>
+__global__ void __launch_bounds__(256) attention_grad_prep_kernel(const PrepParams p) {
+  constexpr int TPR = HD / 8;
+  const long long id = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / TPR;
+  const int t = threadIdx.x % TPR;
+  const long long rows = static_cast<long long>(p.B) * p.Lqp;
+  const long long row = id / p.H;
+  const int h = static_cast<int>(id - row * p.H);
+  const bool in = row < rows;
+  const int b = in ? static_cast<int>(row / p.Lqp) : 0;
+  const int i = in ? static_cast<int>(row - static_cast<long long>(b) * p.Lqp) : 0;
+  const bool real = in && i < p.Lq;
+  float d = 0.f, n = 0.f;
+  if (real) {
+    float o[8], g[8];
+    load8(p.out, p.out_dtype, static_cast<size_t>(b) * p.o_bs + i * p.ldo + static_cast<size_t>(h) * HD + 8 * t, o);
+    load8(p.dout, BF16 ? ANIMA_BF16 : ANIMA_F16, static_cast<size_t>(b) * p.do_bs + i * p.lddo + static_cast<size_t>(h) * HD + 8 * t, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      d = fmaf(o[j], g[j], d);
+      n = fmaf(g[j], g[j], n);
+    }
+  }
+#pragma unroll
+  for (int s = TPR / 2; s > 0; s >>= 1) {
+    d += __shfl_xor_sync(0xffffffffu, d, s);
+    if (!BF16) n += __shfl_xor_sync(0xffffffffu, n, s);
+  }
+  if (!in || t) return;
+  const size_t at = (static_cast<size_t>(b) * p.H + h) * p.Lqp + i;
+  const float l = real ? p.lse[(static_cast<size_t>(b) * p.H + h) * p.Lq + i] : -INFINITY;
+  p.nlse2[at] = l == -INFINITY ? -INFINITY : fmaf(l, -1.4426950408889634f, p.shift);
+  p.ndelta[at] = -d;
+  if (!BF16 && real && n > 0.f)
+    atomicMax(p.top + 2 * ((p.kv_batch > 1 ? b : 0) * (p.H / p.group) + h / p.group), __float_as_uint(n));
+}
+
+// fp16: the largest |V_j|^2 of each k/v head over the keys that count; a warp a row and head.
+__global__ void __launch_bounds__(256) attention_grad_vmax_kernel(const __half* v, long long ldv, long long v_bs, int Hk,
+                                                                  int D, int Lk, const int* key_len, unsigned* top) {
+  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
+  const int len = key_len ? min(Lk, key_len[b]) : Lk;
+  float best = 0.f;
+  for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < len; j += gridDim.x * 8) {
+    const __half2* r = reinterpret_cast<const __half2*>(v + b * v_bs + j * ldv + static_cast<long long>(h) * D);
+    float n = 0.f;
+    for (int c = lane; c < D / 2; c += 32) {
+      const float2 x = __half22float2(r[c]);
+      n = fmaf(x.x, x.x, fmaf(x.y, x.y, n));
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) n += __shfl_xor_sync(0xffffffffu, n, s);
+    best = fmaxf(best, n);
+  }
+  if (lane == 0 && best > 0.f) atomicMax(top + 2 * (b * Hk + h) + 1, __float_as_uint(best));
+}
+
+// The gradients of split units: the splits' partial sums added in order. A thread has four columns of
+// one row; the rows of a warp are neighbours, as the partials lie.
+template <int HD>
+__global__ void __launch_bounds__(128) attention_grad_join_kernel(const Params p) {
+  const int kv_tiles = p.kv_splits > 1 ? p.kv_units * 2 : 0;
+  int tile = blockIdx.x;
+  const bool kv = tile < kv_tiles;
+  if (!kv) tile -= kv_tiles;
+  const int unit = kv ? tile / 2 : tile, a = kv ? tile % 2 : 0;
+  const int splits = kv ? p.kv_splits : p.q_splits, tiles = kv ? p.kv_units * 2 : p.q_units;
+  const float4* part = reinterpret_cast<const float4*>(kv ? p.kv_part : p.q_part) +
+                       (static_cast<size_t>(tile) * (HD / 4) + blockIdx.y) * TILE + threadIdx.x;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < splits; ++i) {
+    const float4 v = part[static_cast<size_t>(i) * tiles * (HD / 4) * TILE];
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  int bh, blk, b, h;
+  if (kv) {
+    const int Hk = p.H / p.group, heads = p.kv_units / p.nkb;
+    bh = p.causal ? unit % heads : unit / p.nkb;
+    blk = p.causal ? unit / heads : unit % p.nkb;
+    b = bh / Hk;
+    h = bh - b * Hk;
+  } else {
+    const int heads = p.B * p.H;
+    bh = p.causal ? unit % heads : unit / p.nqb;
+    blk = p.causal ? p.nqb - 1 - unit / heads : unit % p.nqb;
+    b = bh / p.H;
+    h = bh - b * p.H;
+  }
+  const int r = blk * TILE + threadIdx.x;
+  if (r >= (kv ? p.Lk : p.Lq)) return;
+  void* out = kv ? (a ? p.dk : p.dv) : p.dq;
+  const size_t at = (kv ? (a ? b * p.dk_bs + r * p.lddk : b * p.dv_bs + r * p.lddv) : b * p.dq_bs + r * p.lddq) +
+                    static_cast<size_t>(h) * HD + blockIdx.y * 4;
+  if (p.grad_dtype == ANIMA_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = s;
+  } else {
+    uint2 w;
+    if (p.grad_dtype == ANIMA_BF16)
+      w = make_uint2(pack2<true>(s.x, s.y), pack2<true>(s.z, s.w));
+    else
+      w = make_uint2(pack2<false>(s.x, s.y), pack2<false>(s.z, s.w));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = w;
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+struct Plan {
+  int group, kv_batch, Lqp, nkb, nqb, kv_units, q_units, kv_splits, q_splits;
+  size_t lse_off, delta_off, top_off, top_bytes, kv_off, q_off, bytes;
+};
+
+// Units are split along their walk only where there are too few of them to fill the SMs: each split
+// writes and reads back an fp32 tile, and joining is a launch more, so a split keeps at least four
+// blocks (about 5 us of work against the 2 to 3 us that joining costs).
+int splits_of(long long blocks, long long all_units, int sms) {
+  long long s = 1;
+  if (all_units < sms) s = sms / all_units;
+  if (s > blocks / 4) s = blocks / 4;
+  if (s > 16) s = 16;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+int plan_of(const anima_ctx* ctx, const anima_attention_args* a, Plan& pl) {
+  pl.group = a->group > 1 ? a->group : 1;
+  const bool bcast = a->batch > 1 && a->k_bstride == 0 && a->v_bstride == 0;
+  pl.kv_batch = bcast ? 1 : a->batch;
+  pl.nqb = (a->Lq + TILE - 1) / TILE;
+  pl.nkb = (a->Lk + TILE - 1) / TILE;
+  pl.Lqp = pl.nqb * TILE;
+  const long long kv = static_cast<long long>(pl.kv_batch) * (a->heads / pl.group) * pl.nkb;
+  const long long q = static_cast<long long>(a->batch) * a->heads * pl.nqb;
+  ANIMA_REQUIRE(kv < (1LL << 26) && q < (1LL << 26) && a->Lq <= (1 << 30) && a->Lk <= (1 << 30),
+                "anima_attention_backward: problem too large");
+  const long long walk = static_cast<long long>(pl.nqb) * pl.group * (a->batch / pl.kv_batch);
+  ANIMA_REQUIRE(walk < (1LL << 31), "anima_attention_backward: problem too large");
+  pl.kv_units = static_cast<int>(kv);
+  pl.q_units = static_cast<int>(q);
+  pl.kv_splits = splits_of(walk, kv + q, ctx->num_sms);
+  pl.q_splits = splits_of(pl.nkb, kv + q, ctx->num_sms);
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at += (n + 255) / 256 * 256;
+    return o;
+  };
+  const size_t stat = static_cast<size_t>(a->batch) * a->heads * pl.Lqp * 4;
+  pl.lse_off = take(stat);
+  pl.delta_off = take(stat);
+  pl.top_bytes = a->dtype == ANIMA_F16 ? static_cast<size_t>(pl.kv_batch) * (a->heads / pl.group) * 8 : 0;
+  pl.top_off = take(pl.top_bytes);
+  const size_t tile = static_cast<size_t>(TILE) * a->head_dim * 4;
+  pl.kv_off = take(pl.kv_splits > 1 ? tile * 2 * pl.kv_units * pl.kv_splits : 0);
+  pl.q_off = take(pl.q_splits > 1 ? tile * pl.q_units * pl.q_splits : 0);
+  pl.bytes = at;
+  return ANIMA_OK;
+}
+
+int check(const char* fn, const anima_attention_grad_args* g) {
+  const anima_attention_args* a = &g->fwd;
+  ANIMA_REQUIRE(a->batch > 0 && a->heads > 0 && a->Lq > 0 && a->Lk > 0, "%s: empty problem", fn);
+  ANIMA_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "%s: head_dim %d (64 or 128)", fn, a->head_dim);
+  ANIMA_REQUIRE(a->dtype == ANIMA_BF16 || a->dtype == ANIMA_F16, "%s: q/k/v dtype must be bf16 or f16", fn);
+  ANIMA_REQUIRE(a->heads % (a->group > 1 ? a->group : 1) == 0, "%s: %d heads do not form groups of %d", fn, a->heads,
+                a->group);
+  ANIMA_REQUIRE(a->batch == 1 || (a->k_bstride == 0 && a->v_bstride == 0) || (a->k_bstride > 0 && a->v_bstride > 0),
+                "%s: k and v batch strides must both be zero (shared) or both positive", fn);
+  return ANIMA_OK;
+}
+
+template <bool BF16, int HD>
+int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, const Params& p, const PrepParams& pp,
+           const CUtensorMap (&tm)[4]) {
+  const anima_attention_args* a = &g->fwd;
+  const long long threads = static_cast<long long>(a->batch) * pl.Lqp * a->heads * (HD / 8);
+  ANIMA_REQUIRE((threads + 255) / 256 < (1LL << 31), "anima_attention_backward: problem too large");
+  ProfScope prof(ctx, "attn.grad", 10.0 * a->batch * a->heads * static_cast<double>(a->Lq) * a->Lk * HD, 0);
+  if (!BF16) {
+    ANIMA_CUDA(cudaMemsetAsync(pp.top, 0, pl.top_bytes, ctx->stream));
+    const int Hk = a->heads / pl.group;
+    ANIMA_REQUIRE(Hk <= 65535 && pl.kv_batch <= 65535, "anima_attention_backward: too many heads or items");
+    const int rows = (a->Lk + 31) / 32;
+    attention_grad_vmax_kernel<<<dim3(rows < 64 ? rows : 64, Hk, pl.kv_batch), 256, 0, ctx->stream>>>(
+        static_cast<const __half*>(a->v) + a->v_off, a->ldv, a->v_bstride, Hk, HD, a->Lk, a->key_len, pp.top);
+    const int st = check_launch("attention_grad_vmax_kernel");
+    if (st) return st;
+  }
+  attention_grad_prep_kernel<BF16, HD><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, ctx->stream>>>(pp);
+  int st = check_launch("attention_grad_prep_kernel");
+  if (st) return st;
+  const auto fn = attention_grad_kernel<BF16, HD>;
+  st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), SMEM_BYTES);
+  if (st) return st;
+  const long long ctas = static_cast<long long>(pl.kv_units) * pl.kv_splits + static_cast<long long>(pl.q_units) * pl.q_splits;
+  ANIMA_REQUIRE(ctas < (1LL << 31), "anima_attention_backward: problem too large");
+  fn<<<static_cast<unsigned>(ctas), THREADS, SMEM_BYTES, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], p);
+  st = check_launch("attention_grad_kernel");
+  if (st || (pl.kv_splits == 1 && pl.q_splits == 1)) return st;
+  const int tiles = (pl.kv_splits > 1 ? pl.kv_units * 2 : 0) + (pl.q_splits > 1 ? pl.q_units : 0);
+  attention_grad_join_kernel<HD><<<dim3(tiles, HD / 4), TILE, 0, ctx->stream>>>(p);
+  return check_launch("attention_grad_join_kernel");
+}
+
+}  // namespace agrad
+}  // namespace anima
+
+extern "C" int anima_attention_backward_workspace(anima_ctx* ctx, const anima_attention_grad_args* g, size_t* bytes) {
+  ANIMA_REQUIRE(ctx && g && bytes, "anima_attention_backward_workspace: NULL argument");
+  int st = agrad::check("anima_attention_backward_workspace", g);
+  if (st) return st;
+  agrad::Plan pl;
+  st = agrad::plan_of(ctx, &g->fwd, pl);
+  if (st) return st;
+  *bytes = pl.bytes;
+  return ANIMA_OK;
+}
+
+extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_grad_args* g) {
+  using namespace anima::agrad;
+  ANIMA_REQUIRE(ctx && g, "anima_attention_backward: NULL argument");
+  ANIMA_ON_DEVICE(ctx);
+  int st = check("anima_attention_backward", g);
+  if (st) return st;
+  const anima_attention_args* a = &g->fwd;
+  ANIMA_REQUIRE(a->q && a->k && a->v && a->out && g->lse && g->dout && g->dq && g->dk && g->dv,
+                "anima_attention_backward: NULL data pointer");
+  ANIMA_REQUIRE(a->out_dtype == ANIMA_F32 || a->out_dtype == ANIMA_BF16 || a->out_dtype == ANIMA_F16,
+                "anima_attention_backward: out_dtype %d", a->out_dtype);
+  ANIMA_REQUIRE(g->grad_dtype == ANIMA_F32 || g->grad_dtype == a->dtype,
+                "anima_attention_backward: grad_dtype %d (f32 or that of q)", g->grad_dtype);
+  Plan pl;
+  st = plan_of(ctx, a, pl);
+  if (st) return st;
+  const long long cq = static_cast<long long>(a->heads) * a->head_dim, ck = cq / pl.group;
+  ANIMA_REQUIRE(a->q_off >= 0 && a->k_off >= 0 && a->v_off >= 0 && a->ldq >= a->q_off + cq && a->ldk >= a->k_off + ck &&
+                    a->ldv >= a->v_off + ck && a->ldo >= cq && g->lddo >= cq && g->lddq >= cq && g->lddk >= ck &&
+                    g->lddv >= ck,
+                "anima_attention_backward: row stride too small");
+  ANIMA_REQUIRE(a->q_off % 8 == 0 && a->k_off % 8 == 0 && a->v_off % 8 == 0, "anima_attention_backward: column offsets "
+                "must be multiples of 8");
+  const bool many = a->batch > 1;
+  const struct {
+    const void* p;
+    long long ld, bs;
+    bool batched;
+  } all[8] = {{a->q, a->ldq, a->q_bstride, many},
+              {a->k, a->ldk, a->k_bstride, pl.kv_batch > 1},
+              {a->v, a->ldv, a->v_bstride, pl.kv_batch > 1},
+              {a->out, a->ldo, a->o_bstride, many},
+              {g->dout, g->lddo, g->do_bstride, many},
+              {g->dq, g->lddq, g->dq_bstride, many},
+              {g->dk, g->lddk, g->dk_bstride, pl.kv_batch > 1},
+              {g->dv, g->lddv, g->dv_bstride, pl.kv_batch > 1}};
+  for (const auto& t : all)
+    ANIMA_REQUIRE(reinterpret_cast<uintptr_t>(t.p) % 16 == 0 && t.ld % 8 == 0 && (!t.batched || (t.bs % 8 == 0 && t.bs > 0)),
+                  "anima_attention_backward: tensors must be 16-byte aligned, row and batch strides positive multiples "
+                  "of 8 elements");
+  ANIMA_REQUIRE(g->workspace && g->workspace_bytes >= pl.bytes && reinterpret_cast<uintptr_t>(g->workspace) % 256 == 0,
+                "anima_attention_backward: a workspace of %zu bytes (256-byte aligned) is needed, %zu are given", pl.bytes,
+                g->workspace ? g->workspace_bytes : 0);
+  CUtensorMap tm[4];
+  const CUtensorMapDataType dt =
+      a->dtype == ANIMA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint32_t box[3] = {64, anima::attn::TILE, 1};
+  const struct {
+    const void* p;
+    long long ld, bs;
+    int L, batch;
+  } maps[4] = {{a->q, a->ldq, a->q_bstride, a->Lq, a->batch},
+               {a->k, a->ldk, a->k_bstride, a->Lk, pl.kv_batch},
+               {a->v, a->ldv, a->v_bstride, a->Lk, pl.kv_batch},
+               {g->dout, g->lddo, g->do_bstride, a->Lq, a->batch}};
+  for (int i = 0; i < 4; ++i) {
+    const auto& m = maps[i];
+    const uint64_t dims[3] = {static_cast<uint64_t>(m.ld), static_cast<uint64_t>(m.L), static_cast<uint64_t>(m.batch)};
+    const uint64_t str[2] = {static_cast<uint64_t>(m.ld) * 2, static_cast<uint64_t>(m.batch > 1 ? m.bs : m.ld * m.L) * 2};
+    st = make_tmap(&tm[i], dt, 3, m.p, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st) return st;
+  }
+  unsigned char* ws = static_cast<unsigned char*>(g->workspace);
+  const float scale = a->scale > 0.f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim));
+  Params p{};
+  p.B = a->batch;
+  p.H = a->heads;
+  p.group = pl.group;
+  p.Lq = a->Lq;
+  p.Lk = a->Lk;
+  p.Lqp = pl.Lqp;
+  p.kv_batch = pl.kv_batch;
+  p.q_col = a->q_off;
+  p.k_col = a->k_off;
+  p.v_col = a->v_off;
+  p.causal = a->causal ? 1 : 0;
+  p.key_len = a->key_len;
+  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.nlse2 = reinterpret_cast<float*>(ws + pl.lse_off);
+  p.ndelta = reinterpret_cast<float*>(ws + pl.delta_off);
+  p.top = reinterpret_cast<unsigned*>(ws + pl.top_off);
+  p.dq = g->dq;
+  p.dk = g->dk;
+  p.dv = g->dv;
+  p.lddq = g->lddq;
+  p.lddk = g->lddk;
+  p.lddv = g->lddv;
+  p.dq_bs = many ? g->dq_bstride : 0;
+  p.dk_bs = pl.kv_batch > 1 ? g->dk_bstride : 0;
+  p.dv_bs = pl.kv_batch > 1 ? g->dv_bstride : 0;
+  p.grad_dtype = g->grad_dtype;
+  p.kv_units = pl.kv_units;
+  p.q_units = pl.q_units;
+  p.nkb = pl.nkb;
+  p.nqb = pl.nqb;
+  p.kv_splits = pl.kv_splits;
+  p.q_splits = pl.q_splits;
+  p.kv_part = reinterpret_cast<float*>(ws + pl.kv_off);
+  p.q_part = reinterpret_cast<float*>(ws + pl.q_off);
+  PrepParams pp{};
+  pp.out = a->out;
+  pp.dout = g->dout;
+  pp.lse = g->lse;
+  pp.ldo = a->ldo;
+  pp.o_bs = many ? a->o_bstride : 0;
+  pp.lddo = g->lddo;
+  pp.do_bs = many ? g->do_bstride : 0;
+  pp.out_dtype = a->out_dtype;
+  pp.B = a->batch;
+  pp.H = a->heads;
+  pp.group = pl.group;
+  pp.Lq = a->Lq;
+  pp.Lqp = pl.Lqp;
+  pp.kv_batch = pl.kv_batch;
+  pp.shift = a->dtype == ANIMA_F16 ? kP16Shift : 0.f;
+  pp.nlse2 = reinterpret_cast<float*>(ws + pl.lse_off);
+  pp.ndelta = reinterpret_cast<float*>(ws + pl.delta_off);
+  pp.top = reinterpret_cast<unsigned*>(ws + pl.top_off);
+  if (a->dtype == ANIMA_BF16)
+    return a->head_dim == 128 ? launch<true, 128>(ctx, g, pl, p, pp, tm) : launch<true, 64>(ctx, g, pl, p, pp, tm);
+  return a->head_dim == 128 ? launch<false, 128>(ctx, g, pl, p, pp, tm) : launch<false, 64>(ctx, g, pl, p, pp, tm);
+}

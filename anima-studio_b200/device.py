@@ -35,7 +35,8 @@ EXPORTS = [
     "anima_timestep_embedding", "anima_euler_step", "anima_lincomb", "anima_selftest_wait_timeout",
     "anima_ctx_set_attention_split", "anima_ipc_alloc", "anima_ipc_open", "anima_ipc_close", "anima_ipc_free",
     "anima_peer_barrier", "anima_conv3x3", "anima_channel_norm", "anima_rotary", "anima_residual_norm",
-    "anima_residual_norm_backward_workspace", "anima_residual_norm_backward",
+    "anima_residual_norm_backward_workspace", "anima_residual_norm_backward", "anima_attention_lse",
+    "anima_attention_lse_workspace", "anima_attention_backward", "anima_attention_backward_workspace",
 ]
 
 
@@ -82,6 +83,15 @@ class AttentionArgs(C.Structure):
                 ("v", C.c_void_p), ("ldv", C.c_longlong), ("v_bstride", C.c_longlong), ("v_off", C.c_int),
                 ("out", C.c_void_p), ("ldo", C.c_longlong), ("o_bstride", C.c_longlong), ("out_dtype", C.c_int),
                 ("key_len", C.c_void_p), ("scale", C.c_float), ("group", C.c_int), ("causal", C.c_int)]
+
+
+class AttentionGradArgs(C.Structure):
+    _fields_ = [("fwd", AttentionArgs), ("lse", C.c_void_p),
+                ("dout", C.c_void_p), ("lddo", C.c_longlong), ("do_bstride", C.c_longlong), ("grad_dtype", C.c_int),
+                ("dq", C.c_void_p), ("lddq", C.c_longlong), ("dq_bstride", C.c_longlong),
+                ("dk", C.c_void_p), ("lddk", C.c_longlong), ("dk_bstride", C.c_longlong),
+                ("dv", C.c_void_p), ("lddv", C.c_longlong), ("dv_bstride", C.c_longlong),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class RotaryArgs(C.Structure):
@@ -154,6 +164,10 @@ def load_library(path: str = LIB_PATH):
             "anima_residual_norm": [vp, C.POINTER(ResidualNormArgs)],
             "anima_residual_norm_backward_workspace": [vp, C.POINTER(ResidualNormArgs), C.POINTER(sz)],
             "anima_residual_norm_backward": [vp, C.POINTER(ResidualNormArgs)],
+            "anima_attention_lse_workspace": [vp, C.POINTER(AttentionArgs), C.POINTER(sz)],
+            "anima_attention_lse": [vp, C.POINTER(AttentionArgs), vp, vp, sz],
+            "anima_attention_backward_workspace": [vp, C.POINTER(AttentionGradArgs), C.POINTER(sz)],
+            "anima_attention_backward": [vp, C.POINTER(AttentionGradArgs)],
         }
         for name, args in sig.items():
             fn = getattr(lib, name)
@@ -182,7 +196,8 @@ LAUNCHING = set(EXPORTS) - {"anima_ctx_create", "anima_ctx_destroy", "anima_ctx_
                             "anima_last_error", "anima_alloc", "anima_free", "anima_upload", "anima_download",
                             "anima_profile_report", "anima_version", "anima_zero", "anima_selftest_wait_timeout",
                             "anima_ctx_set_attention_split", "anima_ipc_alloc", "anima_ipc_open", "anima_ipc_close",
-                            "anima_ipc_free", "anima_residual_norm_backward_workspace"}
+                            "anima_ipc_free", "anima_residual_norm_backward_workspace",
+                            "anima_attention_lse_workspace", "anima_attention_backward_workspace"}
 
 
 class KernelTimer:

@@ -506,6 +506,141 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, Lq: int, Lk:
     return out
 
 
+def _reach(fn: str, name: str, t: torch.Tensor, off: int, items: int, bstride: int, rows: int, ld: int, cols: int):
+    """Refuse strides that lead past the end of t's memory (or before its start)."""
+    if off < 0 or ld < off + cols or (items > 1 and bstride < 0):
+        raise dev.AnimaError(1, f"{fn}: {name}'s row stride {ld} is below its {off} + {cols} columns, or its batch "
+                                f"stride {bstride} negative")
+    need = off + (items - 1) * bstride + (rows - 1) * ld + cols
+    have = t.numel() if t.is_contiguous() else t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+    if need > have:
+        raise dev.AnimaError(1, f"{fn}: {name} has {have} elements, its sizes and strides reach {need}")
+
+
+def _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, batch, q_bstride, k_bstride, v_bstride,
+                key_len, out, o_bstride, scale, group, causal):
+    """The checked arguments that attention_lse and attention_backward share; returns them with the
+    number of k/v items (1 where the batch shares one K/V) and the k/v columns."""
+    if Lq <= 0 or Lk <= 0 or H <= 0 or batch <= 0 or group <= 0 or H % group:
+        raise dev.AnimaError(1, f"{fn}: batch {batch}, {Lq} queries, {Lk} keys, {H} heads in groups of {group}")
+    if D not in (64, 128):
+        raise dev.AnimaError(1, f"{fn}: head_dim {D} (64 or 128)")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise dev.AnimaError(1, f"{fn}: q, k and v are bf16 or fp16, not {q.dtype}")
+    C, Ck = H * D, H // group * D
+    a = dev.AttentionArgs(batch=batch, heads=H, head_dim=D, Lq=Lq, Lk=Lk, dtype=_dt(q), scale=scale or 0.0, group=group,
+                          causal=bool(causal))
+    kv_items = batch
+    if batch > 1 and k_bstride == 0 and v_bstride == 0:
+        kv_items = 1
+    for n, t, ld, off, items, bs, L, cols in (("q", q, ldq or C, q_off, batch, q_bstride, Lq, C),
+                                              ("k", k, ldk or Ck, k_off, kv_items, k_bstride, Lk, Ck),
+                                              ("v", v, ldv or Ck, v_off, kv_items, v_bstride, Lk, Ck)):
+        if t.dtype != q.dtype or t.device != q.device:
+            raise dev.AnimaError(1, f"{fn}: {n} is {t.dtype} on {t.device}, q {q.dtype} on {q.device}")
+        if items > 1 and bs <= 0:
+            raise dev.AnimaError(1, f"{fn}: {n}_bstride {bs} with {batch} items (k and v may both have 0: shared)")
+        _reach(fn, n, t, off, items, bs, L, ld, cols)
+        setattr(a, n, t.data_ptr())
+        setattr(a, "ld" + n, ld)
+        setattr(a, n + "_off", off)
+        setattr(a, n + "_bstride", bs)
+    if key_len is not None:
+        _vector(fn, "key_len", key_len, key_len.numel(), torch.int32, q.device)
+        if key_len.numel() < kv_items:
+            raise dev.AnimaError(1, f"{fn}: {key_len.numel()} key lengths for {kv_items} k/v items")
+        a.key_len = key_len.data_ptr()
+    if out is not None:
+        a.o_bstride = _grad_out(fn, "out", out, batch, Lq, C, o_bstride, q.device)
+        a.out, a.ldo, a.out_dtype = out.data_ptr(), _ld(out), _dt(out)
+    return a, kv_items, Ck
+
+
+def _grad_out(fn, name, t, items, L, cols, bstride, device, dtype=None) -> int:
+    """Check a 2-D [items * L, >= cols] tensor (rows of item b from b * bstride on where that is given)
+    and return its batch stride."""
+    if t.dim() != 2 or t.stride(1) != 1 or t.device != device or t.dtype not in dev.DTYPE_CODE or \
+            (dtype is not None and t.dtype != dtype):
+        raise dev.AnimaError(1, f"{fn}: {name} has to be 2-D with contiguous rows" +
+                                (f", {dtype}" if dtype is not None else "") + f", on {device}; is {t.dtype} "
+                                f"{tuple(t.shape)} on {t.device}")
+    bs = bstride if bstride is not None else L * _ld(t)
+    if bstride is None and t.shape[0] < items * L:
+        raise dev.AnimaError(1, f"{fn}: {name} is {tuple(t.shape)}, expected [{items * L}, {cols}]")
+    _reach(fn, name, t, 0, items, bs, L, _ld(t), cols)
+    return bs
+
+
+def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, Lq: int, Lk: int, H: int, D: int = 128,
+                  ldq: int | None = None, ldk: int | None = None, ldv: int | None = None, q_off: int = 0,
+                  k_off: int = 0, v_off: int = 0, batch: int = 1, q_bstride: int = 0, k_bstride: int = 0,
+                  v_bstride: int = 0, key_len: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  out_dtype=None, o_bstride: int | None = None, scale: float | None = None, group: int = 1,
+                  causal: bool = False, name: str | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """attention() for training: the same arguments (bf16 or fp16 q/k/v, D 64 or 128), and beside the
+    output [batch * Lq, H D] the row statistics lse [batch, H, Lq] that attention_backward needs: ln of
+    each query's sum of exponentials, -inf (with an output of zeros) where it sees no key. k and v may
+    hold anything, NaN included, past key_len. Its workspace comes from torch's allocator, so calls on
+    several streams and captured graphs share nothing."""
+    fn = "attention_lse"
+    if out is None:
+        out = torch.empty(batch * Lq, H * D, dtype=out_dtype or q.dtype, device=q.device)
+    a, _, _ = _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, batch, q_bstride, k_bstride,
+                          v_bstride, key_len, out, o_bstride, scale, group, causal)
+    lse = torch.empty(batch, H, Lq, dtype=torch.float32, device=q.device)
+    ctx = ctx_for(q)
+    need = C.c_size_t()
+    dev.check(ctx.lib.anima_attention_lse_workspace(ctx.h, C.byref(a), C.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    ctx.call("anima_attention_lse", C.byref(a), ptr(lse), ptr(ws), need, tag=name, work=4.0 * batch * Lq * Lk * D * H)
+    return out, lse
+
+
+def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                       lse: torch.Tensor, *, Lq: int, Lk: int, H: int, D: int = 128, ldq: int | None = None,
+                       ldk: int | None = None, ldv: int | None = None, q_off: int = 0, k_off: int = 0, v_off: int = 0,
+                       batch: int = 1, q_bstride: int = 0, k_bstride: int = 0, v_bstride: int = 0,
+                       key_len: torch.Tensor | None = None, o_bstride: int | None = None, scale: float | None = None,
+                       group: int = 1, causal: bool = False, do_bstride: int | None = None,
+                       dq: torch.Tensor | None = None, dk: torch.Tensor | None = None, dv: torch.Tensor | None = None,
+                       grad_dtype=None, name: str | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients (dq, dk, dv) of attention_lse's q, k and v for the gradient dout [batch * Lq, H D] of
+    its output; out and lse are what it returned, the rest its arguments. Probabilities are recomputed. dq
+    is [batch * Lq, H D], dk and dv [items * Lk, (H / group) D]: a shared k/v head sums over its q heads,
+    and where the batch shares one K/V (k_bstride = v_bstride = 0) there is one item, the sum over all.
+    Given dq, dk, dv may be slices of one tensor; new ones have grad_dtype (q's type or fp32). Keys past
+    key_len get zeros. The same inputs give the same bits."""
+    fn = "attention_backward"
+    if out.dim() != 2 or dout.dim() != 2:
+        raise dev.AnimaError(1, f"{fn}: out and dout are 2-D [batch * Lq, H D]")
+    a, kv_items, Ck = _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, batch, q_bstride,
+                                  k_bstride, v_bstride, key_len, out, o_bstride, scale, group, causal)
+    dv_ = q.device
+    if lse.dtype != torch.float32 or lse.shape != (batch, H, Lq) or not lse.is_contiguous() or lse.device != dv_:
+        raise dev.AnimaError(1, f"{fn}: lse has to be a dense fp32 [{batch}, {H}, {Lq}] on {dv_}")
+    gt = next((t.dtype for t in (dq, dk, dv) if t is not None), grad_dtype or q.dtype)
+    if gt not in (torch.float32, q.dtype) or grad_dtype not in (None, gt):
+        raise dev.AnimaError(1, f"{fn}: gradients are {gt}, have to be {q.dtype} or fp32 (grad_dtype {grad_dtype})")
+    new = lambda rows, cols: torch.empty(rows, cols, dtype=gt, device=dv_)  # noqa: E731
+    dq = new(batch * Lq, H * D) if dq is None else dq
+    dk = new(kv_items * Lk, Ck) if dk is None else dk
+    dv = new(kv_items * Lk, Ck) if dv is None else dv
+    g = dev.AttentionGradArgs(fwd=a, lse=lse.data_ptr(), grad_dtype=dev.DTYPE_CODE[gt])
+    g.do_bstride = _grad_out(fn, "dout", dout, batch, Lq, H * D, do_bstride, dv_, q.dtype)
+    g.dout, g.lddo = dout.data_ptr(), _ld(dout)
+    g.dq_bstride = _grad_out(fn, "dq", dq, batch, Lq, H * D, None, dv_, gt)
+    g.dk_bstride = _grad_out(fn, "dk", dk, kv_items, Lk, Ck, None, dv_, gt)
+    g.dv_bstride = _grad_out(fn, "dv", dv, kv_items, Lk, Ck, None, dv_, gt)
+    g.dq, g.lddq, g.dk, g.lddk, g.dv, g.lddv = (dq.data_ptr(), _ld(dq), dk.data_ptr(), _ld(dk), dv.data_ptr(), _ld(dv))
+    ctx = ctx_for(q)
+    need = C.c_size_t()
+    dev.check(ctx.lib.anima_attention_backward_workspace(ctx.h, C.byref(g), C.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dv_)
+    g.workspace, g.workspace_bytes = ws.data_ptr(), need.value
+    ctx.call("anima_attention_backward", C.byref(g), tag=name, work=10.0 * batch * Lq * Lk * D * H, kernels=2)
+    return dq, dk, dv
+
+
 # ----------------------------------------------------------------------------- model glue
 
 def patchify(latent: torch.Tensor) -> torch.Tensor:

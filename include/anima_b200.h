@@ -308,6 +308,40 @@ int anima_attention(anima_ctx* ctx, const anima_attention_args* a);
  * All calls share the array: calls on one device that overlap on the GPU (any context or stream)
  * race. */
 int anima_attention_noalloc(anima_ctx* ctx, const anima_attention_args* a);
+/* Attention with its backward pass (no reference counterpart: the reference does not train).
+ *
+ * anima_attention_lse: anima_attention that also writes lse [batch, heads, Lq] (fp32), the natural
+ * logarithm of each row's sum of exponentials over its visible keys, -inf where it sees none (its output
+ * row is 0). head_dim 64 or 128, bf16/fp16 q/k/v, on the tensor cores; same arguments otherwise. What
+ * lies in k and v behind key_len may be anything, NaN included. workspace: device memory of the caller
+ * (256-byte aligned) of anima_attention_lse_workspace bytes (0 for most shapes), free again when the
+ * call's work is done; nothing is shared between calls. */
+int anima_attention_lse_workspace(anima_ctx* ctx, const anima_attention_args* a, size_t* bytes);
+int anima_attention_lse(anima_ctx* ctx, const anima_attention_args* a, float* lse, void* workspace,
+                        size_t workspace_bytes);
+/* anima_attention_backward: from dout, the gradient of out, those of q, k and v:
+ *   P = exp(scale q k^T - lse), dS = P (dout v^T - rowsum(dout out)),
+ *   dv = P^T dout, dq = scale dS k, dk = scale dS^T q.
+ * fwd: the forward's arguments, with out as it was written; lse: likewise. dout has q's type, the
+ * gradients q's type or fp32 (grad_dtype). dk and dv have the k/v heads (a shared head sums over its q
+ * heads) and, where k and v are shared by the batch (both batch strides 0), a single item, the sum over
+ * all. Rows of keys past key_len get zeros. dq, dk, dv: head h at columns h * head_dim from the pointer,
+ * rows and items their strides apart (so slices of one q|k|v gradient will do); they must not overlap
+ * the inputs. P and dS are rounded to q's type, sums are fp32; no atomics on the gradients, so the same
+ * inputs give the same bits. All tensors 16-byte aligned with strides that are multiples of 8 elements.
+ * workspace: as above, of anima_attention_backward_workspace bytes. */
+typedef struct {
+  anima_attention_args fwd;
+  const float* lse;
+  const void* dout; long long lddo, do_bstride;
+  int grad_dtype;
+  void* dq; long long lddq, dq_bstride;
+  void* dk; long long lddk, dk_bstride;
+  void* dv; long long lddv, dv_bstride;
+  void* workspace; size_t workspace_bytes;
+} anima_attention_grad_args;
+int anima_attention_backward_workspace(anima_ctx* ctx, const anima_attention_grad_args* g, size_t* bytes);
+int anima_attention_backward(anima_ctx* ctx, const anima_attention_grad_args* g);
 /* ops.elementwise (ops.js:154-160): op 0 copy, 1 add, 2 silu, 3 silu_mul; n fp32 elements. */
 int anima_elementwise(anima_ctx* ctx, int op, const float* a, const float* b, float* y, long long n);
 /* ops.zero (ops.js:89-93). */

@@ -1,0 +1,345 @@
+"""Attention with its backward pass on a B200, against the formulas in 64 bits.
+
+Tolerances are worst-case bounds, element by element, of the roundings that the kernels make. With h
+half a step of the operands' type: P, dS and every output round once to that type (h of their value
+each), and delta is taken from the rounded output (h of sum |dO O|). What is in fp32 (scores, exponents,
+sums of up to a few thousand terms) stays below F = 2^-16 of the magnitudes that are summed."""
+
+import math
+
+import pytest
+import torch
+
+from tests.conftest import pkg
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F = 2.0 ** -16
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return pkg("ops")
+
+
+def randn(seed, *shape, dtype=FP, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def reference(q, k, v, do, *, group=1, causal=False, lens=None, scale=None, dtype, out_dtype=None, grad_dtype=None):
+    """q, do [B, H, Lq, D], k, v [B, Hk, Lk, D] in 64 bits: values and tolerances of out, lse, dq, dk, dv
+    ([B, heads, L, D]; dk and dv of every item on its own)."""
+    B, H, Lq, D = q.shape
+    Lk = k.shape[2]
+    scale = scale or 1 / math.sqrt(D)
+    h = half_step(dtype)
+    ho, hg = (half_step(t or dtype) for t in (out_dtype, grad_dtype))
+    tiny = 2.0 ** -24 if dtype == HF else 0.0  # steps of fp16 below 2^-14 no longer shrink
+    kk, vv = (t.repeat_interleave(group, 1) for t in (k, v))
+    hidden = torch.zeros(B, 1, Lq, Lk, dtype=torch.bool, device=DEV)
+    if causal:
+        hidden |= torch.ones(Lq, Lk, dtype=torch.bool, device=DEV).triu(1)
+    if lens is not None:
+        hidden |= (torch.arange(Lk, device=DEV) >= lens.view(B, 1, 1, 1))
+        gone = (torch.arange(Lk, device=DEV) >= lens.view(B, 1, 1))[..., None]
+        kk, vv = kk.masked_fill(gone, 0.0), vv.masked_fill(gone, 0.0)
+    s = (q @ kk.transpose(-1, -2) * scale).masked_fill(hidden, float("-inf"))
+    lse = torch.logsumexp(s, -1)
+    p = torch.where(torch.isfinite(lse)[..., None], torch.exp(s - lse[..., None]), torch.zeros_like(s))
+    out = p @ vv
+    dv = p.transpose(-1, -2) @ do
+    dp = do @ vv.transpose(-1, -2)
+    delta = (do * out).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    dq, dk = ds @ kk * scale, ds.transpose(-1, -2) @ q * scale
+    # bounds. e_p: of P itself, from scores in fp32
+    s_abs = (q.abs() @ kk.abs().transpose(-1, -2) * scale).masked_fill(hidden, 0.0)
+    e_p = F + 2.0 ** -20 * s_abs
+    e_out = ((h + e_p) * p + tiny * ~hidden) @ vv.abs() + ho * out.abs() + tiny
+    e_delta = (do.abs() * (e_out + F * out.abs())).sum(-1, keepdim=True)
+    dp_abs = do.abs() @ vv.abs().transpose(-1, -2)
+    bound = 2 * do.norm(dim=-1).amax() * v.nan_to_num(0).norm(dim=-1).amax() if tiny else 0.0
+    e_ds = (h + e_p) * ds.abs() + p * (e_delta + F * dp_abs + e_p * delta.abs()) + 2.0 ** -38 * bound
+    e_ds = e_ds.masked_fill(hidden, 0.0)
+    rows = lambda e, m, y: scale * (e @ m.abs()) + hg * y.abs() + tiny  # noqa: E731
+    T = lambda t: t.transpose(-1, -2)  # noqa: E731
+    tol = {"out": e_out, "lse": 2.0 ** -20 * (4 + s_abs.amax(-1) + lse.nan_to_num(0, 0, 0).abs()),
+           "dq": rows(e_ds + F * ds.abs(), kk, dq), "dk": rows(T(e_ds + F * ds.abs()), q, dk),
+           "dv": T((h + e_p) * p) @ do.abs() + hg * dv.abs() + tiny}
+    val = {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+    for n in ("dk", "dv"):  # shared heads
+        for t in (val, tol):
+            t[n] = t[n].view(B, H // group, group, Lk, D).sum(2)
+    return val, tol
+
+
+def check(got, val, tol, names=("out", "lse", "dq", "dk", "dv")):
+    for n in names:
+        g, r = got[n].double(), val[n]
+        same = (g == r) | ((g - r).abs() <= tol[n])
+        assert bool(same.all()), (n, (g - r).abs().nan_to_num(9e9).sub(tol[n]).max().item(), (~same).sum().item())
+
+
+class Case:
+    """Plain [B * L, heads * D] tensors of one problem, the call's arguments, and the reference's views."""
+
+    def __init__(self, B, H, group, D, Lq, Lk, dtype, *, causal=False, lens=None, seed=0, gscale=1.0, sharp=1.0):
+        self.B, self.H, self.Hk, self.D, self.Lq, self.Lk, self.dtype = B, H, H // group, D, Lq, Lk, dtype
+        self.q = randn(seed + 1, B * Lq, H * D, dtype=dtype, scale=sharp)
+        self.k = randn(seed + 2, B * Lk, self.Hk * D, dtype=dtype, scale=sharp)
+        self.v = randn(seed + 3, B * Lk, self.Hk * D, dtype=dtype)
+        self.do = randn(seed + 4, B * Lq, H * D, dtype=dtype, scale=gscale)
+        self.lens = torch.tensor(lens, dtype=torch.int32, device=DEV) if lens is not None else None
+        self.kw = dict(Lq=Lq, Lk=Lk, H=H, D=D, batch=B, group=group, causal=causal, key_len=self.lens,
+                       q_bstride=Lq * H * D, k_bstride=Lk * self.Hk * D, v_bstride=Lk * self.Hk * D)
+        self.ref_kw = dict(group=group, causal=causal, lens=self.lens, dtype=dtype)
+
+    def heads(self, t, L):
+        return t.view(self.B, L, -1, self.D).transpose(1, 2)
+
+    def reference(self, **kw):
+        a = [self.heads(t, L).double() for t, L in ((self.q, self.Lq), (self.k, self.Lk), (self.v, self.Lk), (self.do, self.Lq))]
+        return reference(*a, **{**self.ref_kw, **kw})
+
+    def run(self, ops, fwd={}, bwd={}):
+        out, lse = ops.attention_lse(self.q, self.k, self.v, **self.kw, **fwd)
+        dq, dk, dv = ops.attention_backward(self.do, self.q, self.k, self.v, out, lse, **self.kw, **bwd)
+        return {"out": self.heads(out, self.Lq), "lse": lse, "dq": self.heads(dq, self.Lq),
+                "dk": self.heads(dk, self.Lk), "dv": self.heads(dv, self.Lk)}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("Lq,Lk", [(1, 1), (1, 77), (77, 1), (77, 77), (128, 128), (129, 257), (300, 64), (513, 1000),
+                                   (64, 2048), (2048, 64), (255, 256)])
+def test_lengths(ops, dtype, D, Lq, Lk):
+    c = Case(1, 2, 1, D, Lq, Lk, dtype)
+    check(c.run(ops), *c.reference())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("Lq,Lk", [(1, 1), (2, 2), (77, 77), (128, 128), (300, 300), (129, 500), (500, 129), (1025, 1025)])
+def test_causal_shared_heads(ops, dtype, D, Lq, Lk):
+    c = Case(2, 4, 2, D, Lq, Lk, dtype, causal=True)
+    check(c.run(ops), *c.reference())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Lq,Lk,lens", [(200, 333, (333, 129, 1, 0)), (130, 256, (128, 256, 500, -3)), (64, 700, (1, 640, 699, 513))])
+def test_key_lengths(ops, dtype, D, causal, Lq, Lk, lens):
+    c = Case(4, 4, 4, D, Lq, Lk, dtype, causal=causal, lens=lens)
+    val, tol = c.reference()
+    got = c.run(ops)
+    check(got, val, tol)
+    for b, n in enumerate(lens):  # nothing flows past them, and rows that see no key have lse = -inf
+        n = max(0, min(n, Lk))
+        assert bool((got["dk"][b, :, n:] == 0).all() and (got["dv"][b, :, n:] == 0).all())
+        if n == 0:
+            assert bool((got["out"][b] == 0).all() and (got["dq"][b] == 0).all() and got["lse"][b].eq(-math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -6e4])
+def test_what_lies_behind_key_len_does_not_count(ops, dtype, D, bad):
+    lens = (131, 200, 64)
+    c = Case(3, 2, 1, D, 150, 260, dtype, lens=lens)
+    ref = c.run(ops)
+    for b, n in enumerate(lens):
+        for t in (c.k, c.v):
+            t.view(3, 260, -1)[b, n:] = bad
+    got = c.run(ops)
+    for n in ref:
+        assert torch.equal(ref[n], got[n]), n
+    # so it is with attention() on the same kernel
+    if D == 128:
+        assert torch.equal(ops.attention(c.q, c.k, c.v, **c.kw), ref["out"].transpose(1, 2).reshape(3 * 150, -1))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_packed_gradients_strides_and_neighbours(ops, dtype):
+    """q|k|v in one tensor, its gradient likewise, rows with a gap behind them; what is not a gradient
+    stays as it was."""
+    B, L, H, D = 2, 150, 4, 64
+    C = H * D
+    x = randn(1, B * L, 3 * C + 8, dtype=dtype)
+    do = randn(2, B * L, C, dtype=dtype)
+    ld = 3 * C + 8
+    kw = dict(Lq=L, Lk=L, H=H, D=D, batch=B, ldq=ld, ldk=ld, ldv=ld, q_off=0, k_off=C, v_off=2 * C, q_bstride=L * ld,
+              k_bstride=L * ld, v_bstride=L * ld)
+    wide = torch.full((B * L, C + 16), 3.0, dtype=dtype, device=DEV)
+    out, lse = ops.attention_lse(x, x, x, out=wide[:, 8:C + 8], **kw)
+    dx = torch.full((B * L + 1, ld), 7.0, dtype=dtype, device=DEV)
+    d = [dx[:B * L, i * C:(i + 1) * C] for i in range(3)]
+    got = ops.attention_backward(do, x, x, x, out, lse, dq=d[0], dk=d[1], dv=d[2], **kw)
+    assert all(a is b for a, b in zip(got, d))
+    view = lambda t: t.reshape(B, L, H, D).transpose(1, 2)  # noqa: E731
+    val, tol = reference(*(view(x[:, i * C:(i + 1) * C]).double() for i in range(3)), view(do).double(), dtype=dtype)
+    check({"out": view(out), "lse": lse, "dq": view(d[0]), "dk": view(d[1]), "dv": view(d[2])}, val, tol)
+    assert bool((dx[:, 3 * C:] == 7).all() and (dx[B * L] == 7).all())
+    assert bool((wide[:, :8] == 3).all() and (wide[:, C + 8:] == 3).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("Lq,Lk", [(200, 130), (70, 600)])
+def test_shared_kv_sums_over_the_batch(ops, dtype, Lq, Lk):
+    """k_bstride = v_bstride = 0: all items read one K/V (and key_len[0]); its gradient is the sum."""
+    B, H, D = 3, 2, 64
+    c = Case(B, H, 1, D, Lq, Lk, dtype, lens=(Lk - 5,) * B)
+    for t in (c.k, c.v):
+        t.view(B, Lk, -1)[1:] = t.view(B, Lk, -1)[0]
+    val, tol = c.reference()
+    one = {"k": c.k[:Lk].contiguous(), "v": c.v[:Lk].contiguous()}
+    kw = {**c.kw, "k_bstride": 0, "v_bstride": 0, "key_len": c.lens[:1]}
+    out, lse = ops.attention_lse(c.q, one["k"], one["v"], **kw)
+    dq, dk, dv = ops.attention_backward(c.do, c.q, one["k"], one["v"], out, lse, **kw)
+    assert dk.shape == (Lk, H * D)
+    check({"out": c.heads(out, Lq), "lse": lse, "dq": c.heads(dq, Lq)}, val, tol, ("out", "lse", "dq"))
+    for n, g in (("dk", dk), ("dv", dv)):
+        assert bool(((g.view(Lk, H, D).transpose(0, 1).double() - val[n].sum(0)).abs() <= tol[n].sum(0)).all()), n
+
+
+@pytest.mark.parametrize("out_dtype", [None, FP])
+@pytest.mark.parametrize("grad_dtype", [None, FP])
+def test_fp32_output_and_gradients(ops, out_dtype, grad_dtype):
+    c = Case(1, 2, 1, 128, 200, 1030, BF)
+    got = c.run(ops, dict(out_dtype=out_dtype), dict(grad_dtype=grad_dtype))
+    assert got["out"].dtype == (out_dtype or BF) and got["dq"].dtype == got["dk"].dtype == (grad_dtype or BF)
+    check(got, *c.reference(out_dtype=out_dtype, grad_dtype=grad_dtype))
+
+
+@pytest.mark.parametrize("gscale", [1e-6, 1e-3, 300.0])
+def test_fp16_gradients_of_any_size(ops, gscale):
+    """dS is moved into fp16's range by a power of two: gradients in fp32 keep their digits whatever
+    the size of dout (whose own subnormals are exact inputs)."""
+    c = Case(1, 2, 1, 64, 260, 2000, HF, gscale=gscale)
+    got = c.run(ops, dict(out_dtype=FP), dict(grad_dtype=FP))
+    val, _ = c.reference()
+    for n in ("dq", "dk", "dv"):
+        # |dP - delta| P near 2^-11 of the bound, 2^4 above fp16's subnormals: steps of 2^-11 each
+        assert ((got[n].double() - val[n]).norm() / val[n].norm()).item() < 2 * half_step(HF), n
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scale_and_sharp_rows(ops, dtype):
+    """Another softmax scale, and scores so far apart that most probabilities are 0 or 1."""
+    c = Case(1, 2, 1, 64, 140, 300, dtype, sharp=3.0)
+    c.kw["scale"] = 0.5
+    check(c.run(ops), *c.reference(scale=0.5))
+
+
+def test_against_differences(ops):
+    """The loss sum(out w), out in fp32, moves as dq, dk and dv say. bf16 inputs leave whole steps to
+    move by: an element of q, k or v changes by 1/8, the slope's error is cubic."""
+    c = Case(1, 1, 1, 64, 40, 50, BF, seed=5)
+    for n in "qkv":
+        setattr(c, n, (getattr(c, n) * 8).round().div(8).clamp(-3, 3))  # so that +- 1/8 is exact in bf16
+    got = c.run(ops, {}, dict(grad_dtype=FP))
+
+    def loss():
+        out, _ = ops.attention_lse(c.q, c.k, c.v, out_dtype=FP, **c.kw)
+        return (out.double() * c.do.double()).sum().item()
+
+    for n, L in (("q", 40), ("k", 50), ("v", 50)):
+        t, keep = getattr(c, n), getattr(c, n).clone()
+        d = (randn(9, *t.shape) > 0).to(BF) * 0.25 - 0.125
+        t.copy_(keep + d)
+        up = loss()
+        t.copy_(keep - d)
+        slope = (up - loss()) / 2
+        t.copy_(keep)
+        g = got["d" + n].transpose(1, 2).reshape(L, -1).double()
+        # third-order term of a step of 1/8 in every element: scores move by up to 1/8 sqrt(64) / 8, a few
+        # per cent of the slope's own size, which for random signs is |g| / 8
+        assert abs(slope - (g * d.double()).sum().item()) <= 0.2 * g.norm().item() * 0.125 * 2, n
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_same_bits_again(ops, causal):
+    c = Case(1, 8, 2, 128, 1500, 1500, BF, causal=causal)
+    a, b = c.run(ops), c.run(ops)
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
+
+
+def test_long_self_attention_stream_k(ops):
+    """4096 tokens of 16 heads, the key blocks spread over the SMs: the output has attention()'s bits,
+    two heads are compared in full, and the workspace is the call's own."""
+    c = Case(1, 16, 1, 128, 4096, 4096, HF)
+    got = c.run(ops)
+    assert torch.equal(ops.attention(c.q, c.k, c.v, **c.kw), got["out"].transpose(1, 2).reshape(4096, -1))
+    for h in (0, 11):
+        one = [c.heads(t, 4096)[:, h:h + 1].double() for t in (c.q, c.k, c.v, c.do)]
+        val, tol = reference(*one, dtype=HF)
+        check({n: t[:, h:h + 1] for n, t in got.items()}, val, tol)
+
+
+def test_captured_replayed_and_two_at_once(ops):
+    """Two graphs of the same step hold workspaces of their own: replayed at the same time on two
+    streams, on inputs that came after the capture, both give the eager bits."""
+    c = Case(2, 4, 2, 128, 700, 900, BF, lens=(900, 333))
+    c.run(ops)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(c.run(ops))
+    for n in ("q", "k", "v", "do"):
+        getattr(c, n).copy_(randn(77, *getattr(c, n).shape, dtype=BF))
+    c.lens.copy_(torch.tensor([640, 0], dtype=torch.int32))
+    want = c.run(ops)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for g, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    for got in outs:
+        for n in want:
+            assert torch.equal(got[n], want[n]), n
+    check(want, *c.reference())
+    with torch.cuda.stream(streams[0]):
+        side = c.run(ops)
+    torch.cuda.synchronize()
+    for n in want:
+        assert torch.equal(side[n], want[n]), n
+
+
+def test_offsets_past_32_bits(ops):
+    """Items 2^31 + 1024 elements apart."""
+    bs = 2 ** 31 + 1024
+    H, D, L = 1, 64, 100
+    c = Case(2, H, 1, D, L, L, BF)
+    kw = {**c.kw, "q_bstride": bs, "k_bstride": bs, "v_bstride": bs, "ldq": 3 * D, "ldk": 3 * D, "ldv": 3 * D, "q_off": 0,
+          "k_off": D, "v_off": 2 * D}
+    far = torch.empty(bs + L * 3 * D, dtype=BF, device=DEV)
+    for b in range(2):
+        rows = far[b * bs:b * bs + L * 3 * D].view(L, 3 * D)
+        for i, t in enumerate((c.q, c.k, c.v)):
+            rows[:, i * D:(i + 1) * D] = t[b * L:(b + 1) * L]
+    out, lse = ops.attention_lse(far, far, far, **kw)
+    dq, dk, dv = ops.attention_backward(c.do, far, far, far, out, lse, **kw)
+    want = c.run(ops)
+    for n, t in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        assert torch.equal(c.heads(t, L), want[n]), n
+
+
+def test_library_refusals(ops):
+    err = pkg("device").AnimaError
+    c = Case(1, 2, 1, 64, 32, 32, BF)
+    odd = torch.empty(33 * 128 + 4, dtype=BF, device=DEV)[4:].as_strided((32, 128), (128, 1))
+    with pytest.raises(err, match="aligned"):
+        ops.attention_lse(odd, c.k, c.v, **c.kw)
+    out, lse = ops.attention_lse(c.q, c.k, c.v, **c.kw)
+    with pytest.raises(err, match="aligned"):
+        ops.attention_backward(c.do, c.q, c.k, c.v, out, lse, dq=odd, **c.kw)

@@ -24,7 +24,8 @@ def err():
 
 def test_structs_match_the_c_header(tmp_path):
     dev = pkg("device")
-    structs = {"anima_rotary_args": dev.RotaryArgs, "anima_residual_norm_args": dev.ResidualNormArgs}
+    structs = {"anima_rotary_args": dev.RotaryArgs, "anima_residual_norm_args": dev.ResidualNormArgs,
+               "anima_attention_grad_args": dev.AttentionGradArgs}
     cc = shutil.which("gcc") or shutil.which("cc")
     if cc is None:
         pytest.skip("no C compiler")
@@ -124,4 +125,39 @@ def test_residual_norm_backward_refuses(ops, err, change):
     kw = dict(dh=t(6, 16), dx_out=t(6, 16), x_out=t(6, 16), y=t(6, 16), rows_per_item=3, gate=t(2, 16))
     with pytest.raises(err) as e:
         ops.residual_norm_backward(**{**kw, **change})
+    assert e.value.status == 1
+
+
+ATTN_BAD = [
+    dict(Lq=0), dict(Lk=0), dict(H=3, group=2), dict(H=0), dict(batch=0), dict(D=96), dict(q=t(20, 128)),
+    dict(k=t(24, 64, dtype=torch.float16)), dict(q=t(19, 128, dtype=torch.bfloat16)), dict(k=t(23, 64, dtype=torch.bfloat16)),
+    dict(ldq=64), dict(ldk=32), dict(q_off=-8), dict(q_off=8), dict(v_off=64), dict(k_bstride=0), dict(v_bstride=-64),
+    dict(q_bstride=11 * 128), dict(key_len=t(2)), dict(key_len=t(1, dtype=torch.int32)),
+]
+
+
+def attn_kw():
+    b = dict(dtype=torch.bfloat16)
+    return dict(q=t(20, 128, **b), k=t(24, 64, **b), v=t(24, 64, **b), Lq=10, Lk=12, H=2, D=64, group=2, batch=2,
+                q_bstride=1280, k_bstride=768, v_bstride=768)
+
+
+@pytest.mark.parametrize("change", ATTN_BAD + [dict(out=t(19, 128)), dict(out=t(20, 127)), dict(out=t(20, 256).T)])
+def test_attention_lse_refuses(ops, err, change):
+    with pytest.raises(err) as e:
+        ops.attention_lse(**{**attn_kw(), **change})
+    assert e.value.status == 1
+
+
+@pytest.mark.parametrize("change", ATTN_BAD + [
+    dict(out=t(19, 128)), dict(dout=t(20, 128)), dict(dout=t(19, 128, dtype=torch.bfloat16)), dict(lse=t(2, 2, 9)),
+    dict(lse=t(2, 2, 10, dtype=torch.float64)), dict(lse=t(2, 10, 2).transpose(1, 2)), dict(dq=t(20, 127)),
+    dict(dk=t(24, 64), dv=t(24, 64, dtype=torch.bfloat16)), dict(dk=t(23, 64)), dict(dq=t(20, 128, dtype=torch.float16)),
+    dict(grad_dtype=torch.float16), dict(dq=t(20, 128), grad_dtype=torch.bfloat16), dict(dout=t(2, 10, 128, dtype=torch.bfloat16)),
+])
+def test_attention_backward_refuses(ops, err, change):
+    b = dict(dtype=torch.bfloat16)
+    kw = dict(dout=t(20, 128, **b), out=t(20, 128, **b), lse=t(2, 2, 10), **attn_kw())
+    with pytest.raises(err) as e:
+        ops.attention_backward(**{**kw, **change})
     assert e.value.status == 1
