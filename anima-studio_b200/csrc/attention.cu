@@ -64,8 +64,7 @@ struct Params {
   int persist;       // whole units, CTA c taking units c, c + grid, ... (grid = SM count)
   int group;         // q heads per k/v head (k/v head = h / group)
   int causal;        // key j visible to query i only when j <= i
-  int zero_tail;     // key_len given: V's rows past it are zeroed before P V (0 x NaN is not 0)
-  float* lse;        // [batch][heads][Lq] ln of each row's sum of exponentials, or NULL
+  float* lse;        // TRAIN: [batch][heads][Lq] ln of each row's sum of exponentials
   float* ws;         // [units][PART_FLOATS] partial softmax states of split units
   unsigned* flags;   // [units] tail part written (cleared by the head part)
 };
@@ -205,7 +204,9 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 }
 
 // 18 warps are allocated registers as 20: 96 x 32 x 20 = 61440 of the SM's 65536
-template <bool BF16, int HD>
+// TRAIN: also writes lse, and clears V's rows behind key_len in shared memory (P is 0 there, but 0 x NaN
+// is not).
+template <bool BF16, int HD, bool TRAIN>
 __global__ void __launch_bounds__(THREADS, 1)
     attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const Params p) {
@@ -224,7 +225,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* o_done = bars + 13;  // [2] per tile: PV_X(j) complete
   uint64_t* drain = bars + 15;
   uint64_t* q_empty = bars + 16;  // the segment's last QK^T has completed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint64_t* v_tail = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* nseg_slot = reinterpret_cast<int*>(tmem_slot + 2);
   int4* segs = reinterpret_cast<int4*>(smem + OFF_SEG);
@@ -234,6 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
+    mbar_init(v_tail, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -260,14 +263,20 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int nseg = *nseg_slot;
 
   if (warp == kProducerWarp) {
-    if (lane == 0) {
+    // TRAIN: all lanes follow (they clear rows together), waits have one outcome for the warp
+    if (TRAIN || lane == 0) {
+      auto wait = [&](uint64_t* wb, uint32_t ph, unsigned err) {
+        const bool done = mbar_wait(wb, ph, abort_flag, err);
+        return TRAIN ? __all_sync(0xffffffffu, done) != 0 : done;
+      };
+      const bool lead = !TRAIN || lane == 0;
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
       // the last arm of q_full, k_full[0], k_full[1], v_full[0], v_full[1]: 2 bits each (armed, parity)
       uint32_t armed = 0;
       auto arm = [&](int i, uint32_t ph) { armed = (armed & ~(3u << (2 * i))) | ((2u | ph) << (2 * i)); };
-      int gb = 0, qn = 0;                   // key blocks and Q loads so far
+      int gb = 0, qn = 0, tails = 0;        // key blocks, Q loads and cleared V blocks so far
       for (int si = 0; si < nseg && !*abort_flag; ++si) {
         const int4 sg = segs[si];  // unit, kb0, kb1, kind
         const int qp = sg.x % p.q_pairs, bh = sg.x / p.q_pairs;
@@ -277,40 +286,64 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (nb <= 0) continue;
         const int q0 = qp * 2 * TILE;
         const int qc = p.q_col + h * HD, kc = p.k_col + (h / p.group) * HD, vc = p.v_col + (h / p.group) * HD;
-        if (qn > 0 && !mbar_wait(q_empty, (qn - 1) & 1, abort_flag, kErrTimeoutEmpty)) break;
-        mbar_arrive_expect_tx(q_full, 2 * ATOMS * ATOM);
+        if (qn > 0 && !wait(q_empty, (qn - 1) & 1, kErrTimeoutEmpty)) break;
+        if (lead) {
+          mbar_arrive_expect_tx(q_full, 2 * ATOMS * ATOM);
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int t = 0; t < ATOMS; ++t)
-            tma_load_3d(smem + OFF_Q + x * TILE_BYTES + t * ATOM, &tm_q, q_full, qc + 64 * t, q0 + x * TILE, b);
+            for (int t = 0; t < ATOMS; ++t)
+              tma_load_3d(smem + OFF_Q + x * TILE_BYTES + t * ATOM, &tm_q, q_full, qc + 64 * t, q0 + x * TILE, b);
+        }
         arm(0, qn & 1);
         ++qn;
         for (int j = 0; j < nb; ++j) {
           const int G = gb + j, kb = sg.y + j;
           const int st = G & 1;
           const uint32_t ph = (G >> 1) & 1;
-          if (!mbar_wait(&k_empty[st], ph ^ 1, abort_flag, kErrTimeoutEmpty)) break;
-          mbar_arrive_expect_tx(&k_full[st], ATOMS * ATOM);
+          if (!wait(&k_empty[st], ph ^ 1, kErrTimeoutEmpty)) break;
+          if (lead) {
+            mbar_arrive_expect_tx(&k_full[st], ATOMS * ATOM);
 #pragma unroll
-          for (int t = 0; t < ATOMS; ++t)
-            tma_load_3d(smem + OFF_K + st * TILE_BYTES + t * ATOM, &tm_k, &k_full[st], kc + 64 * t, kb * TILE, kvb);
+            for (int t = 0; t < ATOMS; ++t)
+              tma_load_3d(smem + OFF_K + st * TILE_BYTES + t * ATOM, &tm_k, &k_full[st], kc + 64 * t, kb * TILE, kvb);
+          }
           arm(1 + st, ph);
-          if (!mbar_wait(&v_empty[st], ph ^ 1, abort_flag, kErrTimeoutEmpty)) break;
-          mbar_arrive_expect_tx(&v_full[st], ATOMS * ATOM);
+          if (!wait(&v_empty[st], ph ^ 1, kErrTimeoutEmpty)) break;
+          // the block that key_len ends in: V lands on a barrier of its own, its hidden rows are cleared,
+          // and only then is it full
+          const int left = TRAIN && p.key_len ? min(p.Lk, p.key_len[kvb]) - kb * TILE : TILE;
+          uint64_t* vb = left < TILE ? v_tail : &v_full[st];
+          if (lead) {
+            mbar_arrive_expect_tx(vb, ATOMS * ATOM);
 #pragma unroll
-          for (int t = 0; t < ATOMS; ++t)
-            tma_load_3d(smem + OFF_V + st * TILE_BYTES + t * ATOM, &tm_v, &v_full[st], vc + 64 * t, kb * TILE, kvb);
+            for (int t = 0; t < ATOMS; ++t)
+              tma_load_3d(smem + OFF_V + st * TILE_BYTES + t * ATOM, &tm_v, vb, vc + 64 * t, kb * TILE, kvb);
+          }
+          if (TRAIN && left < TILE) {
+            if (!wait(v_tail, tails & 1, kErrTimeoutFull)) {
+              arm(5, tails & 1);
+              break;
+            }
+            ++tails;
+            const int n = (TILE - left) * 8;  // 16-byte pieces of an atom's rows
+            for (int c = lane; c < n * ATOMS; c += 32)
+              *reinterpret_cast<uint4*>(smem + OFF_V + st * TILE_BYTES + (c / n) * ATOM + left * 128 + (c % n) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lead) mbar_arrive(&v_full[st]);
+          }
           arm(3 + st, ph);
         }
         gb += nb;
       }
       if (*abort_flag) {
         // let every copy this thread started land before the CTA exits
-        for (int i = 0; i < 5; ++i) {
+        for (int i = 0; i < 6; ++i) {
           const uint32_t a = (armed >> (2 * i)) & 3u;
           if (!(a & 2u)) continue;
-          uint64_t* fb = bars + (i < 3 ? i : i + 2);  // q_full, k_full[0..1], v_full[0..1]
+          uint64_t* fb = i == 5 ? v_tail : bars + (i < 3 ? i : i + 2);  // q_full, k_full[0..1], v_full[0..1], v_tail
           const unsigned long long t0 = globaltimer();
           while (!mbar_test(smem_u32(fb), a & 1u)) {
             if (globaltimer() - t0 > kWaitTimeoutNs) {
@@ -440,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                (HD / 2) * hf;
       };
       auto put_lse = [&](int qrow, float v) {  // one of a row's two warps
-        if (p.lse && hf == 0 && qrow < p.Lq) p.lse[static_cast<size_t>(segs[si].x / p.q_pairs) * p.Lq + qrow] = v;
+        if (TRAIN && hf == 0 && qrow < p.Lq) p.lse[static_cast<size_t>(segs[si].x / p.q_pairs) * p.Lq + qrow] = v;
       };
       if (nb <= 0) {
         int qrow;
@@ -547,22 +580,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int t = 0; t < 32; ++t) orr[t] = __float_as_uint(__uint_as_float(orr[t]) * alpha);
             tmem_st32(o_addr + 32 * c, orr);
-          }
-        }
-        if (p.zero_tail && masked) {
-          // the block that key_len ends in: what lies behind may be anything, and the tensor core
-          // multiplies it by P = 0. Each tile's warps clear all of V's hidden rows before their P V.
-          const int left = min(p.Lk, p.key_len[p.kv_bcast ? 0 : segs[si].x / p.q_pairs / p.heads]) - (kb0 + j) * TILE;
-          if (left < TILE) {
-            if (!warp_wait(&v_full[jp], (G >> 1) & 1, abort_flag, kErrTimeoutFull)) {
-              ok = false;
-              continue;
-            }
-            const int n = (TILE - left) * 8;  // 16-byte pieces of an atom's rows
-            for (int t = (warp & 7) * 32 + lane; t < n * ATOMS; t += 256)
-              *reinterpret_cast<uint4*>(smem + OFF_V + jp * TILE_BYTES + (t / n) * ATOM + left * 128 + (t % n) * 16) =
-                  make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
           }
         }
         tmem_st_wait();
@@ -1075,7 +1092,6 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratc
   p.o_bstride = a->batch > 1 ? a->o_bstride : 0;
   p.out_dtype = a->out_dtype;
   p.key_len = a->key_len;
-  p.zero_tail = a->key_len ? 1 : 0;
   p.lse = lse;
   p.kv_bcast = kv_bcast ? 1 : 0;
   p.group = group;
@@ -1120,9 +1136,10 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratc
                  4.0 * a->batch * a->heads * static_cast<double>(a->Lq) * a->Lk * a->head_dim, 0);
   using Kfn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const attn::Params);
   const int kind = a->dtype == ANIMA_BF16 ? 1 : 0;
-  const Kfn fns[2][2] = {{attn::attention_kernel<false, 128>, attn::attention_kernel<true, 128>},
-                         {attn::attention_kernel<false, 64>, attn::attention_kernel<true, 64>}};
-  const Kfn fn = fns[a->head_dim == 64][kind];
+  const Kfn fns[3][2] = {{attn::attention_kernel<false, 128, false>, attn::attention_kernel<true, 128, false>},
+                         {attn::attention_kernel<false, 128, true>, attn::attention_kernel<true, 128, true>},
+                         {attn::attention_kernel<false, 64, true>, attn::attention_kernel<true, 64, true>}};
+  const Kfn fn = fns[!lse ? 0 : a->head_dim == 128 ? 1 : 2][kind];
   {
     int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), attn::SMEM_BYTES);
     if (st) return st;

@@ -94,6 +94,11 @@ __device__ __forceinline__ float ds_scale(const Params& p, int kv_head) {
   return ldexpf(1.f, e);
 }
 
+// Blocks that a mask cuts and whole ones are two copies of the code: the selects cost a whole block a
+// third of its issue slots.
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
 struct Bars {
   uint64_t *x_full, *y0_full, *y1_full, *y0_empty, *y1_empty, *s_full, *dp_full, *p_full, *ds_full, *acc_done, *drain;
 };
@@ -419,11 +424,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                    warp_wait(bar.s_full, i & 1, abort_flag, kErrTimeoutFull)))
           break;
         tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[32];
-          tmem_ld32(t_s + lane_addr + 64 * hf + 32 * c, r);
-          tmem_ld_wait(r);
+        const uint32_t ts = t_s + lane_addr + 64 * hf, td = t_dp + lane_addr + 64 * hf;
+        auto probabilities = [&](auto mask, const uint32_t(&r)[32], int c) {
           uint32_t pk[16];
 #pragma unroll
           for (int t = 0; t < 32; t += 4) {
@@ -432,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const f2 a1 =
                 fma2(make_float2(__uint_as_float(r[t + 2]), __uint_as_float(r[t + 3])), sc2, make_float2(l.z, l.w));
             float e[4] = {ex2(a0.x), ex2(a0.y), ex2(a1.x), ex2(a1.y)};
-            if (masked) {
+            if constexpr (decltype(mask)::value) {
 #pragma unroll
               for (int u = 0; u < 4; ++u)
                 if (64 * hf + 32 * c + t + u < first) e[u] = 0.f;
@@ -442,7 +444,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             pk[t / 2] = pack2<BF16>(e[0], e[1]);
             pk[t / 2 + 1] = pack2<BF16>(e[2], e[3]);
           }
-          tmem_st16(t_s + lane_addr + 64 * hf + 16 * c, pk);
+          tmem_st16(ts + 16 * c, pk);
+        };
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld32(ts, r0);
+          tmem_ld_wait(r0);
+          tmem_ld32(ts + 32, r1);  // in flight while the first half is computed
+          if (masked) probabilities(Yes{}, r0, 0); else probabilities(No{}, r0, 0);
+          tmem_ld_wait(r1);
+          if (masked) probabilities(Yes{}, r1, 1); else probabilities(No{}, r1, 1);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -450,11 +461,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         arrive_one_lane(bar.p_full);
         if (!(ok = warp_wait(bar.dp_full, i & 1, abort_flag, kErrTimeoutFull))) break;
         tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[32];
-          tmem_ld32(t_dp + lane_addr + 64 * hf + 32 * c, r);
-          tmem_ld_wait(r);
+        auto gradients = [&](auto mask, const uint32_t(&r)[32], int c) {
           uint32_t pk[16];
 #pragma unroll
           for (int t = 0; t < 32; t += 4) {
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!BF16) p0 = mul2(p0, c2), p1 = mul2(p1, c2);
             g0 = mul2(g0, p0);
             g1 = mul2(g1, p1);
-            if (masked) {  // 0 whatever dP is
+            if constexpr (decltype(mask)::value) {  // 0 whatever dP is
               const int q = 64 * hf + 32 * c + t;
               if (q < first) g0.x = 0.f;
               if (q + 1 < first) g0.y = 0.f;
@@ -475,7 +482,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             pk[t / 2] = pack2<BF16>(g0.x, g0.y);
             pk[t / 2 + 1] = pack2<BF16>(g1.x, g1.y);
           }
-          tmem_st16(t_dp + lane_addr + 64 * hf + 16 * c, pk);
+          tmem_st16(td + 16 * c, pk);
+        };
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld32(td, r0);
+          tmem_ld_wait(r0);
+          tmem_ld32(td + 32, r1);
+          if (masked) gradients(Yes{}, r0, 0); else gradients(No{}, r0, 0);
+          tmem_ld_wait(r1);
+          if (masked) gradients(Yes{}, r1, 1); else gradients(No{}, r1, 1);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -489,28 +505,29 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int left = kv_len - kb * TILE;
         const bool masked = left < TILE || (p.causal && kb == w.blk);
         const int end = p.causal && kb == w.blk ? min(left, row + 1) : left;
-        const uint32_t ts = (i & 1 ? t_s1 : t_s) + lane_addr + 64 * hf;
+        const uint32_t ts = (i & 1 ? t_s1 : t_s) + lane_addr + 64 * hf, td = t_dp + lane_addr + 64 * hf;
         if (!(ok = warp_wait(&bar.s_full[i & 1], (i >> 1) & 1, abort_flag, kErrTimeoutFull))) break;
         tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[32];
-          tmem_ld32(ts + 32 * c, r);
-          tmem_ld_wait(r);
+        auto probabilities = [&](const uint32_t(&r)[32], int c) {
 #pragma unroll
           for (int t = 0; t < 32; t += 2) {
             const f2 a = fma2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, nlse2);
             pr[32 * c + t] = ex2(a.x);
             pr[32 * c + t + 1] = ex2(a.y);
           }
+        };
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld32(ts, r0);
+          tmem_ld_wait(r0);
+          tmem_ld32(ts + 32, r1);
+          probabilities(r0, 0);
+          tmem_ld_wait(r1);
+          probabilities(r1, 1);
         }
         if (!(ok = warp_wait(bar.dp_full, i & 1, abort_flag, kErrTimeoutFull))) break;
         tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[32];
-          tmem_ld32(t_dp + lane_addr + 64 * hf + 32 * c, r);
-          tmem_ld_wait(r);
+        auto gradients = [&](auto mask, const uint32_t(&r)[32], int c) {
           uint32_t pk[16];
 #pragma unroll
           for (int t = 0; t < 32; t += 2) {
@@ -518,13 +535,22 @@ __global__ void __launch_bounds__(THREADS, 1)
             f2 pp = make_float2(pr[32 * c + t], pr[32 * c + t + 1]);
             if (!BF16) pp = mul2(pp, c2);
             g = mul2(g, pp);
-            if (masked) {  // 0 whatever S and dP are
+            if constexpr (decltype(mask)::value) {  // 0 whatever S and dP are
               if (64 * hf + 32 * c + t >= end) g.x = 0.f;
               if (64 * hf + 32 * c + t + 1 >= end) g.y = 0.f;
             }
             pk[t / 2] = pack2<BF16>(g.x, g.y);
           }
-          tmem_st16(t_dp + lane_addr + 64 * hf + 16 * c, pk);
+          tmem_st16(td + 16 * c, pk);
+        };
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld32(td, r0);
+          tmem_ld_wait(r0);
+          tmem_ld32(td + 32, r1);
+          if (masked) gradients(Yes{}, r0, 0); else gradients(No{}, r0, 0);
+          tmem_ld_wait(r1);
+          if (masked) gradients(Yes{}, r1, 1); else gradients(No{}, r1, 1);
         }
         if (left < TILE && p.key_len) {
           // K's rows behind key_len may hold anything, and dS K multiplies them by 0
