@@ -11,17 +11,22 @@
 // gradients need; in return nothing is added up in memory between units, so there are no atomics and
 // the same inputs give the same bits.
 //
-// 320 threads: warps 0-7 turn S and dP into P and dS (warp w: the 32 tensor-memory lanes of quadrant
-// w % 4, column half w / 4), warp 8 loads tiles by TMA, warp 9 allocates tensor memory and issues the
-// products. A k/v unit computes the transposed S^T = K Q^T and dP^T = V dO^T (lanes = keys), so that
+// 576 threads: warps 0-15 turn S and dP into P and dS (warp w: the 32 tensor-memory lanes of quadrant
+// w % 4, column quarter w / 4), warp 16 loads tiles by TMA, warp 17 allocates tensor memory and issues
+// the products. A k/v unit computes the transposed S^T = K Q^T and dP^T = V dO^T (lanes = keys), so that
 // P^T and dS^T, rounded to 16 bits and written back over S^T and dP^T, are the A operand of
 // dV += P^T dO and dK += dS^T Q straight from tensor memory, with the Q and dO tiles that are in
 // shared memory anyway as their MN-major B operand. Issue order per block:
 //   dV(i) S(i+1) [dS(i) written] dK(i) dP(i+1)
 // so the exponentials of block i + 1 overlap dK(i) and dP(i+1), and the products dS(i) overlap dV(i)
-// and S(i+1). A q unit has S twice in tensor memory: dQ(i) dP(i+1) S(i+2).
+// and S(i+1). A q unit has dP twice in tensor memory, and S is read into registers at once, so S(i+1)
+// and dP(i+1) are computed while block i is: S(i+1) dP(i+1) | [dS(i) written] dQ(i).
+// A k/v unit's lse and delta belong to columns, the same for all lanes. Loading them costs dearly there
+// (beside products that read both operands from shared memory, 8 16-byte loads a warp took 5700 cycles
+// for 190), so the tensor core adds them: S^T and dP^T get one more step of 16 inner indices, a constant
+// column times each value's 16-bit parts (three of them: value = hi + mid + low to 2^-24 of it).
 // Tensor memory, k/v unit: S^T [0,128) dP^T [128,256) dV [256,256+D) dK [256+D,256+2D);
-// q unit: S [0,128) and [384,512), dP [128,256), dQ [256,256+D).
+// q unit: S [0,128), dP [128,256) and [384,512), dQ [256,256+D).
 //
 // Roundings. P and dS round to the operands' type before their products (fp32 sums). In fp16 both are
 // moved into its range by powers of two that are undone in fp32: P <= 1 by 2^14; dS by a factor from
@@ -43,10 +48,9 @@ using attn::ATOM;
 using attn::ex2;
 using attn::pack2;
 using attn::TILE;
-using attn::warp_wait;
 
-constexpr int THREADS = 320;
-constexpr int MATH_WARPS = 8;
+constexpr int THREADS = 576;
+constexpr int MATH_WARPS = 16;
 constexpr int TILE_BYTES = 2 * ATOM;  // a tile's slot: 128 rows of 128 16-bit columns (64: half of it is used)
 // shared memory: the unit's two tiles | ring of up to 3 first tiles | ring of 2 second tiles | row
 // statistics of the ring's stages | barriers. A k/v unit: K, V | Q | dO; a q unit: Q, dO | K | V.
@@ -57,11 +61,15 @@ constexpr int OFF_Y1 = OFF_Y0 + Y0_STAGES * TILE_BYTES;
 constexpr int Y1_STAGES = 2;
 // a k/v unit needs only two stages of Q: the third's place holds the statistics
 constexpr int KV_Y0_STAGES = 2;
-constexpr int OFF_STAT = OFF_Y0 + KV_Y0_STAGES * TILE_BYTES;  // [2 stages][nlse2 | ndelta][128]
+constexpr int STAT_TILE = TILE * 32;                             // 128 rows of 16 16-bit columns
+constexpr int OFF_STAT = OFF_Y0 + KV_Y0_STAGES * TILE_BYTES;  // [2 stages][lse | delta][STAT_TILE]
+constexpr int OFF_ONES = OFF_STAT + 2 * 2 * STAT_TILE;        // [lse | delta][STAT_TILE]
+static_assert(OFF_ONES + 2 * STAT_TILE <= OFF_Y1, "the statistics fit the place of a tile");
 constexpr int OFF_BAR = OFF_Y1 + Y1_STAGES * TILE_BYTES;
 constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
 static_assert(SMEM_BYTES <= 232448, "fits a block's shared memory");
 constexpr float kP16Shift = 14.0f;  // fp16: P is held as 2^14 P
+constexpr float kLse16 = 128.0f;    // fp16: lse enters the product as 128 x (its 128th)
 
 struct Params {
   int B, H, group, Lq, Lk, Lqp;  // Lqp: Lq rounded up to whole tiles
@@ -72,6 +80,7 @@ struct Params {
   float scale, scale_log2;
   const float* nlse2;   // [B][H][Lqp] -lse log2(e) (fp16: + 14), -inf for rows without a key
   const float* ndelta;  // [B][H][Lqp] -delta
+  const uint8_t* stat;  // [B][H][nqb][lse | delta][STAT_TILE] nlse2 / scale_log2 and ndelta in 16-bit parts
   const unsigned* top;  // fp16: [kv_batch][Hk][2] largest |dO_i|^2 and |V_j|^2, as bits
   void *dq, *dk, *dv;
   long long lddq, lddk, lddv, dq_bs, dk_bs, dv_bs;
@@ -86,23 +95,104 @@ __device__ __forceinline__ int keys_of(const Params& p, int kvb) {
   return p.key_len ? max(0, min(p.Lk, p.key_len[kvb])) : p.Lk;
 }
 
-// The power of two that moves this k/v head's dS into fp16 (its bound to 2^15 at most).
-__device__ __forceinline__ float ds_scale(const Params& p, int kv_head) {
-  const float bound = 2.f * sqrtf(__uint_as_float(p.top[2 * kv_head])) * sqrtf(__uint_as_float(p.top[2 * kv_head + 1]));
-  if (!(bound > 0.f) || bound == INFINITY) return 1.f;
-  const int e = min(max(14 - ilogbf(bound), -100), 100);
-  return ldexpf(1.f, e);
+// fp16: floor(log2) of the bound 2 max|dO_i| max|V_j| of a k/v head's |dS| (and twice its |delta|).
+__device__ __forceinline__ int ds_exponent(const unsigned* top, int kv_head) {
+  const float bound = 2.f * sqrtf(__uint_as_float(top[2 * kv_head])) * sqrtf(__uint_as_float(top[2 * kv_head + 1]));
+  if (!(bound > 0.f) || bound == INFINITY) return 0;
+  return min(max(ilogbf(bound), -100), 100);
 }
+// The power of two that moves dS into fp16 (2^15 at most), and the one that delta / it fits fp16 with.
+__device__ __forceinline__ float ds_scale(int e) { return ldexpf(1.f, 14 - e); }
+__device__ __forceinline__ float delta_unit(int e) { return ldexpf(1.f, min(max(e - 14, -24), 15)); }
+
+// Where column 0 of a statistics row lies: K-major without swizzle, 8 rows x 16 bytes in a row of 128.
+__device__ __forceinline__ int stat_row(int r) { return (r >> 3) * 256 + (r & 7) * 16; }
 
 // Blocks that a mask cuts and whole ones are two copies of the code: the selects cost a whole block a
 // third of its issue slots.
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
+// The products' operands. A shared-memory matrix descriptor is a low word, which holds the address, and a
+// high word that only the layout sets; every step of a product is the low word plus a constant.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) {
+  return static_cast<uint32_t>(sdesc_sw128(saddr, lbo_bytes, 1024));
+}
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024, version 1, 128-byte swizzle
+
+// As umma_f16 and umma_f16_ts, for a whole warp: every lane comes here with the same operands and the
+// elected one (lead) issues. The warp's control flow stays uniform, so operands can live in uniform
+// registers and a product costs few issue slots - the sub-partition shares them with busy math warps.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc,
+                                        uint32_t lead, uint32_t hi = kDescHi) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc,
+                                        uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
+// A warp's bounded wait. One lane polls: the barrier takes the lanes of a poll one by one, and 32 of them
+// cost 130 to 300 cycles even where the phase had long been complete. The warp agrees on the outcome.
+__device__ __forceinline__ uint32_t mbar_test_lead(uint32_t bar, uint32_t parity, uint32_t lead) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 e, %3, 0;\n\tsetp.ne.b32 p, %3, %3;\n\t"
+      "@e mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(lead)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t lead, volatile int* abort_flag,
+                                          unsigned err) {
+  const uint32_t a = smem_u32(bar);
+  if (!__any_sync(0xffffffffu, mbar_test_lead(a, parity, lead))) {
+    const unsigned long long t0 = globaltimer();
+    while (!__any_sync(0xffffffffu, mbar_test_lead(a, parity, lead))) {
+      const bool late = globaltimer() - t0 > kWaitTimeoutNs;
+      if (__any_sync(0xffffffffu, late || *abort_flag)) {
+        if (late) {
+          flag_error(err);
+          *abort_flag = 1;
+        }
+        return false;
+      }
+    }
+  }
+  __syncwarp();  // what the polling lane has seen complete, all have
+  return true;
+}
+
+// The statistics' tiles: rows of 8 in 256 bytes, the second 8 columns 128 bytes on, no swizzle.
+constexpr uint32_t kStatHi = (256u >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t stat_lo(uint32_t saddr) { return (saddr >> 4) | ((128u >> 4) << 16); }
+
 struct Bars {
-  uint64_t *x_full, *y0_full, *y1_full, *y0_empty, *y1_empty, *s_full, *dp_full, *p_full, *ds_full, *acc_done, *drain;
+  uint64_t *x_full, *y0_full, *y1_full, *y0_empty, *y1_empty, *s_full, *s_free, *dp_full, *p_full, *ds_full, *acc_done, *drain;
 };
-constexpr int kBars = 1 + 3 + 2 + 3 + 2 + 2 + 1 + 1 + 1 + 1 + 1;
+constexpr int kBars = 1 + 3 + 2 + 3 + 2 + 1 + 1 + 2 + 1 + 1 + 1 + 1;
 
 // What a block does: a k/v unit or a q unit, and its range of iterations.
 struct Work {
@@ -163,32 +253,62 @@ __device__ __forceinline__ void kv_iteration(const Params& p, const Work& w, int
   h = w.h * p.group + g;
 }
 
-// 16-bit values of a column half h lie at the half's own columns, so neither of a row's two warps
-// overwrites what the other still reads: k-step k (16 of the 128 inner indices, 8 columns) of the A operand.
-__device__ __forceinline__ uint32_t half_cols(int k) { return (k >> 2) * 64 + (k & 3) * 8; }
+// 16-bit values of a column quarter lie at the quarter's own columns, so none of a row's four warps
+// overwrites what another still reads: k-step k (16 of the 128 inner indices, 8 columns) of the A operand.
+__device__ __forceinline__ uint32_t quarter_cols(int k) { return (k >> 1) * 32 + (k & 1) * 8; }
 
-// Row `row` of the unit's tile, columns [c0, c0 + 32): to the gradient, or to a partial sum.
-__device__ __forceinline__ void put32(void* out, int dtype, size_t at, const uint32_t (&r)[32], float f) {
+// N neighbouring columns of a gradient's row.
+template <int N>
+__device__ __forceinline__ void put(void* out, int dtype, size_t at, const float (&v)[N]) {
   if (dtype == ANIMA_F32) {
     float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      d[t] = make_float4(__uint_as_float(r[4 * t]) * f, __uint_as_float(r[4 * t + 1]) * f,
-                         __uint_as_float(r[4 * t + 2]) * f, __uint_as_float(r[4 * t + 3]) * f);
+    for (int t = 0; t < N / 4; ++t) d[t] = make_float4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
   } else {
     uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
     const bool bf = dtype == ANIMA_BF16;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < N / 8; ++t) {
       uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = __uint_as_float(r[8 * t + 2 * e]) * f, b = __uint_as_float(r[8 * t + 2 * e + 1]) * f;
-        w[e] = bf ? pack2<true>(a, b) : pack2<false>(a, b);
-      }
+      for (int e = 0; e < 4; ++e)
+        w[e] = bf ? pack2<true>(v[8 * t + 2 * e], v[8 * t + 2 * e + 1]) : pack2<false>(v[8 * t + 2 * e], v[8 * t + 2 * e + 1]);
       d[t] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
+}
+
+// 2^x of a pair on the FMA and integer pipes: x = n + f, |f| <= 1/2, by adding 1.5 2^23 (whose sum has n
+// in its low bits), 2^f by a polynomial of degree 4 (least largest relative error, 2.6e-6), times 2^n put
+// together from n's bits. x below -127 gives 0, NaN stays NaN.
+__device__ __forceinline__ f2 exp2_fma(f2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  const f2 m = add2(x, dup2(12582912.0f));
+  const f2 f = sub2(x, add2(m, dup2(-12582912.0f)));
+  f2 q = fma2(dup2(0.009570101f), f, dup2(0.05591786f));
+  q = fma2(q, f, dup2(0.24024744f));
+  q = fma2(q, f, dup2(0.6931218f));
+  q = fma2(q, f, dup2(0.9999993f));
+  const f2 e = make_float2(__int_as_float((__float_as_int(m.x) << 23) + 0x3F800000),
+                           __int_as_float((__float_as_int(m.y) << 23) + 0x3F800000));
+  return mul2(q, e);
+}
+// The special-function unit gives 16 powers a cycle and SM, 1024 cycles for a block: every kFmaEvery-th
+// pair goes the other way.
+constexpr int kFmaEvery = 4;
+__device__ __forceinline__ f2 exp2_pair(f2 x, int t) {
+  if ((t / 2) % kFmaEvery == kFmaEvery - 1) return exp2_fma(x);
+  return make_float2(ex2(x.x), ex2(x.y));
+}
+
+// Values that are computed here and not later (the compiler would move them behind the next wait).
+template <int N>
+__device__ __forceinline__ void settle(float (&v)[N]) {
+#pragma unroll
+  for (int t = 0; t < N; t += 8)
+    asm volatile("" : "+f"(v[t]), "+f"(v[t + 1]), "+f"(v[t + 2]), "+f"(v[t + 3]), "+f"(v[t + 4]), "+f"(v[t + 5]),
+                 "+f"(v[t + 6]), "+f"(v[t + 7]));
 }
 
 template <bool BF16, int HD>
@@ -201,22 +321,34 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
-  const Bars bar{bars, bars + 1, bars + 4, bars + 6, bars + 9, bars + 11, bars + 13, bars + 14, bars + 15, bars + 16,
-                 bars + 17};
+  const Bars bar{bars,      bars + 1,  bars + 4,  bars + 6,  bars + 9,  bars + 11,
+                 bars + 12, bars + 13, bars + 15, bars + 16, bars + 17, bars + 18};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same for all lanes, and known to be
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kProducerWarp = MATH_WARPS, kMmaWarp = MATH_WARPS + 1;
+  uint32_t lead;  // one lane of the warp: it polls and issues
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}\n" : "=r"(lead));
   const Work w = work_of(p);
   const int y0_stages = w.kv ? KV_Y0_STAGES : Y0_STAGES;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const bool math = bars + i == bar.p_full || bars + i == bar.ds_full;
+      const bool math = bars + i == bar.s_free || bars + i == bar.p_full || bars + i == bar.ds_full;
       mbar_init(bars + i, math ? MATH_WARPS : 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
+  }
+  if (w.kv && threadIdx.x < 2 * TILE) {  // the constant columns: 1 (or fp16's unit) three times, then zeros
+    const int which = threadIdx.x / TILE;
+    uint8_t* row = smem + OFF_ONES + which * STAT_TILE + stat_row(threadIdx.x % TILE);
+    float one = 1.f;
+    if (!BF16) one = which ? delta_unit(ds_exponent(p.top, w.b * (p.H / p.group) + w.h)) : kLse16;
+    *reinterpret_cast<uint4*>(row) = make_uint4(pack2<BF16>(one, one), pack2<BF16>(one, 0.f), 0u, 0u);
+    *reinterpret_cast<uint4*>(row + 128) = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
   }
   if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, 512);
@@ -226,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t t_s = tmem, t_dp = tmem + 128, t_acc = tmem + 256, t_acc2 = tmem + 256 + HD, t_s1 = tmem + 384;
+  const uint32_t t_s = tmem, t_dp = tmem + 128, t_acc = tmem + 256, t_acc2 = tmem + 256 + HD, t_dp1 = tmem + 384;
 
   if (warp == kProducerWarp) {
     if (lane == 0 && w.n > 0) {
@@ -254,15 +386,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < w.n; ++i) {
         int b = 0, h = 0, qb = 0;
         if (w.kv) kv_iteration(p, w, i, b, h, qb);
-        const size_t stat = (static_cast<size_t>(b) * p.H + h) * p.Lqp + static_cast<size_t>(qb) * TILE;
-        float* st = reinterpret_cast<float*>(smem + OFF_STAT);
+        const size_t stat = ((static_cast<size_t>(b) * p.H + h) * p.nqb + qb) * (2 * STAT_TILE);
         if (!mbar_wait(&bar.y0_empty[s0], ph0 ^ 1, abort_flag, kErrTimeoutEmpty)) break;
         if (w.kv) {
-          // the statistics come and go with Q: its place is freed last, after dK(i) and so after dS(i)
-          mbar_arrive_expect_tx(&bar.y0_full[s0], BYTES + 2 * TILE * 4);
+          // the statistics come and go with Q: its place is freed last
+          mbar_arrive_expect_tx(&bar.y0_full[s0], BYTES + 2 * STAT_TILE);
           load(OFF_Y0 + s0 * TILE_BYTES, &tm_q, &bar.y0_full[s0], p.q_col + h * HD, qb * TILE, b);
-          bulk_load_1d(st + s0 * 2 * TILE, p.nlse2 + stat, TILE * 4, &bar.y0_full[s0]);
-          bulk_load_1d(st + s0 * 2 * TILE + TILE, p.ndelta + stat, TILE * 4, &bar.y0_full[s0]);
+          bulk_load_1d(smem + OFF_STAT + s0 * 2 * STAT_TILE, p.stat + stat, 2 * STAT_TILE, &bar.y0_full[s0]);
         } else {
           mbar_arrive_expect_tx(&bar.y0_full[s0], BYTES);
           load(OFF_Y0 + s0 * TILE_BYTES, &tm_k, &bar.y0_full[s0], kc, (w.lo + i) * TILE, kvb);
@@ -296,36 +426,48 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0 && w.n > 0) {
-      const uint32_t id_s = idesc_f16(TILE, TILE, BF16, false);
-      const uint32_t id_acc = idesc_f16(TILE, HD, BF16, true);
-      const uint32_t sx = smem_u32(smem + OFF_X), sy0 = smem_u32(smem + OFF_Y0), sy1 = smem_u32(smem + OFF_Y1);
+    if (w.n > 0) {
+      constexpr uint32_t id_s = idesc_f16(TILE, TILE, BF16, false);
+      constexpr uint32_t id_acc = idesc_f16(TILE, HD, BF16, true);
+      // low words of the unit's tiles and the rings' first places, read along the head's dims (K-major)
+      // and along the rows (MN-major); a place further is TILE_BYTES on
+      const uint32_t x0 = desc_lo(smem_u32(smem + OFF_X), 16), x1 = x0 + (TILE_BYTES >> 4);
+      const uint32_t y0 = desc_lo(smem_u32(smem + OFF_Y0), 16), y1 = desc_lo(smem_u32(smem + OFF_Y1), 16);
+      constexpr uint32_t kRows = (ATOM >> 4) - 1 << 16;  // from the K-major word to the MN-major one
+      constexpr uint32_t kPlace = TILE_BYTES >> 4;
       // d = A B^T over the head's dims, both tiles K-major in shared memory
       auto dims_product = [&](uint32_t d, uint32_t a, uint32_t b) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (k >> 2) * ATOM + (k & 3) * 32;
-          umma_f16(d, sdesc_sw128(a + off, 16, 1024), sdesc_sw128(b + off, 16, 1024), id_s, k > 0 ? 1u : 0u);
+          const uint32_t off = ((k >> 2) * ATOM + (k & 3) * 32) >> 4;
+          umma_ss(d, a + off, b + off, id_s, k > 0 ? 1u : 0u, lead);
         }
+      };
+      // d += a column's statistic in every lane (which: 0 lse, 1 delta), from Q's place s
+      const uint32_t ones = stat_lo(smem_u32(smem + OFF_ONES)), stats = stat_lo(smem_u32(smem + OFF_STAT));
+      auto add_statistic = [&](uint32_t d, int which, int s) {
+        if (w.kv)
+          umma_ss(d, ones + which * (STAT_TILE >> 4), stats + (2 * s + which) * (STAT_TILE >> 4), id_s, 1u, lead, kStatHi);
       };
       // d (+)= A B, A 128 x 128 16-bit in tensor memory, B's rows the inner index
       auto rows_product = [&](uint32_t d, uint32_t a, uint32_t b, bool first) {
 #pragma unroll
         for (int k = 0; k < TILE / 16; ++k)
-          umma_f16_ts(d, a + half_cols(k), sdesc_sw128(b + k * 16 * 128, ATOM, 1024), id_acc,
-                      (!first || k > 0) ? 1u : 0u);
+          umma_ts(d, a + quarter_cols(k), b + kRows + k * (16 * 128 >> 4), id_acc, (!first || k > 0) ? 1u : 0u, lead);
       };
-      auto full = [&](uint64_t* fb, uint32_t ph) { return mbar_wait(fb, ph, abort_flag, kErrTimeoutFull); };
+      auto full = [&](uint64_t* fb, uint32_t ph) { return warp_wait(fb, ph, lead, abort_flag, kErrTimeoutFull); };
       bool ok = full(bar.x_full, 0) && full(&bar.y0_full[0], 0);
       if (ok) {
         tc_fence_after();
-        dims_product(t_s, sx, sy0);
-        umma_commit(&bar.s_full[0]);
+        dims_product(t_s, x0, y0);
+        add_statistic(t_s, 0, 0);
+        commit(bar.s_full, lead);
         ok = full(&bar.y1_full[0], 0);
       }
       if (ok) {
-        dims_product(t_dp, sx + TILE_BYTES, sy1);
-        umma_commit(bar.dp_full);
+        dims_product(t_dp, x1, y1);
+        add_statistic(t_dp, 1, 0);
+        commit(bar.dp_full, lead);
       }
       if (w.kv) {
         int s = 0;  // stage of block i (both rings have two)
@@ -336,58 +478,56 @@ __global__ void __launch_bounds__(THREADS, 1)
           const bool more = i + 1 < w.n;
           if (!(ok = full(bar.p_full, i & 1))) break;
           tc_fence_after();
-          rows_product(t_acc, t_s, sy1 + s * TILE_BYTES, i == 0);  // dV
-          umma_commit(&bar.y1_empty[s]);
+          rows_product(t_acc, t_s, y1 + s * kPlace, i == 0);  // dV
+          commit(&bar.y1_empty[s], lead);
           if (more) {
             if (!(ok = full(&bar.y0_full[s1], ph1))) break;
-            dims_product(t_s, sx, sy0 + s1 * TILE_BYTES);
-            umma_commit(&bar.s_full[0]);
+            dims_product(t_s, x0, y0 + s1 * kPlace);
+            add_statistic(t_s, 0, s1);
+            commit(bar.s_full, lead);
           }
           if (!(ok = full(bar.ds_full, i & 1))) break;
           tc_fence_after();
-          rows_product(t_acc2, t_dp, sy0 + s * TILE_BYTES, i == 0);  // dK
-          umma_commit(&bar.y0_empty[s]);
+          rows_product(t_acc2, t_dp, y0 + s * kPlace, i == 0);  // dK
+          commit(&bar.y0_empty[s], lead);
           if (more) {
             if (!(ok = full(&bar.y1_full[s1], ph1))) break;
-            dims_product(t_dp, sx + TILE_BYTES, sy1 + s1 * TILE_BYTES);
-            umma_commit(bar.dp_full);
+            dims_product(t_dp, x1, y1 + s1 * kPlace);
+            add_statistic(t_dp, 1, s1);
+            commit(bar.dp_full, lead);
           }
           s = s1;
           ph = ph1;
         }
       } else {
-        int r0 = 0, n0 = 1;  // ring places of K: block i, the next S
-        uint32_t pn0 = 0;    // the phase of the next S's place
-        auto next_s = [&](int j) {
-          if (!full(&bar.y0_full[n0], pn0)) return false;
-          dims_product(j & 1 ? t_s1 : t_s, sx, sy0 + n0 * TILE_BYTES);
-          umma_commit(&bar.s_full[j & 1]);
-          if (++n0 == Y0_STAGES) n0 = 0, pn0 ^= 1;
-          return true;
-        };
-        if (ok) umma_commit(&bar.y1_empty[0]);
-        if (ok && w.n > 1) ok = next_s(1);
+        int r0 = 0, n0 = 1;  // ring places of K: block i, block i + 1
+        uint32_t pn0 = 0;    // the phase of the latter
+        if (ok) commit(&bar.y1_empty[0], lead);
         for (int i = 0; ok && i < w.n; ++i) {
-          if (!(ok = full(bar.ds_full, i & 1))) break;
-          tc_fence_after();
-          rows_product(t_acc, t_dp, sy0 + r0 * TILE_BYTES, i == 0);  // dQ
-          umma_commit(&bar.y0_empty[r0]);
-          if (++r0 == Y0_STAGES) r0 = 0;
           if (i + 1 < w.n) {
             const int s1 = (i + 1) & 1;
+            if (!(ok = full(bar.s_free, i & 1) && full(&bar.y0_full[n0], pn0))) break;
+            tc_fence_after();
+            dims_product(t_s, x0, y0 + n0 * kPlace);
+            commit(bar.s_full, lead);
+            if (++n0 == Y0_STAGES) n0 = 0, pn0 ^= 1;
             if (!(ok = full(&bar.y1_full[s1], ((i + 1) >> 1) & 1))) break;
-            dims_product(t_dp, sx + TILE_BYTES, sy1 + s1 * TILE_BYTES);
-            umma_commit(bar.dp_full);
-            umma_commit(&bar.y1_empty[s1]);
+            dims_product(s1 ? t_dp1 : t_dp, x1, y1 + s1 * kPlace);
+            commit(&bar.dp_full[s1], lead);
+            commit(&bar.y1_empty[s1], lead);
           }
-          if (i + 2 < w.n && !(ok = next_s(i + 2))) break;
+          if (!(ok = full(bar.ds_full, i & 1))) break;
+          tc_fence_after();
+          rows_product(t_acc, i & 1 ? t_dp1 : t_dp, y0 + r0 * kPlace, i == 0);  // dQ
+          commit(&bar.y0_empty[r0], lead);
+          if (++r0 == Y0_STAGES) r0 = 0;
         }
       }
       if (ok) {
-        umma_commit(bar.acc_done);
+        commit(bar.acc_done, lead);
       } else {
         // every product this thread issued completes before the block frees tensor memory
-        umma_commit(bar.drain);
+        commit(bar.drain, lead);
         const unsigned long long t0 = globaltimer();
         while (!mbar_test(smem_u32(bar.drain), 0)) {
           if (globaltimer() - t0 > kWaitTimeoutNs) {
@@ -398,82 +538,72 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else {
-    const int hf = warp >> 2, quad = warp & 3;
+    const int qt = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     const f2 sc2 = dup2(p.scale_log2);
     const int kv_len = keys_of(p, p.kv_batch > 1 ? w.b : 0);
     float cds = 1.f;  // fp16: dS is held as c dS
-    if (!BF16) cds = ds_scale(p, (p.kv_batch > 1 ? w.b : 0) * (p.H / p.group) + (w.kv ? w.h : w.h / p.group));
+    if (!BF16)
+      cds = ds_scale(ds_exponent(p.top, (p.kv_batch > 1 ? w.b : 0) * (p.H / p.group) + (w.kv ? w.h : w.h / p.group)));
     const f2 c2 = dup2(BF16 ? 1.f : cds * exp2f(-kP16Shift));  // P arrives as 2^14 P
     bool ok = true;
-    float pr[64];  // this half row of P
+    float pr[32];  // this quarter row of P
     for (int i = 0; i < w.n; ++i) {
       if (w.kv) {
         int b, h, qb;
         kv_iteration(p, w, i, b, h, qb);
-        const int s = i & 1;
-        const uint32_t ph = (i >> 1) & 1;
-        const float* nlse2 = reinterpret_cast<const float*>(smem + OFF_STAT) + s * 2 * TILE + 64 * hf;
-        const float* ndelta = nlse2 + TILE;
         // lanes are keys: a hidden key's whole row, and on the diagonal block queries before the key
         const bool diag = p.causal && qb == w.blk;
         const bool masked = diag || w.blk * TILE + TILE > kv_len;
         const int first = w.blk * TILE + row >= kv_len ? TILE : (diag ? row : 0);  // first query that sees it
-        if (!(ok = warp_wait(&bar.y0_full[s], ph, abort_flag, kErrTimeoutFull) &&
-                   warp_wait(bar.s_full, i & 1, abort_flag, kErrTimeoutFull)))
-          break;
+        if (!(ok = warp_wait(bar.s_full, i & 1, lead, abort_flag, kErrTimeoutFull))) break;
         tc_fence_after();
-        const uint32_t ts = t_s + lane_addr + 64 * hf, td = t_dp + lane_addr + 64 * hf;
-        auto probabilities = [&](auto mask, const uint32_t(&r)[32], int c) {
+        const uint32_t ts = t_s + lane_addr + 32 * qt, td = t_dp + lane_addr + 32 * qt;
+        auto probabilities = [&](auto mask, const uint32_t(&r)[32]) {
           uint32_t pk[16];
 #pragma unroll
           for (int t = 0; t < 32; t += 4) {
-            const float4 l = *reinterpret_cast<const float4*>(nlse2 + 32 * c + t);
-            const f2 a0 = fma2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, make_float2(l.x, l.y));
-            const f2 a1 =
-                fma2(make_float2(__uint_as_float(r[t + 2]), __uint_as_float(r[t + 3])), sc2, make_float2(l.z, l.w));
-            float e[4] = {ex2(a0.x), ex2(a0.y), ex2(a1.x), ex2(a1.y)};
+            const f2 a0 = mul2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2);
+            const f2 a1 = mul2(make_float2(__uint_as_float(r[t + 2]), __uint_as_float(r[t + 3])), sc2);
+            const f2 e0 = exp2_pair(a0, t), e1 = exp2_pair(a1, t + 2);
+            float e[4] = {e0.x, e0.y, e1.x, e1.y};
             if constexpr (decltype(mask)::value) {
 #pragma unroll
               for (int u = 0; u < 4; ++u)
-                if (64 * hf + 32 * c + t + u < first) e[u] = 0.f;
+                if (32 * qt + t + u < first) e[u] = 0.f;
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) pr[32 * c + t + u] = e[u];
+            for (int u = 0; u < 4; ++u) pr[t + u] = e[u];
             pk[t / 2] = pack2<BF16>(e[0], e[1]);
             pk[t / 2 + 1] = pack2<BF16>(e[2], e[3]);
           }
-          tmem_st16(ts + 16 * c, pk);
+          tmem_st16(ts, pk);
         };
         {
-          uint32_t r0[32], r1[32];
-          tmem_ld32(ts, r0);
-          tmem_ld_wait(r0);
-          tmem_ld32(ts + 32, r1);  // in flight while the first half is computed
-          if (masked) probabilities(Yes{}, r0, 0); else probabilities(No{}, r0, 0);
-          tmem_ld_wait(r1);
-          if (masked) probabilities(Yes{}, r1, 1); else probabilities(No{}, r1, 1);
+          uint32_t r[32];
+          tmem_ld32(ts, r);
+          tmem_ld_wait(r);
+          if (masked) probabilities(Yes{}, r); else probabilities(No{}, r);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         arrive_one_lane(bar.p_full);
-        if (!(ok = warp_wait(bar.dp_full, i & 1, abort_flag, kErrTimeoutFull))) break;
+        if (!(ok = warp_wait(bar.dp_full, i & 1, lead, abort_flag, kErrTimeoutFull))) break;
         tc_fence_after();
-        auto gradients = [&](auto mask, const uint32_t(&r)[32], int c) {
+        auto gradients = [&](auto mask, const uint32_t(&r)[32]) {
           uint32_t pk[16];
 #pragma unroll
           for (int t = 0; t < 32; t += 4) {
-            const float4 d = *reinterpret_cast<const float4*>(ndelta + 32 * c + t);
-            f2 g0 = add2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), make_float2(d.x, d.y));
-            f2 g1 = add2(make_float2(__uint_as_float(r[t + 2]), __uint_as_float(r[t + 3])), make_float2(d.z, d.w));
-            f2 p0 = make_float2(pr[32 * c + t], pr[32 * c + t + 1]), p1 = make_float2(pr[32 * c + t + 2], pr[32 * c + t + 3]);
+            f2 g0 = make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1]));
+            f2 g1 = make_float2(__uint_as_float(r[t + 2]), __uint_as_float(r[t + 3]));
+            f2 p0 = make_float2(pr[t], pr[t + 1]), p1 = make_float2(pr[t + 2], pr[t + 3]);
             if (!BF16) p0 = mul2(p0, c2), p1 = mul2(p1, c2);
             g0 = mul2(g0, p0);
             g1 = mul2(g1, p1);
             if constexpr (decltype(mask)::value) {  // 0 whatever dP is
-              const int q = 64 * hf + 32 * c + t;
+              const int q = 32 * qt + t;
               if (q < first) g0.x = 0.f;
               if (q + 1 < first) g0.y = 0.f;
               if (q + 2 < first) g1.x = 0.f;
@@ -482,16 +612,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             pk[t / 2] = pack2<BF16>(g0.x, g0.y);
             pk[t / 2 + 1] = pack2<BF16>(g1.x, g1.y);
           }
-          tmem_st16(td + 16 * c, pk);
+          tmem_st16(td, pk);
         };
         {
-          uint32_t r0[32], r1[32];
-          tmem_ld32(td, r0);
-          tmem_ld_wait(r0);
-          tmem_ld32(td + 32, r1);
-          if (masked) gradients(Yes{}, r0, 0); else gradients(No{}, r0, 0);
-          tmem_ld_wait(r1);
-          if (masked) gradients(Yes{}, r1, 1); else gradients(No{}, r1, 1);
+          uint32_t r[32];
+          tmem_ld32(td, r);
+          tmem_ld_wait(r);
+          if (masked) gradients(Yes{}, r); else gradients(No{}, r);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -505,57 +632,56 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int left = kv_len - kb * TILE;
         const bool masked = left < TILE || (p.causal && kb == w.blk);
         const int end = p.causal && kb == w.blk ? min(left, row + 1) : left;
-        const uint32_t ts = (i & 1 ? t_s1 : t_s) + lane_addr + 64 * hf, td = t_dp + lane_addr + 64 * hf;
-        if (!(ok = warp_wait(&bar.s_full[i & 1], (i >> 1) & 1, abort_flag, kErrTimeoutFull))) break;
+        const uint32_t ts = t_s + lane_addr + 32 * qt, td = (i & 1 ? t_dp1 : t_dp) + lane_addr + 32 * qt;
+        if (!(ok = warp_wait(bar.s_full, i & 1, lead, abort_flag, kErrTimeoutFull))) break;
         tc_fence_after();
-        auto probabilities = [&](const uint32_t(&r)[32], int c) {
+        auto probabilities = [&](const uint32_t(&r)[32]) {
 #pragma unroll
           for (int t = 0; t < 32; t += 2) {
             const f2 a = fma2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, nlse2);
-            pr[32 * c + t] = ex2(a.x);
-            pr[32 * c + t + 1] = ex2(a.y);
+            const f2 e = exp2_pair(a, t);
+            pr[t] = e.x;
+            pr[t + 1] = e.y;
           }
         };
         {
-          uint32_t r0[32], r1[32];
-          tmem_ld32(ts, r0);
-          tmem_ld_wait(r0);
-          tmem_ld32(ts + 32, r1);
-          probabilities(r0, 0);
-          tmem_ld_wait(r1);
-          probabilities(r1, 1);
+          uint32_t r[32];
+          tmem_ld32(ts, r);
+          tmem_ld_wait(r);
+          tc_fence_before();
+          __syncwarp();
+          arrive_one_lane(bar.s_free);  // S(i + 1) may overwrite it
+          probabilities(r);
+          settle(pr);
         }
-        if (!(ok = warp_wait(bar.dp_full, i & 1, abort_flag, kErrTimeoutFull))) break;
+        if (!(ok = warp_wait(&bar.dp_full[i & 1], (i >> 1) & 1, lead, abort_flag, kErrTimeoutFull))) break;
         tc_fence_after();
-        auto gradients = [&](auto mask, const uint32_t(&r)[32], int c) {
+        auto gradients = [&](auto mask, const uint32_t(&r)[32]) {
           uint32_t pk[16];
 #pragma unroll
           for (int t = 0; t < 32; t += 2) {
             f2 g = add2(make_float2(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), ndelta);
-            f2 pp = make_float2(pr[32 * c + t], pr[32 * c + t + 1]);
+            f2 pp = make_float2(pr[t], pr[t + 1]);
             if (!BF16) pp = mul2(pp, c2);
             g = mul2(g, pp);
             if constexpr (decltype(mask)::value) {  // 0 whatever S and dP are
-              if (64 * hf + 32 * c + t >= end) g.x = 0.f;
-              if (64 * hf + 32 * c + t + 1 >= end) g.y = 0.f;
+              if (32 * qt + t >= end) g.x = 0.f;
+              if (32 * qt + t + 1 >= end) g.y = 0.f;
             }
             pk[t / 2] = pack2<BF16>(g.x, g.y);
           }
-          tmem_st16(td + 16 * c, pk);
+          tmem_st16(td, pk);
         };
         {
-          uint32_t r0[32], r1[32];
-          tmem_ld32(td, r0);
-          tmem_ld_wait(r0);
-          tmem_ld32(td + 32, r1);
-          if (masked) gradients(Yes{}, r0, 0); else gradients(No{}, r0, 0);
-          tmem_ld_wait(r1);
-          if (masked) gradients(Yes{}, r1, 1); else gradients(No{}, r1, 1);
+          uint32_t r[32];
+          tmem_ld32(td, r);
+          tmem_ld_wait(r);
+          if (masked) gradients(Yes{}, r); else gradients(No{}, r);
         }
         if (left < TILE && p.key_len) {
           // K's rows behind key_len may hold anything, and dS K multiplies them by 0
           const int s0 = i % Y0_STAGES;
-          if (!(ok = warp_wait(&bar.y0_full[s0], (i / Y0_STAGES) & 1, abort_flag, kErrTimeoutFull))) break;
+          if (!(ok = warp_wait(&bar.y0_full[s0], (i / Y0_STAGES) & 1, lead, abort_flag, kErrTimeoutFull))) break;
           const int n = (TILE - left) * 8;  // 16-byte pieces of an atom's rows
           for (int t = threadIdx.x; t < n * ATOMS; t += MATH_WARPS * 32)
             *reinterpret_cast<uint4*>(smem + OFF_Y0 + s0 * TILE_BYTES + (t / n) * ATOM + left * 128 + (t % n) * 16) =
@@ -568,7 +694,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         arrive_one_lane(bar.ds_full);
       }
     }
-    if (ok && w.n > 0) ok = warp_wait(bar.acc_done, 0, abort_flag, kErrTimeoutAcc);
+    if (ok && w.n > 0) ok = warp_wait(bar.acc_done, 0, lead, abort_flag, kErrTimeoutAcc);
     if (ok) {
       tc_fence_after();
       const bool split = (w.kv ? p.kv_splits : p.q_splits) > 1;
@@ -576,39 +702,34 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int accs = w.kv ? 2 : 1;  // dV, dK
 #pragma unroll 1
       for (int a = 0; a < accs; ++a) {
-#pragma unroll 1
-        for (int c = 0; c < ATOMS; ++c) {
-          uint32_t v[32];
-          if (w.n > 0) {
-            tmem_ld32((a ? t_acc2 : t_acc) + lane_addr + (HD / 2) * hf + 32 * c, v);
-            tmem_ld_wait(v);
-          } else {
+        constexpr int NC = HD / 4;  // columns of a quarter
+        const int c0 = NC * qt;
+        float v[NC];
+        if (w.n > 0) {
+          uint32_t u[NC];
+          const uint32_t at = (a ? t_acc2 : t_acc) + lane_addr + c0;
+          if constexpr (NC == 32) tmem_ld32(at, u); else tmem_ld16(at, u);
+          tmem_ld_wait(u);
+          float f = BF16 ? 1.f : exp2f(-kP16Shift);
+          if (!w.kv || a) f = BF16 ? p.scale : p.scale / cds;
 #pragma unroll
-            for (int t = 0; t < 32; ++t) v[t] = 0u;
-          }
-          float f;
-          if (w.kv && a == 0)
-            f = BF16 ? 1.f : exp2f(-kP16Shift);
-          else
-            f = BF16 ? p.scale : p.scale / cds;
-          const int c0 = (HD / 2) * hf + 32 * c;
-          if (split) {
-            const size_t slot = w.kv ? (static_cast<size_t>(w.split) * p.kv_units + w.unit) * 2 + a
-                                     : static_cast<size_t>(w.split) * p.q_units + w.unit;
-            float4* d = reinterpret_cast<float4*>(w.kv ? p.kv_part : p.q_part) + (slot * (HD / 4) + c0 / 4) * TILE + row;
+          for (int t = 0; t < NC; ++t) v[t] = __uint_as_float(u[t]) * f;
+        } else {
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
-              d[t * TILE] = make_float4(__uint_as_float(v[4 * t]) * f, __uint_as_float(v[4 * t + 1]) * f,
-                                        __uint_as_float(v[4 * t + 2]) * f, __uint_as_float(v[4 * t + 3]) * f);
-          } else if (w.kv) {
-            if (r < p.Lk) {
-              void* out = a ? p.dk : p.dv;
-              const size_t at = a ? w.b * p.dk_bs + r * p.lddk : w.b * p.dv_bs + r * p.lddv;
-              put32(out, p.grad_dtype, at + static_cast<size_t>(w.h) * HD + c0, v, f);
-            }
-          } else if (r < p.Lq) {
-            put32(p.dq, p.grad_dtype, w.b * p.dq_bs + r * p.lddq + static_cast<size_t>(w.h) * HD + c0, v, f);
-          }
+          for (int t = 0; t < NC; ++t) v[t] = 0.f;
+        }
+        if (split) {
+          const size_t slot = w.kv ? (static_cast<size_t>(w.split) * p.kv_units + w.unit) * 2 + a
+                                   : static_cast<size_t>(w.split) * p.q_units + w.unit;
+          float4* d = reinterpret_cast<float4*>(w.kv ? p.kv_part : p.q_part) + (slot * (HD / 4) + c0 / 4) * TILE + row;
+#pragma unroll
+          for (int t = 0; t < NC / 4; ++t) d[t * TILE] = make_float4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
+        } else if (w.kv) {
+          if (r < p.Lk)
+            put<NC>(a ? p.dk : p.dv, p.grad_dtype,
+                    (a ? w.b * p.dk_bs + r * p.lddk : w.b * p.dv_bs + r * p.lddv) + static_cast<size_t>(w.h) * HD + c0, v);
+        } else if (r < p.Lq) {
+          put<NC>(p.dq, p.grad_dtype, w.b * p.dq_bs + r * p.lddq + static_cast<size_t>(w.h) * HD + c0, v);
         }
       }
     }
@@ -624,8 +745,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 // ------------------------------------------------------------------ before and after it
 
 // delta and the scaled row statistic of every (item, head, query), padded to whole tiles with rows
-// that no key sees; D / 8 threads a row and head, 16 bytes each. In fp16 also the largest |dO_i|^2.
-// Bound by reading out and dout once.
+// that no key sees, in fp32 for the q units and in 16-bit parts for the k/v units; D / 8 threads a row
+// and head, 16 bytes each. Bound by reading out and dout once.
 struct PrepParams {
   const void* out;
   const void* dout;
@@ -633,9 +754,24 @@ struct PrepParams {
   long long ldo, o_bs, lddo, do_bs;
   int out_dtype, B, H, group, Lq, Lqp, kv_batch;
   float shift;  // 14 in fp16
+  float scale_log2;
   float *nlse2, *ndelta;
-  unsigned* top;
+  uint8_t* stat;
+  const unsigned* top;
 };
+
+// v as the sum of three 16-bit values (-inf and NaN: the first alone), packed for the first three columns.
+template <bool BF16>
+__device__ __forceinline__ uint2 three_parts(float v) {
+  float part[3];
+  float rest = v;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    part[i] = BF16 ? __bfloat162float(__float2bfloat16_rn(rest)) : __half2float(__float2half_rn(rest));
+    rest = fabsf(part[i]) < INFINITY ? rest - part[i] : 0.f;
+  }
+  return make_uint2(pack2<BF16>(part[0], part[1]), pack2<BF16>(part[2], 0.f));
+}
 
 __device__ __forceinline__ void load8(const void* p, int dtype, size_t at, float (&v)[8]) {
   if (dtype == ANIMA_F32) {
@@ -666,41 +802,56 @@ __global__ void __launch_bounds__(256) attention_grad_prep_kernel(const PrepPara
   const int b = in ? static_cast<int>(row / p.Lqp) : 0;
   const int i = in ? static_cast<int>(row - static_cast<long long>(b) * p.Lqp) : 0;
   const bool real = in && i < p.Lq;
-  float d = 0.f, n = 0.f;
+  float d = 0.f;
   if (real) {
     float o[8], g[8];
     load8(p.out, p.out_dtype, static_cast<size_t>(b) * p.o_bs + i * p.ldo + static_cast<size_t>(h) * HD + 8 * t, o);
     load8(p.dout, BF16 ? ANIMA_BF16 : ANIMA_F16, static_cast<size_t>(b) * p.do_bs + i * p.lddo + static_cast<size_t>(h) * HD + 8 * t, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      d = fmaf(o[j], g[j], d);
-      n = fmaf(g[j], g[j], n);
-    }
+    for (int j = 0; j < 8; ++j) d = fmaf(o[j], g[j], d);
   }
 #pragma unroll
-  for (int s = TPR / 2; s > 0; s >>= 1) {
-    d += __shfl_xor_sync(0xffffffffu, d, s);
-    if (!BF16) n += __shfl_xor_sync(0xffffffffu, n, s);
-  }
+  for (int s = TPR / 2; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
   if (!in || t) return;
   const size_t at = (static_cast<size_t>(b) * p.H + h) * p.Lqp + i;
   const float l = real ? p.lse[(static_cast<size_t>(b) * p.H + h) * p.Lq + i] : -INFINITY;
-  p.nlse2[at] = l == -INFINITY ? -INFINITY : fmaf(l, -1.4426950408889634f, p.shift);
+  const float nl = l == -INFINITY ? -INFINITY : fmaf(l, -1.4426950408889634f, p.shift);
+  p.nlse2[at] = nl;
   p.ndelta[at] = -d;
-  if (!BF16 && real && n > 0.f)
-    atomicMax(p.top + 2 * ((p.kv_batch > 1 ? b : 0) * (p.H / p.group) + h / p.group), __float_as_uint(n));
+  uint8_t* tile = p.stat + ((static_cast<size_t>(b) * p.H + h) * (p.Lqp / TILE) + i / TILE) * (2 * STAT_TILE) + stat_row(i % TILE);
+  float unit = 1.f;
+  if (!BF16) unit = delta_unit(ds_exponent(p.top, (p.kv_batch > 1 ? b : 0) * (p.H / p.group) + h / p.group));
+  const uint2 lp = three_parts<BF16>(nl / p.scale_log2 * (BF16 ? 1.f : 1.f / kLse16)), dp = three_parts<BF16>(-d / unit);
+  *reinterpret_cast<uint4*>(tile) = make_uint4(lp.x, lp.y, 0u, 0u);
+  *reinterpret_cast<uint4*>(tile + 128) = make_uint4(0u, 0u, 0u, 0u);
+  *reinterpret_cast<uint4*>(tile + STAT_TILE) = make_uint4(dp.x, dp.y, 0u, 0u);
+  *reinterpret_cast<uint4*>(tile + STAT_TILE + 128) = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// fp16: the largest |V_j|^2 of each k/v head over the keys that count; a warp a row and head.
-__global__ void __launch_bounds__(256) attention_grad_vmax_kernel(const __half* v, long long ldv, long long v_bs, int Hk,
-                                                                  int D, int Lk, const int* key_len, unsigned* top) {
-  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
-  const int len = key_len ? min(Lk, key_len[b]) : Lk;
+// fp16: the largest |dO_i|^2 and |V_j|^2 of each k/v head, over all queries and the keys that count; a
+// warp a row and head. Rows [0, v_rows) of a block's share are V's, the others dO's.
+struct TopParams {
+  const __half *v, *dout;
+  long long ldv, v_bs, lddo, do_bs;
+  int H, group, D, Lq, Lk, kv_batch;
+  const int* key_len;
+  unsigned* top;
+};
+__global__ void __launch_bounds__(256) attention_grad_top_kernel(const TopParams p) {
+  const int b = blockIdx.z, lane = threadIdx.x & 31;
+  const int Hk = p.H / p.group;
+  const bool is_v = blockIdx.y < Hk;  // else q head blockIdx.y - Hk
+  const int h = is_v ? blockIdx.y : blockIdx.y - Hk;
+  if (is_v && b >= p.kv_batch) return;
+  const int kvb = p.kv_batch > 1 ? b : 0;
+  const int len = is_v ? (p.key_len ? min(p.Lk, p.key_len[kvb]) : p.Lk) : p.Lq;
+  const __half* base = (is_v ? p.v + b * p.v_bs : p.dout + b * p.do_bs) + static_cast<long long>(h) * p.D;
+  const long long ld = is_v ? p.ldv : p.lddo;
   float best = 0.f;
   for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < len; j += gridDim.x * 8) {
-    const __half2* r = reinterpret_cast<const __half2*>(v + b * v_bs + j * ldv + static_cast<long long>(h) * D);
+    const __half2* r = reinterpret_cast<const __half2*>(base + j * ld);
     float n = 0.f;
-    for (int c = lane; c < D / 2; c += 32) {
+    for (int c = lane; c < p.D / 2; c += 32) {
       const float2 x = __half22float2(r[c]);
       n = fmaf(x.x, x.x, fmaf(x.y, x.y, n));
     }
@@ -708,7 +859,8 @@ __global__ void __launch_bounds__(256) attention_grad_vmax_kernel(const __half* 
     for (int s = 16; s > 0; s >>= 1) n += __shfl_xor_sync(0xffffffffu, n, s);
     best = fmaxf(best, n);
   }
-  if (lane == 0 && best > 0.f) atomicMax(top + 2 * (b * Hk + h) + 1, __float_as_uint(best));
+  // (bits of values that are not negative are ordered as the values; a maximum hangs on no order)
+  if (lane == 0 && best > 0.f) atomicMax(p.top + 2 * (kvb * Hk + (is_v ? h : h / p.group)) + (is_v ? 1 : 0), __float_as_uint(best));
 }
 
 // The gradients of split units: the splits' partial sums added in order. A thread has four columns of
@@ -763,7 +915,7 @@ __global__ void __launch_bounds__(128) attention_grad_join_kernel(const Params p
 
 struct Plan {
   int group, kv_batch, Lqp, nkb, nqb, kv_units, q_units, kv_splits, q_splits;
-  size_t lse_off, delta_off, top_off, top_bytes, kv_off, q_off, bytes;
+  size_t lse_off, delta_off, stat_off, top_off, top_bytes, kv_off, q_off, bytes;
 };
 
 // Units are split along their walk only where there are too few of them to fill the SMs: each split
@@ -803,6 +955,7 @@ int plan_of(const anima_ctx* ctx, const anima_attention_args* a, Plan& pl) {
   const size_t stat = static_cast<size_t>(a->batch) * a->heads * pl.Lqp * 4;
   pl.lse_off = take(stat);
   pl.delta_off = take(stat);
+  pl.stat_off = take(static_cast<size_t>(a->batch) * a->heads * pl.nqb * 2 * STAT_TILE);
   pl.top_bytes = a->dtype == ANIMA_F16 ? static_cast<size_t>(pl.kv_batch) * (a->heads / pl.group) * 8 : 0;
   pl.top_off = take(pl.top_bytes);
   const size_t tile = static_cast<size_t>(TILE) * a->head_dim * 4;
@@ -832,13 +985,27 @@ int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, c
   ANIMA_REQUIRE((threads + 255) / 256 < (1LL << 31), "anima_attention_backward: problem too large");
   ProfScope prof(ctx, "attn.grad", 10.0 * a->batch * a->heads * static_cast<double>(a->Lq) * a->Lk * HD, 0);
   if (!BF16) {
-    ANIMA_CUDA(cudaMemsetAsync(pp.top, 0, pl.top_bytes, ctx->stream));
+    ANIMA_CUDA(cudaMemsetAsync(const_cast<unsigned*>(pp.top), 0, pl.top_bytes, ctx->stream));
     const int Hk = a->heads / pl.group;
-    ANIMA_REQUIRE(Hk <= 65535 && pl.kv_batch <= 65535, "anima_attention_backward: too many heads or items");
-    const int rows = (a->Lk + 31) / 32;
-    attention_grad_vmax_kernel<<<dim3(rows < 64 ? rows : 64, Hk, pl.kv_batch), 256, 0, ctx->stream>>>(
-        static_cast<const __half*>(a->v) + a->v_off, a->ldv, a->v_bstride, Hk, HD, a->Lk, a->key_len, pp.top);
-    const int st = check_launch("attention_grad_vmax_kernel");
+    ANIMA_REQUIRE(Hk + a->heads <= 65535 && a->batch <= 65535, "anima_attention_backward: too many heads or items");
+    TopParams tp{};
+    tp.v = static_cast<const __half*>(a->v) + a->v_off;
+    tp.dout = static_cast<const __half*>(g->dout);
+    tp.ldv = a->ldv;
+    tp.v_bs = pl.kv_batch > 1 ? a->v_bstride : 0;
+    tp.lddo = g->lddo;
+    tp.do_bs = pp.do_bs;
+    tp.H = a->heads;
+    tp.group = pl.group;
+    tp.D = HD;
+    tp.Lq = a->Lq;
+    tp.Lk = a->Lk;
+    tp.kv_batch = pl.kv_batch;
+    tp.key_len = a->key_len;
+    tp.top = const_cast<unsigned*>(pp.top);
+    const int rows = ((a->Lq > a->Lk ? a->Lq : a->Lk) + 31) / 32;
+    attention_grad_top_kernel<<<dim3(rows < 64 ? rows : 64, Hk + a->heads, a->batch), 256, 0, ctx->stream>>>(tp);
+    const int st = check_launch("attention_grad_top_kernel");
     if (st) return st;
   }
   attention_grad_prep_kernel<BF16, HD><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, ctx->stream>>>(pp);
@@ -952,6 +1119,7 @@ extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_gr
   p.scale_log2 = scale * 1.4426950408889634f;
   p.nlse2 = reinterpret_cast<float*>(ws + pl.lse_off);
   p.ndelta = reinterpret_cast<float*>(ws + pl.delta_off);
+  p.stat = ws + pl.stat_off;
   p.top = reinterpret_cast<unsigned*>(ws + pl.top_off);
   p.dq = g->dq;
   p.dk = g->dk;
@@ -989,6 +1157,8 @@ extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_gr
   pp.shift = a->dtype == ANIMA_F16 ? kP16Shift : 0.f;
   pp.nlse2 = reinterpret_cast<float*>(ws + pl.lse_off);
   pp.ndelta = reinterpret_cast<float*>(ws + pl.delta_off);
+  pp.stat = ws + pl.stat_off;
+  pp.scale_log2 = p.scale_log2;
   pp.top = reinterpret_cast<unsigned*>(ws + pl.top_off);
   if (a->dtype == ANIMA_BF16)
     return a->head_dim == 128 ? launch<true, 128>(ctx, g, pl, p, pp, tm) : launch<true, 64>(ctx, g, pl, p, pp, tm);
