@@ -168,9 +168,14 @@ __device__ __forceinline__ uint32_t mbar_test_lead(uint32_t bar, uint32_t parity
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t lead, volatile int* abort_flag,
                                           unsigned err) {
   const uint32_t a = smem_u32(bar);
-  if (!__any_sync(0xffffffffu, mbar_test_lead(a, parity, lead))) {
+  bool done = __any_sync(0xffffffffu, mbar_test_lead(a, parity, lead));
+  if (!done) {
     const unsigned long long t0 = globaltimer();
-    while (!__any_sync(0xffffffffu, mbar_test_lead(a, parity, lead))) {
+    for (;;) {
+      // the clock and the flag are looked at once in 64 polls: they would double the time of each
+#pragma unroll 1
+      for (int i = 0; i < 64 && !done; ++i) done = __any_sync(0xffffffffu, mbar_test_lead(a, parity, lead));
+      if (done) break;
       const bool late = globaltimer() - t0 > kWaitTimeoutNs;
       if (__any_sync(0xffffffffu, late || *abort_flag)) {
         if (late) {
