@@ -13,7 +13,10 @@
 //
 // Both passes are bound by HBM. A row is held in registers by T = C / V threads (V = 8 columns a
 // thread, or 1 where the columns or alignments are odd); the row's sums are warp shuffles and one
-// exchange through shared memory a round. The backward's column sums stay in registers over the rows
+// exchange through shared memory a round. Where the threads hold 8 columns each and none is idle (C = 256,
+// 512, 1024, 2048), mean, squares about the mean and products with the gradient come from one round: the
+// threads' own moments about their own means are merged pairwise, which loses no digits to a large mean.
+// The backward's column sums stay in registers over the rows
 // of a block, each block writes one partial row of sums and a second kernel adds the partials in a
 // fixed order: no atomics, the same inputs give the same bits.
 
@@ -46,6 +49,7 @@ struct Params {
   // backward: the partial sums [item][part][k][C] and which sum is where (-1: not asked for)
   float* part;
   int parts, part_rows, sums;
+  int places;  // of the ring
   int s_gate, s_postw, s_prew, s_scale, s_shift;
 };
 
@@ -234,6 +238,90 @@ __device__ __forceinline__ void load_row(float (&t)[NV][V], const Cols<V, NV>& c
   }
 }
 
+// Moments of a row for one norm: mean, sum of squares about it (rms: about 0), and of a gradient g the
+// sums of g and of g (t - mean).
+struct Moments {
+  float mean, m2, g, gt;
+};
+
+// A thread's 8 NV values.
+template <int NV>
+__device__ __forceinline__ Moments moments_of(const float (&t)[NV][8], const float (*g)[8], int kind) {
+  Moments m{0.f, 0.f, 0.f, 0.f};
+  if (kind == kLayer) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) m.mean += ((t[k][0] + t[k][1]) + (t[k][2] + t[k][3])) + ((t[k][4] + t[k][5]) + (t[k][6] + t[k][7]));
+    m.mean *= 1.0f / (8 * NV);
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float d = t[k][i] - m.mean;
+      m.m2 = fmaf(d, d, m.m2);
+      if (g) {
+        m.g += g[k][i];
+        m.gt = fmaf(g[k][i], d, m.gt);
+      }
+    }
+  return m;
+}
+
+// Two sets of n values each, their means d apart: both terms of the difference change sign with the order,
+// so the two lanes that merge get the same bits.
+template <bool GRAD>
+__device__ __forceinline__ void merge_lanes(Moments& m, int lanes, float n) {
+  const float mean = __shfl_xor_sync(0xffffffffu, m.mean, lanes), m2 = __shfl_xor_sync(0xffffffffu, m.m2, lanes);
+  const float h = 0.5f * (mean - m.mean);
+  if (GRAD) {
+    const float g = __shfl_xor_sync(0xffffffffu, m.g, lanes), gt = __shfl_xor_sync(0xffffffffu, m.gt, lanes);
+    m.gt = fmaf(g - m.g, h, m.gt + gt);  // t - common mean is t - own mean, less h or plus h
+    m.g += g;
+  }
+  m.m2 = fmaf(2.f * n * h, h, m.m2 + m2);
+  m.mean = 0.5f * (m.mean + mean);
+}
+
+constexpr int kRedMoments = 2 * 2 * (kThreads / 32);  // [2 buffers][warps][2 sets]
+
+// The moments of K sets, n values a thread, over the row's threads, to all of them (GRAD0: the first set
+// has a gradient). One barrier, as in row_sum.
+template <int K, bool GRAD0>
+__device__ __forceinline__ void row_moments(Moments (&m)[K], float n, float4* red, int& buf) {
+  auto step = [&](int lanes) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (k == 0 && GRAD0)
+        merge_lanes<true>(m[k], lanes, n);
+      else
+        merge_lanes<false>(m[k], lanes, n);
+    }
+    n *= 2.f;
+  };
+#pragma unroll
+  for (int lanes = 1; lanes < 32; lanes *= 2) step(lanes);
+  const int W = blockDim.x >> 5;
+  if (W == 1) return;
+  float4* slot = red + buf * (W * K);
+  buf ^= 1;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) slot[(threadIdx.x >> 5) * K + k] = make_float4(m[k].mean, m[k].m2, m[k].g, m[k].gt);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {  // lane i goes on with warp i % W's
+    const float4 v = slot[(threadIdx.x & (W - 1)) * K + k];
+    m[k] = Moments{v.x, v.y, v.z, v.w};
+  }
+  for (int lanes = 1; lanes < W; lanes *= 2) step(lanes);
+}
+
+__device__ __forceinline__ float rstd_of(const Moments& m, float inv_c, float eps) {
+  const float v = fmaf(m.m2, inv_c, eps), r = rsqrtf(v);
+  return v > 0.f && v < INFINITY ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;  // a Newton step: rsqrtf is off by up to 2 steps
+}
+
 template <int V, int NV>
 __global__ void __launch_bounds__(kThreads) residual_norm_kernel(const Params p) {
   __shared__ float red[kRedFloats];
@@ -372,6 +460,325 @@ __global__ void __launch_bounds__(kThreads, NV * V <= 8 ? 2 : 1) residual_norm_g
   }
 }
 
+// A ring of rows in shared memory ahead of the row that a block works on: bulk copies of whole rows, one
+// barrier a place. HBM answers in 1.5 to 2 us under load, so 90 KB have to be on their way to each SM;
+// registers held one row ahead (49 KB) and the backward ran at 72% of the copy rate.
+constexpr int kMaxPlaces = 3;
+struct Stream {
+  const void* p;
+  long long ld;  // bytes
+  uint32_t bytes;  // of a row
+};
+template <int N>
+struct Ring {
+  Stream in[N];
+  uint8_t* smem;
+  uint64_t* full;  // [places]
+  volatile int* abort_flag;
+  uint32_t row_bytes;
+
+  // One thread: row r to its place (what was there has been read).
+  __device__ __forceinline__ void fetch(int k, size_t r) const {
+    mbar_arrive_expect_tx(&full[k], row_bytes);
+    uint8_t* d = smem + k * row_bytes;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!in[i].bytes) continue;
+      bulk_load_1d(d, static_cast<const uint8_t*>(in[i].p) + r * in[i].ld, in[i].bytes, &full[k]);
+      d += in[i].bytes;
+    }
+  }
+  // After a wait that ran out nothing is computed any more, but every thread still meets every barrier.
+  __device__ __forceinline__ bool wait(int k, uint32_t phase) const {
+    return mbar_wait(&full[k], phase, abort_flag, kErrTimeoutFull);
+  }
+};
+
+template <int N>
+__device__ __forceinline__ Ring<N> make_ring(const Stream (&in)[N], uint8_t* smem, uint64_t* full, int* abort_flag,
+                                             int places) {
+  Ring<N> r;
+  r.row_bytes = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r.in[i] = in[i];
+    r.row_bytes += in[i].bytes;
+  }
+  r.smem = smem;
+  r.full = full;
+  r.abort_flag = abort_flag;
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < places; ++k) mbar_init(&full[k], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  return r;
+}
+
+__device__ __forceinline__ uint32_t size_of(int dt) { return dt == ANIMA_F32 ? 4 : 2; }
+
+// 8 elements of a row in the ring.
+__device__ __forceinline__ void load8(const uint8_t* row, int dt, int c, float (&v)[8]) {
+  Raw<8> r;
+  load_raw<8>(r, row, dt, c);
+  unpack<8>(r, dt, v);
+}
+
+// A block's rows: part_rows of one item.
+struct Share {
+  int first, last;
+  size_t item, row0;
+};
+__device__ __forceinline__ Share share_of(const Params& p) {
+  Share s;
+  const int item = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  s.item = item;
+  s.row0 = static_cast<size_t>(item) * p.L;
+  s.first = part * p.part_rows;
+  s.last = min(p.L, s.first + p.part_rows);
+  return s;
+}
+
+// The parameters of a thread's columns, in registers for all of a block's rows (read for each row they
+// came from L2, the ring leaves no L1, and those waits were half of the backward's time). MODS: there is a
+// modulation (gate, scale or shift), WEIGHTS: a norm weight; what is not there costs no registers.
+template <int NV, bool MODS, bool WEIGHTS>
+struct Columns {
+  float scale[NV][8], gate[NV][8], pre[NV][8], post[NV][8];  // 1 + scale, alpha gate
+  float alpha;
+  __device__ __forceinline__ Columns(const Params& p, size_t item, int c0, int step) : alpha(p.alpha) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * step;
+      if (MODS) {
+        param<8>(p.scale, item * p.ldscale + c, 0.f, scale[k]);
+        param<8>(p.gate, item * p.ldgate + c, 1.f, gate[k]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          scale[k][i] += 1.f;
+          gate[k][i] *= alpha;
+        }
+      }
+      if (WEIGHTS) {
+        param<8>(p.pre_w, c, 1.f, pre[k]);
+        param<8>(p.post_w, c, 1.f, post[k]);
+      }
+    }
+  }
+  // v (1 + scale), v pre_w, v alpha gate, v post_w
+  __device__ __forceinline__ float by_scale(float v, int k, int i) const { return MODS ? v * scale[k][i] : v; }
+  __device__ __forceinline__ float by_pre(float v, int k, int i) const { return WEIGHTS ? v * pre[k][i] : v; }
+  __device__ __forceinline__ float by_gate(float v, int k, int i) const { return MODS ? v * gate[k][i] : v * alpha; }
+  __device__ __forceinline__ float by_post(float v, int k, int i) const { return WEIGHTS ? v * post[k][i] : v; }
+};
+
+// The forward where every thread holds 8 NV columns (256, 512, 1024, 2048 and 4096 of them in all): one
+// round of moments a norm.
+template <int NV, bool MODS, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads, NV == 1 ? 3 : 2) residual_norm_full_kernel(const Params p) {
+  extern __shared__ __align__(16) uint8_t ring_smem[];
+  __shared__ float4 red[kRedMoments];
+  __shared__ uint64_t full[kMaxPlaces];
+  __shared__ int abort_flag;
+  int buf = 0;
+  const int step = blockDim.x * 8, c0 = threadIdx.x * 8;
+  const Share w = share_of(p);
+  const float inv_c = 1.0f / static_cast<float>(p.C);
+  const Stream in[2] = {{p.x, p.ldx * size_of(p.dtx), p.C * size_of(p.dtx)},
+                        {p.y, p.ldy * size_of(p.dty), p.C * size_of(p.dty)}};
+  const int places = p.places;
+  const auto ring = make_ring<2>(in, ring_smem, full, &abort_flag, places);
+  if (threadIdx.x == 0)
+    for (int k = 0; k < places; ++k)
+      if (w.first + k < w.last) ring.fetch(k, w.row0 + w.first + k);
+  const Columns<NV, MODS, WEIGHTS> cols(p, w.item, c0, step);
+  float shift[NV][8];
+  if (MODS) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) param<8>(p.shift, w.item * p.ldshift + c0 + k * step, 0.f, shift[k]);
+  }
+  int place = 0, before = -1;
+  uint32_t phase = 0;
+  for (int l = w.first; l < w.last; ++l) {
+    const bool live = ring.wait(place, phase);
+    const uint8_t* at = ring.smem + place * ring.row_bytes;
+    const size_t r = w.row0 + l;
+    float x[NV][8], y[NV][8];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      load8(at, p.dtx, c0 + k * step, x[k]);
+      load8(at + in[0].bytes, p.dty, c0 + k * step, y[k]);
+    }
+    if (p.post != kNone) {
+      Moments m[1] = {moments_of<NV>(y, nullptr, p.post)};
+      row_moments<1, false>(m, 8 * NV, red, buf);
+      const float rs = rstd_of(m[0], inv_c, p.eps);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[k][i] = (y[k][i] - m[0].mean) * rs;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[k][i] += cols.by_gate(cols.by_post(y[k][i], k, i), k, i);
+      if (live) store<8>(p.o0, p.dtx, r * p.ldo0 + c0 + k * step, x[k]);
+    }
+    Moments m[1] = {moments_of<NV>(x, nullptr, p.pre)};
+    row_moments<1, false>(m, 8 * NV, red, buf);
+    __syncwarp();
+    // a barrier (one warp: an exchange) behind the last reads of the place before: its next row
+    if (threadIdx.x == 0 && before >= 0 && l - 1 + places < w.last && !abort_flag) ring.fetch(before, r - 1 + places);
+    before = place;
+    if (++place == places) place = 0, phase ^= 1;
+    const float rs = rstd_of(m[0], inv_c, p.eps);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float n = cols.by_pre((x[k][i] - m[0].mean) * rs, k, i);
+        x[k][i] = MODS ? fmaf(n, cols.scale[k][i], shift[k][i]) : n;
+      }
+      if (live) store<8>(p.o1, p.dth, r * p.ldo1 + c0 + k * step, x[k]);
+    }
+  }
+}
+
+// The backward there. A row's statistics and the sums of the pre-norm's gradient come from one round.
+template <int NV, bool MODS, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads, 2) residual_norm_grad_full_kernel(const Params p) {
+  extern __shared__ __align__(16) uint8_t ring_smem[];
+  __shared__ float4 red[kRedMoments];
+  __shared__ uint64_t full[kMaxPlaces];
+  __shared__ int abort_flag;
+  int buf = 0;
+  const int step = blockDim.x * 8, c0 = threadIdx.x * 8;
+  const Share w = share_of(p);
+  const float inv_c = 1.0f / static_cast<float>(p.C);
+  const Stream in[4] = {{p.x, p.ldx * size_of(p.dtx), p.C * size_of(p.dtx)},
+                        {p.dh, p.lddh * size_of(p.dth), p.C * size_of(p.dth)},
+                        {p.y, p.ldy * size_of(p.dty), p.C * size_of(p.dty)},
+                        {p.dx, p.lddx * size_of(p.dtx), p.dx ? p.C * size_of(p.dtx) : 0u}};
+  const int places = p.places;
+  const auto ring = make_ring<4>(in, ring_smem, full, &abort_flag, places);
+  const uint32_t off_h = in[0].bytes, off_y = off_h + in[1].bytes, off_d = off_y + in[2].bytes;
+  if (threadIdx.x == 0)
+    for (int k = 0; k < places; ++k)
+      if (w.first + k < w.last) ring.fetch(k, w.row0 + w.first + k);
+  const Columns<NV, MODS, WEIGHTS> cols(p, w.item, c0, step);
+  float s_shift[NV][8], s_scale[NV][8], s_gate[NV][8], s_prew[NV][8], s_postw[NV][8];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_shift[k][i] = s_scale[k][i] = s_gate[k][i] = s_prew[k][i] = s_postw[k][i] = 0.f;
+  int place = 0, before = -1;
+  uint32_t phase = 0;
+  for (int l = w.first; l < w.last; ++l) {
+    const bool live = ring.wait(place, phase);
+    const uint8_t* at = ring.smem + place * ring.row_bytes;
+    const size_t r = w.row0 + l;
+    float x[NV][8], h[NV][8], y[NV][8];
+    Moments m[2];
+    {
+      float g[NV][8];  // the gradient of n
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        load8(at, p.dtx, c0 + k * step, x[k]);
+        load8(at + off_h, p.dth, c0 + k * step, h[k]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[k][i] = cols.by_pre(cols.by_scale(h[k][i], k, i), k, i);
+      }
+      m[0] = moments_of<NV>(x, g, p.pre);
+    }
+    float rs_y = 1.f;
+    m[1].mean = 0.f;
+    if (p.post != kNone) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) load8(at + off_y, p.dty, c0 + k * step, y[k]);
+      m[1] = moments_of<NV>(y, nullptr, p.post);
+      row_moments<2, true>(m, 8 * NV, red, buf);
+      rs_y = rstd_of(m[1], inv_c, p.eps);
+    } else {
+      Moments m1[1] = {m[0]};
+      row_moments<1, true>(m1, 8 * NV, red, buf);
+      m[0] = m1[0];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) load8(at + off_y, p.dty, c0 + k * step, y[k]);
+    }
+    __syncwarp();
+    // a barrier (one warp: an exchange) behind the last reads of the place before: its next row
+    if (threadIdx.x == 0 && before >= 0 && l - 1 + places < w.last && !abort_flag) ring.fetch(before, r - 1 + places);
+    before = place;
+    if (++place == places) place = 0, phase ^= 1;
+    const float rs = rstd_of(m[0], inv_c, p.eps);
+    const float mg = p.pre == kLayer ? m[0].g * inv_c * rs : 0.f, mgn = m[0].gt * rs * rs * inv_c;
+    float s2[2] = {0.f, 0.f};
+    float d[NV][8];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (p.dx) {
+        load8(at + off_d, p.dtx, c0 + k * step, d[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[k][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float n = (x[k][i] - m[0].mean) * rs, hp = cols.by_pre(h[k][i], k, i), hs = cols.by_scale(h[k][i], k, i);
+        if (MODS) {
+          s_shift[k][i] += h[k][i];
+          s_scale[k][i] = fmaf(hp, n, s_scale[k][i]);
+        }
+        if (WEIGHTS) s_prew[k][i] = fmaf(hs, n, s_prew[k][i]);
+        // dx' + rs (g - mean(g) - n mean(g n))
+        d[k][i] += fmaf(rs, cols.by_pre(hs, k, i), -fmaf(n, mgn, mg));
+      }
+      if (live) store<8>(p.o0, p.dtx, r * p.ldo0 + c0 + k * step, d[k]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = (y[k][i] - m[1].mean) * rs_y;
+        if (MODS) s_gate[k][i] = fmaf(cols.alpha * cols.by_post(d[k][i], k, i), u, s_gate[k][i]);
+        const float t = cols.by_gate(d[k][i], k, i);
+        if (WEIGHTS) s_postw[k][i] = fmaf(t, u, s_postw[k][i]);
+        d[k][i] = cols.by_post(t, k, i);
+        if (p.post != kNone) {
+          y[k][i] = u;
+          s2[0] += d[k][i];
+          s2[1] = fmaf(d[k][i], u, s2[1]);
+        }
+      }
+      if (p.post == kNone && live) store<8>(p.o1, p.dty, r * p.ldo1 + c0 + k * step, d[k]);
+    }
+    if (p.post != kNone) {
+      row_sum(s2, reinterpret_cast<float*>(red), buf);
+      const float m0 = p.post == kLayer ? s2[0] * inv_c : 0.f, m1 = s2[1] * inv_c;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[k][i] = rs_y * (d[k][i] - m0 - y[k][i] * m1);
+        if (live) store<8>(p.o1, p.dty, r * p.ldo1 + c0 + k * step, d[k]);
+      }
+    }
+  }
+  if (!p.sums) return;
+  float* out = p.part + static_cast<size_t>(blockIdx.x) * p.sums * p.C + c0;
+  auto put = [&](int where, const float(&v)[NV][8]) {
+    if (where < 0) return;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) store<8>(out, ANIMA_F32, static_cast<size_t>(where) * p.C + k * step, v[k]);
+  };
+  if (MODS) {
+    put(p.s_shift, s_shift);
+    put(p.s_scale, s_scale);
+    put(p.s_gate, s_gate);
+  }
+  if (WEIGHTS) {
+    put(p.s_prew, s_prew);
+    put(p.s_postw, s_postw);
+  }
+}
+
 struct SumParams {
   const float* part;  // [items][parts][sums][C]
   int items, parts, sums, C;
@@ -402,6 +809,7 @@ __global__ void __launch_bounds__(256) partial_sum_kernel(const SumParams p) {
 
 struct Shape {
   int V, NV, T, Y;  // columns a vector, vectors a thread, threads a row, rows a block
+  bool full;        // every thread holds 8 NV columns, and the warps merge in pairs: the kernels with a ring
 };
 
 Shape shape_of(int C, bool vec) {
@@ -412,18 +820,26 @@ Shape shape_of(int C, bool vec) {
   while (static_cast<long long>(s.NV) * kThreads < n) s.NV *= 2;
   if (s.V == 1) s.NV = s.NV <= 8 ? 8 : 16;
   s.T = ((n + s.NV - 1) / s.NV + 31) / 32 * 32;
-  s.Y = kThreads / s.T;
+  s.full = s.V == 8 && (C == 256 || C == 512 || C == 1024 || C == 2048 || C == 4096);
+  s.Y = s.full ? 1 : kThreads / s.T;
   return s;
 }
 
-// Rows of one item that a block of the backward pass takes: about two blocks an SM over all items.
-void parts_of(const Shape& s, int items, int L, int sms, int& parts, int& part_rows) {
-  const int want = (2 * sms + items - 1) / items;
+// Rows of one item that a block takes, with as many blocks as the SMs hold at once (`threads` of them an
+// SM), or one row each where there are not as many rows.
+void parts_of(const Shape& s, int items, int L, int sms, int threads, int& parts, int& part_rows) {
+  const int blocks = threads / (s.T * s.Y) < 16 ? threads / (s.T * s.Y) : 16;
+  const int want = blocks * sms / items > 1 ? blocks * sms / items : 1;  // (one wave: a block more would double it)
   const int most = (L + s.Y - 1) / s.Y;
   parts = want < most ? want : most;
   part_rows = ((L + parts - 1) / parts + s.Y - 1) / s.Y * s.Y;
   parts = (L + part_rows - 1) / part_rows;
 }
+constexpr int kGradThreads = 512, kForwardThreads = 768;  // an SM, by the kernels' launch bounds
+
+// Places of a ring: three, or two where three would leave an SM with fewer blocks.
+int places_of(const Shape& s, int threads, int row_bytes) { return kMaxPlaces * row_bytes * (threads / s.T) <= 208 * 1024 ? kMaxPlaces : 2; }
+int size_of_host(int dt) { return dt == ANIMA_F32 ? 4 : 2; }
 
 int count_sums(const anima_residual_norm_args* a) {
   return (a->dshift != nullptr) + (a->dscale != nullptr) + (a->dpre_w != nullptr) + (a->dgate != nullptr) +
@@ -519,10 +935,28 @@ extern "C" int anima_residual_norm(anima_ctx* ctx, const anima_residual_norm_arg
   p.ldo0 = a->ldx_out;
   p.o1 = a->h;
   p.ldo1 = a->ldh;
-  const Kernel fn = s.V == 8 ? (s.NV == 1 ? residual_norm_kernel<8, 1> : residual_norm_kernel<8, 2>)
-                             : (s.NV == 8 ? residual_norm_kernel<1, 8> : residual_norm_kernel<1, 16>);
+  Kernel fn = s.V == 8 ? (s.NV == 1 ? residual_norm_kernel<8, 1> : residual_norm_kernel<8, 2>)
+                       : (s.NV == 8 ? residual_norm_kernel<1, 8> : residual_norm_kernel<1, 16>);
+  long long grid = (static_cast<long long>(a->rows) + s.Y - 1) / s.Y;
+  int smem = 0;
+  if (s.full) {
+    const Kernel fns[2][2][2] = {{{residual_norm_full_kernel<1, false, false>, residual_norm_full_kernel<1, false, true>},
+                                  {residual_norm_full_kernel<1, true, false>, residual_norm_full_kernel<1, true, true>}},
+                                 {{residual_norm_full_kernel<2, false, false>, residual_norm_full_kernel<2, false, true>},
+                                  {residual_norm_full_kernel<2, true, false>, residual_norm_full_kernel<2, true, true>}}};
+    fn = fns[s.NV - 1][a->gate || a->scale || a->shift][a->pre_w || a->post_w];
+    const int items = a->rows / a->rows_per_item;
+    parts_of(s, items, a->rows_per_item, ctx->num_sms, kForwardThreads, p.parts, p.part_rows);
+    grid = static_cast<long long>(items) * p.parts;
+    ANIMA_REQUIRE(grid < (1LL << 31), "anima_residual_norm: %d items are too many", items);
+    const int row = a->cols * (size_of_host(a->x_dtype) + size_of_host(a->y_dtype));
+    p.places = places_of(s, kForwardThreads, row);
+    smem = p.places * row;
+    st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), kMaxPlaces * kMaxCols * 8);
+    if (st) return st;
+  }
   ProfScope prof(ctx, "residual_norm", 0, static_cast<double>(a->rows) * a->cols * 12);
-  fn<<<(a->rows + s.Y - 1) / s.Y, dim3(s.T, s.Y), 0, ctx->stream>>>(p);
+  fn<<<static_cast<unsigned>(grid), dim3(s.T, s.Y), smem, ctx->stream>>>(p);
   return check_launch("residual_norm_kernel");
 }
 
@@ -536,7 +970,7 @@ extern "C" int anima_residual_norm_backward_workspace(anima_ctx* ctx, const anim
   for (const bool vec : {false, true}) {
     const Shape s = shape_of(a->cols, vec);
     int parts, part_rows;
-    parts_of(s, a->rows / a->rows_per_item, a->rows_per_item, ctx->num_sms, parts, part_rows);
+    parts_of(s, a->rows / a->rows_per_item, a->rows_per_item, ctx->num_sms, kGradThreads, parts, part_rows);
     const size_t n = static_cast<size_t>(a->rows / a->rows_per_item) * parts * s.Y * count_sums(a) * a->cols * 4;
     if (n > *bytes) *bytes = n;
   }
@@ -563,7 +997,7 @@ extern "C" int anima_residual_norm_backward(anima_ctx* ctx, const anima_residual
   p.ldo0 = a->lddx;
   p.o1 = a->dy;
   p.ldo1 = a->lddy;
-  parts_of(s, items, a->rows_per_item, ctx->num_sms, p.parts, p.part_rows);
+  parts_of(s, items, a->rows_per_item, ctx->num_sms, kGradThreads, p.parts, p.part_rows);
   p.sums = count_sums(a);
   const size_t need = static_cast<size_t>(items) * p.parts * s.Y * p.sums * a->cols * 4;
   ANIMA_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need),
@@ -583,12 +1017,26 @@ extern "C" int anima_residual_norm_backward(anima_ctx* ctx, const anima_residual
   p.s_gate = slot(a->dgate, true);
   p.s_prew = slot(a->dpre_w, false);
   p.s_postw = slot(a->dpost_w, false);
-  const Kernel fn = s.V == 8 ? (s.NV == 1 ? residual_norm_grad_kernel<8, 1> : residual_norm_grad_kernel<8, 2>)
-                             : (s.NV == 8 ? residual_norm_grad_kernel<1, 8> : residual_norm_grad_kernel<1, 16>);
+  const bool mods = a->gate || a->scale || a->shift, weights = a->pre_w || a->post_w;
+  Kernel fn = s.V == 8 ? (s.NV == 1 ? residual_norm_grad_kernel<8, 1> : residual_norm_grad_kernel<8, 2>)
+                       : (s.NV == 8 ? residual_norm_grad_kernel<1, 8> : residual_norm_grad_kernel<1, 16>);
+  int smem = 0;
+  if (s.full) {
+    const Kernel fns[2][2][2] = {{{residual_norm_grad_full_kernel<1, false, false>, residual_norm_grad_full_kernel<1, false, true>},
+                                  {residual_norm_grad_full_kernel<1, true, false>, residual_norm_grad_full_kernel<1, true, true>}},
+                                 {{residual_norm_grad_full_kernel<2, false, false>, residual_norm_grad_full_kernel<2, false, true>},
+                                  {residual_norm_grad_full_kernel<2, true, false>, residual_norm_grad_full_kernel<2, true, true>}}};
+    fn = fns[s.NV - 1][a->gate || a->scale || a->shift][a->pre_w || a->post_w];
+    const int row = a->cols * (size_of_host(a->x_dtype) * (a->dx_out ? 2 : 1) + size_of_host(a->y_dtype) + size_of_host(a->h_dtype));
+    p.places = places_of(s, kGradThreads, row);
+    smem = p.places * row;
+    st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), 2 * kMaxCols * 16);
+    if (st) return st;
+  }
   ANIMA_REQUIRE(static_cast<long long>(items) * p.parts < (1LL << 31) && items <= 65535,
                 "anima_residual_norm_backward: %d items are too many", items);
   ProfScope prof(ctx, "residual_norm.grad", 0, static_cast<double>(a->rows) * a->cols * 20);
-  fn<<<items * p.parts, dim3(s.T, s.Y), 0, ctx->stream>>>(p);
+  fn<<<items * p.parts, dim3(s.T, s.Y), smem, ctx->stream>>>(p);
   st = check_launch("residual_norm_grad_kernel");
   if (st || p.sums == 0) return st;
   sp.part = p.part;
