@@ -67,27 +67,30 @@ def _contig_rows(t: torch.Tensor):
         raise dev.AnimaError(1, "expected a 2-D tensor with contiguous rows")
 
 
-def _rows(fn: str, name: str, t: torch.Tensor, rows: int, cols: int, dtype=None, device=None, exact: bool = False):
-    """Refuse what is not `rows` contiguous rows of at least (exact: just) `cols` columns of a kernel type."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or (exact and t.shape[1] != cols):
-        raise dev.AnimaError(1, f"{fn}: {name} is {tuple(t.shape)}, expected [{rows}, {cols}]")
-    if cols and t.stride(1) != 1 and t.shape[1] > 1 or (rows > 1 and t.stride(0) < 0):
-        raise dev.AnimaError(1, f"{fn}: {name} needs contiguous rows (strides {t.stride()})")
-    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
-        raise dev.AnimaError(1, f"{fn}: {name} is {t.dtype}" + (f", expected {dtype}" if dtype is not None else ""))
-    if device is not None and t.device != device:
-        raise dev.AnimaError(1, f"{fn}: {name} is on {t.device}, expected {device}")
+def _rows(fn: str, name: str, t: torch.Tensor, rows: int, cols: int, dtype=None, device=None, exact: bool = False) -> int:
+    """Refuse what is not `rows` contiguous rows of at least (exact: just) `cols` columns of a kernel
+    type, on device index `device`; returns the row stride. (Small calls are bound by the host: each
+    attribute of a tensor is asked for once.)"""
+    shape, st, dt = t.shape, t.stride(), t.dtype
+    if len(shape) != 2 or shape[0] != rows or (shape[1] != cols if exact else shape[1] < cols):
+        raise dev.AnimaError(1, f"{fn}: {name} is {tuple(shape)}, expected [{rows}, {cols}]")
+    if st[1] != 1 and shape[1] > 1:
+        raise dev.AnimaError(1, f"{fn}: {name} needs contiguous rows (strides {st})")
+    if dt not in _FLOATS or (dtype is not None and dt is not dtype):
+        raise dev.AnimaError(1, f"{fn}: {name} is {dt}" + (f", expected {dtype}" if dtype is not None else ""))
+    if device is not None and t.get_device() != device:
+        raise dev.AnimaError(1, f"{fn}: {name} is on {t.device}, expected device {device}")
+    return st[0] if rows > 1 else shape[1]  # a single row's stride says nothing
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Row stride of what _rows has let pass (a single row's stride says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+_FLOATS = frozenset((torch.float32, torch.bfloat16, torch.float16))
 
 
-def _vector(fn: str, name: str, t: torch.Tensor, n: int, dtype, device):
-    """Refuse what is not a dense vector of n elements of `dtype` on `device`."""
-    if t.dim() != 1 or t.numel() != n or t.dtype != dtype or not t.is_contiguous() or t.device != device:
-        raise dev.AnimaError(1, f"{fn}: {name} has to be a dense {dtype} [{n}] on {device}, is {t.dtype} "
+def _vector(fn: str, name: str, t: torch.Tensor, n: int, dtype, device: int):
+    """Refuse what is not a dense vector of n elements of `dtype` on device index `device`."""
+    shape = t.shape
+    if len(shape) != 1 or shape[0] != n or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != device:
+        raise dev.AnimaError(1, f"{fn}: {name} has to be a dense {dtype} [{n}] on device {device}, is {t.dtype} "
                                 f"{tuple(t.shape)} on {t.device}")
 
 
@@ -212,26 +215,27 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, *, H
     (2i, 2i + 1) when interleaved; the other dims are copied. Row r stands at positions[r] (int32), or
     at offset + r % rows_per_item (default: all rows are one item). inverse: the transposed rotation,
     for gradients. Returns (out_q, out_k), new tensors unless given; out_q may be q itself."""
-    _rows("rotary", "q", q, q.shape[0], Hq * D)
-    rows = q.shape[0]
+    rows, dt, at, R = q.shape[0], q.dtype, q.get_device(), inv_freq.shape[0] * 2
+    a = dev.RotaryArgs(dtype=dev.DTYPE_CODE.get(dt, -1), rows=rows, D=D, R=R, Hq=Hq, mscale=mscale, offset=offset,
+                       rows_per_item=rows_per_item or max(rows, 1), interleaved=interleaved, inverse=inverse)
+    a.ldq = _rows("rotary", "q", q, rows, Hq * D)
     if out_q is None:
-        out_q = torch.empty(rows, Hq * D, dtype=q.dtype, device=q.device)
-    _rows("rotary", "out_q", out_q, rows, Hq * D, q.dtype, q.device)
-    a = dev.RotaryArgs(dtype=_dt(q), rows=rows, D=D, R=2 * inv_freq.numel(), q=q.data_ptr(), ldq=_ld(q), Hq=Hq,
-                       out_q=out_q.data_ptr(), ldoq=_ld(out_q), inv_freq=inv_freq.data_ptr(), mscale=mscale,
-                       offset=offset, rows_per_item=rows_per_item or max(rows, 1), interleaved=interleaved,
-                       inverse=inverse)
+        out_q, a.ldoq = torch.empty((rows, Hq * D), dtype=dt, device=q.device), Hq * D
+    else:
+        a.ldoq = _rows("rotary", "out_q", out_q, rows, Hq * D, dt, at)
+    a.q, a.out_q, a.inv_freq = q.data_ptr(), out_q.data_ptr(), inv_freq.data_ptr()
     if k is not None:
+        a.ldk, a.Hk = _rows("rotary", "k", k, rows, Hk * D, dt, at), Hk
         if out_k is None:
-            out_k = torch.empty(rows, Hk * D, dtype=q.dtype, device=q.device)
-        _rows("rotary", "k", k, rows, Hk * D, q.dtype, q.device)
-        _rows("rotary", "out_k", out_k, rows, Hk * D, q.dtype, q.device)
-        a.k, a.ldk, a.Hk, a.out_k, a.ldok = k.data_ptr(), _ld(k), Hk, out_k.data_ptr(), _ld(out_k)
+            out_k, a.ldok = torch.empty((rows, Hk * D), dtype=dt, device=q.device), Hk * D
+        else:
+            a.ldok = _rows("rotary", "out_k", out_k, rows, Hk * D, dt, at)
+        a.k, a.out_k = k.data_ptr(), out_k.data_ptr()
     elif Hk or out_k is not None:
         raise dev.AnimaError(1, "rotary: Hk or out_k without k")
-    _vector("rotary", "inv_freq", inv_freq, inv_freq.numel(), torch.float64, q.device)
+    _vector("rotary", "inv_freq", inv_freq, R // 2, torch.float64, at)
     if positions is not None:
-        _vector("rotary", "positions", positions, rows, torch.int32, q.device)
+        _vector("rotary", "positions", positions, rows, torch.int32, at)
         a.positions = positions.data_ptr()
     ctx_for(q).call("anima_rotary", C.byref(a))
     return out_q, out_k
@@ -246,30 +250,32 @@ def _residual_norm_args(fn, x, y, alpha, gate, post, post_w, pre, pre_w, scale, 
         raise dev.AnimaError(1, f"{fn}: post {post!r} (None, 'rms' or 'layer'), pre {pre!r} ('rms' or 'layer')")
     if x.dim() != 2:
         raise dev.AnimaError(1, f"{fn}: x has to be a 2-D tensor of rows")
-    rows, cols = x.shape
-    _rows(fn, "y", y, rows, cols, None, x.device, exact=True)
+    (rows, cols), at = x.shape, x.get_device()
     L = rows_per_item or max(rows, 1)
-    a = dev.ResidualNormArgs(rows=rows, cols=cols, rows_per_item=L, x_dtype=_dt(x), y_dtype=_dt(y), post=NORM_KIND[post],
-                             pre=NORM_KIND[pre], alpha=alpha, eps=eps, y=y.data_ptr(), ldy=_ld(y))
     items = rows // L
+    a = dev.ResidualNormArgs(rows=rows, cols=cols, rows_per_item=L, post=NORM_KIND[post], pre=NORM_KIND[pre], alpha=alpha,
+                             eps=eps)
+    a.ldy = _rows(fn, "y", y, rows, cols, None, at, exact=True)
+    a.x_dtype, a.y_dtype, a.y = dev.DTYPE_CODE.get(x.dtype, -1), _dt(y), y.data_ptr()
     for name, m in (("gate", gate), ("scale", scale), ("shift", shift)):
         if m is None:
             continue
         if m.dim() == 1:
-            _vector(fn, name, m, cols, torch.float32, x.device)
+            _vector(fn, name, m, cols, torch.float32, at)
             if items > 1:
                 raise dev.AnimaError(1, f"{fn}: {name} [{cols}] for {items} items of rows (a [items, cols] tensor)")
             ld = cols
         else:
-            _rows(fn, name, m, items, cols, torch.float32, x.device, exact=True)
-            ld = _ld(m)
+            ld = _rows(fn, name, m, items, cols, torch.float32, at, exact=True)
         setattr(a, name, m.data_ptr())
         setattr(a, "ld_" + name, ld)
-    for name, w in (("post_w", post_w), ("pre_w", pre_w)):
-        if w is not None:
-            _vector(fn, name, w, cols, torch.float32, x.device)
-            setattr(a, name, w.data_ptr())
-    return a
+    if post_w is not None:
+        _vector(fn, "post_w", post_w, cols, torch.float32, at)
+        a.post_w = post_w.data_ptr()
+    if pre_w is not None:
+        _vector(fn, "pre_w", pre_w, cols, torch.float32, at)
+        a.pre_w = pre_w.data_ptr()
+    return a, rows, cols, at
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, *, alpha: float = 1.0, gate: torch.Tensor | None = None,
@@ -284,19 +290,22 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, alpha: float = 1.0, gate:
     taking those of item r // rows_per_item; post_w, pre_w: fp32 [cols]. h has out_dtype (default
     x's). x_out may be x itself. The reference runs the gate and the adaLN norm apart (dit.js:261-314)."""
     fn = "residual_norm"
-    a = _residual_norm_args(fn, x, y, alpha, gate, post, post_w, pre, pre_w, scale, shift, eps, rows_per_item)
-    _rows(fn, "x", x, a.rows, a.cols)
+    a, rows, cols, at = _residual_norm_args(fn, x, y, alpha, gate, post, post_w, pre, pre_w, scale, shift, eps,
+                                            rows_per_item)
+    dt, a.ldx = x.dtype, _rows(fn, "x", x, rows, cols)
     if x_out is None:
-        x_out = torch.empty(a.rows, a.cols, dtype=x.dtype, device=x.device)
+        x_out, a.ldx_out = torch.empty((rows, cols), dtype=dt, device=x.device), cols
+    else:
+        a.ldx_out = _rows(fn, "x_out", x_out, rows, cols, dt, at, exact=True)
     if h is None:
-        h = torch.empty(a.rows, a.cols, dtype=out_dtype or x.dtype, device=x.device)
+        h, a.ldh = torch.empty((rows, cols), dtype=out_dtype or dt, device=x.device), cols
+        if h.dtype not in _FLOATS:
+            raise dev.AnimaError(1, f"{fn}: out_dtype {out_dtype}")
     elif out_dtype not in (None, h.dtype):
         raise dev.AnimaError(1, f"{fn}: h is {h.dtype}, out_dtype {out_dtype}")
-    _rows(fn, "x_out", x_out, a.rows, a.cols, x.dtype, x.device, exact=True)
-    _rows(fn, "h", h, a.rows, a.cols, None, x.device, exact=True)
-    a.h_dtype = _dt(h)
-    a.x, a.ldx, a.x_out, a.ldx_out = x.data_ptr(), _ld(x), x_out.data_ptr(), _ld(x_out)
-    a.h, a.ldh = h.data_ptr(), _ld(h)
+    else:
+        a.ldh = _rows(fn, "h", h, rows, cols, None, at, exact=True)
+    a.h_dtype, a.x, a.x_out, a.h = _dt(h), x.data_ptr(), x_out.data_ptr(), h.data_ptr()
     ctx_for(x).call("anima_residual_norm", C.byref(a))
     return x_out, h
 
@@ -325,27 +334,28 @@ def residual_norm_backward(dh: torch.Tensor, dx_out: torch.Tensor | None, x_out:
     forward's arguments. dx (x's type) may be dx_out itself, dy (y's type) y itself. Statistics are
     computed again in fp32 from y and the stored x_out; column sums are in fp32 and of fixed order."""
     fn = "residual_norm_backward"
-    a = _residual_norm_args(fn, x_out, y, alpha, gate, post, post_w, pre, pre_w, scale, shift, eps, rows_per_item)
-    rows, cols, dv = a.rows, a.cols, x_out.device
-    _rows(fn, "x_out", x_out, rows, cols)
-    _rows(fn, "dh", dh, rows, cols, None, dv, exact=True)
-    dx = torch.empty(rows, cols, dtype=x_out.dtype, device=dv) if dx is None else dx
-    dy = torch.empty(rows, cols, dtype=y.dtype, device=dv) if dy is None else dy
-    _rows(fn, "dx", dx, rows, cols, x_out.dtype, dv, exact=True)
-    _rows(fn, "dy", dy, rows, cols, y.dtype, dv, exact=True)
-    a.x_out, a.ldx_out, a.h_dtype = x_out.data_ptr(), _ld(x_out), _dt(dh)
-    a.dh, a.lddh, a.dx, a.lddx, a.dy, a.lddy = (dh.data_ptr(), _ld(dh), dx.data_ptr(), _ld(dx), dy.data_ptr(),
-                                                _ld(dy))
+    a, rows, cols, at = _residual_norm_args(fn, x_out, y, alpha, gate, post, post_w, pre, pre_w, scale, shift, eps,
+                                            rows_per_item)
+    dt, dv = x_out.dtype, x_out.device
+    a.ldx_out, a.lddh = _rows(fn, "x_out", x_out, rows, cols), _rows(fn, "dh", dh, rows, cols, None, at, exact=True)
+    if dx is None:
+        dx, a.lddx = torch.empty((rows, cols), dtype=dt, device=dv), cols
+    else:
+        a.lddx = _rows(fn, "dx", dx, rows, cols, dt, at, exact=True)
+    if dy is None:
+        dy, a.lddy = torch.empty((rows, cols), dtype=y.dtype, device=dv), cols
+    else:
+        a.lddy = _rows(fn, "dy", dy, rows, cols, y.dtype, at, exact=True)
+    a.h_dtype, a.x_out, a.dh, a.dx, a.dy = _dt(dh), x_out.data_ptr(), dh.data_ptr(), dx.data_ptr(), dy.data_ptr()
     if dx_out is not None:
-        _rows(fn, "dx_out", dx_out, rows, cols, x_out.dtype, dv, exact=True)
-        a.dx_out, a.lddx_out = dx_out.data_ptr(), _ld(dx_out)
+        a.lddx_out, a.dx_out = _rows(fn, "dx_out", dx_out, rows, cols, dt, at, exact=True), dx_out.data_ptr()
     grads = {}
-    for name, t in (("gate", gate), ("post_w", post_w), ("pre_w", pre_w), ("scale", scale), ("shift", shift)):
+    for name, t in (("dgate", gate), ("dpost_w", post_w), ("dpre_w", pre_w), ("dscale", scale), ("dshift", shift)):
         g = None
         if t is not None:
             g = (torch.empty if rows else torch.zeros)(t.shape, dtype=torch.float32, device=dv)
-            setattr(a, "d" + name, g.data_ptr())
-        grads["d" + name] = g
+            setattr(a, name, g.data_ptr())
+        grads[name] = g
     ctx = ctx_for(x_out)
     need = C.c_size_t()
     dev.check(ctx.lib.anima_residual_norm_backward_workspace(ctx.h, C.byref(a), C.byref(need)))
@@ -512,9 +522,12 @@ def _reach(fn: str, name: str, t: torch.Tensor, off: int, items: int, bstride: i
         raise dev.AnimaError(1, f"{fn}: {name}'s row stride {ld} is below its {off} + {cols} columns, or its batch "
                                 f"stride {bstride} negative")
     need = off + (items - 1) * bstride + (rows - 1) * ld + cols
-    have = t.numel() if t.is_contiguous() else t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
-    if need > have:
-        raise dev.AnimaError(1, f"{fn}: {name} has {have} elements, its sizes and strides reach {need}")
+    if t.is_contiguous() and need <= t.numel():
+        return
+    have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+    if t.is_contiguous() or need > have:
+        raise dev.AnimaError(1, f"{fn}: {name} has {t.numel()} elements ({have} behind its start), its sizes and strides "
+                                f"reach {need}")
 
 
 def _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, batch, q_bstride, k_bstride, v_bstride,
@@ -527,48 +540,46 @@ def _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, b
         raise dev.AnimaError(1, f"{fn}: head_dim {D} (64 or 128)")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise dev.AnimaError(1, f"{fn}: q, k and v are bf16 or fp16, not {q.dtype}")
-    C, Ck = H * D, H // group * D
-    a = dev.AttentionArgs(batch=batch, heads=H, head_dim=D, Lq=Lq, Lk=Lk, dtype=_dt(q), scale=scale or 0.0, group=group,
-                          causal=bool(causal))
-    kv_items = batch
-    if batch > 1 and k_bstride == 0 and v_bstride == 0:
-        kv_items = 1
-    for n, t, ld, off, items, bs, L, cols in (("q", q, ldq or C, q_off, batch, q_bstride, Lq, C),
-                                              ("k", k, ldk or Ck, k_off, kv_items, k_bstride, Lk, Ck),
-                                              ("v", v, ldv or Ck, v_off, kv_items, v_bstride, Lk, Ck)):
-        if t.dtype != q.dtype or t.device != q.device:
+    C, Ck, dt, at = H * D, H // group * D, q.dtype, q.get_device()
+    kv_items = 1 if batch > 1 and k_bstride == 0 and v_bstride == 0 else batch
+    ldq, ldk, ldv = ldq or C, ldk or Ck, ldv or Ck
+    for n, t, ld, off, items, bs, L, cols in (("q", q, ldq, q_off, batch, q_bstride, Lq, C),
+                                              ("k", k, ldk, k_off, kv_items, k_bstride, Lk, Ck),
+                                              ("v", v, ldv, v_off, kv_items, v_bstride, Lk, Ck)):
+        if t.dtype is not dt or t.get_device() != at:
             raise dev.AnimaError(1, f"{fn}: {n} is {t.dtype} on {t.device}, q {q.dtype} on {q.device}")
         if items > 1 and bs <= 0:
             raise dev.AnimaError(1, f"{fn}: {n}_bstride {bs} with {batch} items (k and v may both have 0: shared)")
         _reach(fn, n, t, off, items, bs, L, ld, cols)
-        setattr(a, n, t.data_ptr())
-        setattr(a, "ld" + n, ld)
-        setattr(a, n + "_off", off)
-        setattr(a, n + "_bstride", bs)
+    a = dev.AttentionArgs(batch, H, D, Lq, Lk, dev.DTYPE_CODE[dt], q.data_ptr(), ldq, q_bstride, q_off, k.data_ptr(), ldk,
+                          k_bstride, k_off, v.data_ptr(), ldv, v_bstride, v_off)
+    a.scale, a.group, a.causal = scale or 0.0, group, bool(causal)
     if key_len is not None:
-        _vector(fn, "key_len", key_len, key_len.numel(), torch.int32, q.device)
+        _vector(fn, "key_len", key_len, key_len.numel(), torch.int32, at)
         if key_len.numel() < kv_items:
             raise dev.AnimaError(1, f"{fn}: {key_len.numel()} key lengths for {kv_items} k/v items")
         a.key_len = key_len.data_ptr()
     if out is not None:
-        a.o_bstride = _grad_out(fn, "out", out, batch, Lq, C, o_bstride, q.device)
-        a.out, a.ldo, a.out_dtype = out.data_ptr(), _ld(out), _dt(out)
+        a.ldo, a.o_bstride = _grad_out(fn, "out", out, batch, Lq, C, o_bstride, at)
+        a.out, a.out_dtype = out.data_ptr(), _dt(out)
     return a, kv_items, Ck
 
 
-def _grad_out(fn, name, t, items, L, cols, bstride, device, dtype=None) -> int:
+def _grad_out(fn, name, t, items, L, cols, bstride, device, dtype=None) -> tuple[int, int]:
     """Check a 2-D [items * L, >= cols] tensor (rows of item b from b * bstride on where that is given)
-    and return its batch stride."""
-    if t.dim() != 2 or t.stride(1) != 1 or t.device != device or t.dtype not in dev.DTYPE_CODE or \
-            (dtype is not None and t.dtype != dtype):
+    and return its row and batch strides."""
+    shape, st, dt = t.shape, t.stride(), t.dtype
+    if len(shape) != 2 or st[1] != 1 or t.get_device() != device or dt not in _FLOATS or (dtype is not None and dt is not dtype):
         raise dev.AnimaError(1, f"{fn}: {name} has to be 2-D with contiguous rows" +
-                                (f", {dtype}" if dtype is not None else "") + f", on {device}; is {t.dtype} "
+                                (f", {dtype}" if dtype is not None else "") + f", on device {device}; is {t.dtype} "
                                 f"{tuple(t.shape)} on {t.device}")
-    bs = bstride if bstride is not None else L * _ld(t)
-    if bstride is None and t.shape[0] < items * L:
-        raise dev.AnimaError(1, f"{fn}: {name} is {tuple(t.shape)}, expected [{items * L}, {cols}]")
-    _reach(fn, name, t, 0, items, bs, L, _ld(t), cols)
-    return bs
+    ld = st[0] if shape[0] > 1 else shape[1]
+    if bstride is None:
+        if shape[0] < items * L or shape[1] < cols or ld < cols:
+            raise dev.AnimaError(1, f"{fn}: {name} is {tuple(t.shape)}, expected [{items * L}, {cols}]")
+        return ld, L * ld
+    _reach(fn, name, t, 0, items, bstride, L, ld, cols)
+    return ld, bstride
 
 
 def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, Lq: int, Lk: int, H: int, D: int = 128,
@@ -592,7 +603,7 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, Lq: int,
     need = C.c_size_t()
     dev.check(ctx.lib.anima_attention_lse_workspace(ctx.h, C.byref(a), C.byref(need)))
     ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-    ctx.call("anima_attention_lse", C.byref(a), ptr(lse), ptr(ws), need, tag=name, work=4.0 * batch * Lq * Lk * D * H)
+    ctx.call("anima_attention_lse", C.byref(a), lse.data_ptr(), ws.data_ptr() if need.value else None, need, tag=name, work=4.0 * batch * Lq * Lk * D * H)
     return out, lse
 
 
@@ -615,27 +626,35 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         raise dev.AnimaError(1, f"{fn}: out and dout are 2-D [batch * Lq, H D]")
     a, kv_items, Ck = _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, batch, q_bstride,
                                   k_bstride, v_bstride, key_len, out, o_bstride, scale, group, causal)
-    dv_ = q.device
-    if lse.dtype != torch.float32 or lse.shape != (batch, H, Lq) or not lse.is_contiguous() or lse.device != dv_:
-        raise dev.AnimaError(1, f"{fn}: lse has to be a dense fp32 [{batch}, {H}, {Lq}] on {dv_}")
-    gt = next((t.dtype for t in (dq, dk, dv) if t is not None), grad_dtype or q.dtype)
+    at, device, Cq = q.get_device(), q.device, H * D
+    if lse.dtype is not torch.float32 or lse.shape != (batch, H, Lq) or not lse.is_contiguous() or lse.get_device() != at:
+        raise dev.AnimaError(1, f"{fn}: lse has to be a dense fp32 [{batch}, {H}, {Lq}] on {device}")
+    gt = grad_dtype or q.dtype
+    for t in (dv, dk, dq):
+        if t is not None:
+            gt = t.dtype
     if gt not in (torch.float32, q.dtype) or grad_dtype not in (None, gt):
         raise dev.AnimaError(1, f"{fn}: gradients are {gt}, have to be {q.dtype} or fp32 (grad_dtype {grad_dtype})")
-    new = lambda rows, cols: torch.empty(rows, cols, dtype=gt, device=dv_)  # noqa: E731
-    dq = new(batch * Lq, H * D) if dq is None else dq
-    dk = new(kv_items * Lk, Ck) if dk is None else dk
-    dv = new(kv_items * Lk, Ck) if dv is None else dv
-    g = dev.AttentionGradArgs(fwd=a, lse=lse.data_ptr(), grad_dtype=dev.DTYPE_CODE[gt])
-    g.do_bstride = _grad_out(fn, "dout", dout, batch, Lq, H * D, do_bstride, dv_, q.dtype)
-    g.dout, g.lddo = dout.data_ptr(), _ld(dout)
-    g.dq_bstride = _grad_out(fn, "dq", dq, batch, Lq, H * D, None, dv_, gt)
-    g.dk_bstride = _grad_out(fn, "dk", dk, kv_items, Lk, Ck, None, dv_, gt)
-    g.dv_bstride = _grad_out(fn, "dv", dv, kv_items, Lk, Ck, None, dv_, gt)
-    g.dq, g.lddq, g.dk, g.lddk, g.dv, g.lddv = (dq.data_ptr(), _ld(dq), dk.data_ptr(), _ld(dk), dv.data_ptr(), _ld(dv))
+    g = dev.AttentionGradArgs()
+    g.fwd, g.lse, g.dout, g.grad_dtype = a, lse.data_ptr(), dout.data_ptr(), dev.DTYPE_CODE[gt]
+    g.lddo, g.do_bstride = _grad_out(fn, "dout", dout, batch, Lq, Cq, do_bstride, at, q.dtype)
+    if dq is None:
+        dq, g.lddq, g.dq_bstride = torch.empty((batch * Lq, Cq), dtype=gt, device=device), Cq, Lq * Cq
+    else:
+        g.lddq, g.dq_bstride = _grad_out(fn, "dq", dq, batch, Lq, Cq, None, at, gt)
+    if dk is None:
+        dk, g.lddk, g.dk_bstride = torch.empty((kv_items * Lk, Ck), dtype=gt, device=device), Ck, Lk * Ck
+    else:
+        g.lddk, g.dk_bstride = _grad_out(fn, "dk", dk, kv_items, Lk, Ck, None, at, gt)
+    if dv is None:
+        dv, g.lddv, g.dv_bstride = torch.empty((kv_items * Lk, Ck), dtype=gt, device=device), Ck, Lk * Ck
+    else:
+        g.lddv, g.dv_bstride = _grad_out(fn, "dv", dv, kv_items, Lk, Ck, None, at, gt)
+    g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     ctx = ctx_for(q)
     need = C.c_size_t()
     dev.check(ctx.lib.anima_attention_backward_workspace(ctx.h, C.byref(g), C.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dv_)
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
     g.workspace, g.workspace_bytes = ws.data_ptr(), need.value
     ctx.call("anima_attention_backward", C.byref(g), tag=name, work=10.0 * batch * Lq * Lk * D * H, kernels=2)
     return dq, dk, dv
