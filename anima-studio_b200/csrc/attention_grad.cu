@@ -757,9 +757,9 @@ struct PrepParams {
   const void* dout;
   const float* lse;
   long long ldo, o_bs, lddo, do_bs;
-  int out_dtype, B, H, group, Lq, Lqp, kv_batch;
+  int out_dtype, H, group, Lq, Lqp, kv_batch;
   float shift;  // 14 in fp16
-  float scale_log2;
+  float inv_scale_log2;
   float *nlse2, *ndelta;
   uint8_t* stat;
   const unsigned* top;
@@ -778,59 +778,67 @@ __device__ __forceinline__ uint2 three_parts(float v) {
   return make_uint2(pack2<BF16>(part[0], part[1]), pack2<BF16>(part[2], 0.f));
 }
 
-__device__ __forceinline__ void load8(const void* p, int dtype, size_t at, float (&v)[8]) {
-  if (dtype == ANIMA_F32) {
-    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-    const float4 a = q[0], b = q[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-  const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = resnorm::lo16(w[i], dtype);
-    v[2 * i + 1] = resnorm::hi16(w[i], dtype);
-  }
-}
+constexpr int kPrepRows = 2;  // (row, head) pairs of a thread, their loads in flight together
 
 template <bool BF16, int HD>
 __global__ void __launch_bounds__(256) attention_grad_prep_kernel(const PrepParams p) {
-  constexpr int TPR = HD / 8;
-  const long long id = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / TPR;
-  const int t = threadIdx.x % TPR;
-  const long long rows = static_cast<long long>(p.B) * p.Lqp;
-  const long long row = id / p.H;
-  const int h = static_cast<int>(id - row * p.H);
-  const bool in = row < rows;
-  const int b = in ? static_cast<int>(row / p.Lqp) : 0;
-  const int i = in ? static_cast<int>(row - static_cast<long long>(b) * p.Lqp) : 0;
-  const bool real = in && i < p.Lq;
-  float d = 0.f;
-  if (real) {
-    float o[8], g[8];
-    load8(p.out, p.out_dtype, static_cast<size_t>(b) * p.o_bs + i * p.ldo + static_cast<size_t>(h) * HD + 8 * t, o);
-    load8(p.dout, BF16 ? ANIMA_BF16 : ANIMA_F16, static_cast<size_t>(b) * p.do_bs + i * p.lddo + static_cast<size_t>(h) * HD + 8 * t, g);
+  using resnorm::load_raw;
+  using resnorm::unpack;
+  constexpr int TPR = HD / 8, PAIRS = 256 / TPR;
+  const int b = blockIdx.y, t = threadIdx.x % TPR;
+  const unsigned pairs = static_cast<unsigned>(p.Lqp) * p.H;
+  unsigned row[kPrepRows], h[kPrepRows];
+  bool in[kPrepRows], real[kPrepRows];
+  resnorm::Raw<8> o[kPrepRows], g[kPrepRows];
+  float lse[kPrepRows];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) d = fmaf(o[j], g[j], d);
+  for (int u = 0; u < kPrepRows; ++u) {
+    const unsigned id = (blockIdx.x * kPrepRows + u) * PAIRS + threadIdx.x / TPR;
+    in[u] = id < pairs;
+    row[u] = id / p.H;
+    h[u] = id - row[u] * p.H;
+    real[u] = in[u] && row[u] < static_cast<unsigned>(p.Lq);
+    lse[u] = -INFINITY;
+    if (real[u]) {
+      const size_t col = static_cast<size_t>(h[u]) * HD + 8 * t;
+      load_raw<8>(o[u], p.out, p.out_dtype, b * p.o_bs + row[u] * p.ldo + col);
+      load_raw<8>(g[u], p.dout, BF16 ? ANIMA_BF16 : ANIMA_F16, b * p.do_bs + row[u] * p.lddo + col);
+      lse[u] = p.lse[(static_cast<size_t>(b) * p.H + h[u]) * p.Lq + row[u]];
+    }
   }
 #pragma unroll
-  for (int s = TPR / 2; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-  if (!in || t) return;
-  const size_t at = (static_cast<size_t>(b) * p.H + h) * p.Lqp + i;
-  const float l = real ? p.lse[(static_cast<size_t>(b) * p.H + h) * p.Lq + i] : -INFINITY;
-  const float nl = l == -INFINITY ? -INFINITY : fmaf(l, -1.4426950408889634f, p.shift);
-  p.nlse2[at] = nl;
-  p.ndelta[at] = -d;
-  uint8_t* tile = p.stat + ((static_cast<size_t>(b) * p.H + h) * (p.Lqp / TILE) + i / TILE) * (2 * STAT_TILE) + stat_row(i % TILE);
-  float unit = 1.f;
-  if (!BF16) unit = delta_unit(ds_exponent(p.top, (p.kv_batch > 1 ? b : 0) * (p.H / p.group) + h / p.group));
-  const uint2 lp = three_parts<BF16>(nl / p.scale_log2 * (BF16 ? 1.f : 1.f / kLse16)), dp = three_parts<BF16>(-d / unit);
-  *reinterpret_cast<uint4*>(tile) = make_uint4(lp.x, lp.y, 0u, 0u);
-  *reinterpret_cast<uint4*>(tile + 128) = make_uint4(0u, 0u, 0u, 0u);
-  *reinterpret_cast<uint4*>(tile + STAT_TILE) = make_uint4(dp.x, dp.y, 0u, 0u);
-  *reinterpret_cast<uint4*>(tile + STAT_TILE + 128) = make_uint4(0u, 0u, 0u, 0u);
+  for (int u = 0; u < kPrepRows; ++u) {
+    float d = 0.f;
+    if (real[u]) {
+      float x[8], y[8];
+      unpack<8>(o[u], p.out_dtype, x);
+      unpack<8>(g[u], BF16 ? ANIMA_BF16 : ANIMA_F16, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d = fmaf(x[j], y[j], d);
+    }
+#pragma unroll
+    for (int s = TPR / 2; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+    if (!in[u]) continue;
+    const size_t bh = static_cast<size_t>(b) * p.H + h[u];
+    const float nl = lse[u] == -INFINITY ? -INFINITY : fmaf(lse[u], -1.4426950408889634f, p.shift);
+    // the row's lanes share its writes
+    if (t == 0) p.nlse2[bh * p.Lqp + row[u]] = nl;
+    if (t == 1) p.ndelta[bh * p.Lqp + row[u]] = -d;
+    if (t >= 2 && t < 6) {
+      const int which = (t - 2) >> 1, half = t & 1;
+      uint8_t* tile = p.stat + ((bh * (p.Lqp / TILE) + row[u] / TILE) * 2 + which) * STAT_TILE + stat_row(row[u] % TILE) + half * 128;
+      uint2 parts = make_uint2(0u, 0u);
+      if (!half) {
+        float v = nl * p.inv_scale_log2 * (BF16 ? 1.f : 1.f / kLse16);
+        if (which) {
+          v = -d;
+          if (!BF16) v /= delta_unit(ds_exponent(p.top, (p.kv_batch > 1 ? b : 0) * (p.H / p.group) + h[u] / p.group));
+        }
+        parts = three_parts<BF16>(v);
+      }
+      *reinterpret_cast<uint4*>(tile) = make_uint4(parts.x, parts.y, 0u, 0u);
+    }
+  }
 }
 
 // fp16: the largest |dO_i|^2 and |V_j|^2 of each k/v head, over all queries and the keys that count; a
@@ -986,8 +994,9 @@ template <bool BF16, int HD>
 int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, const Params& p, const PrepParams& pp,
            const CUtensorMap (&tm)[4]) {
   const anima_attention_args* a = &g->fwd;
-  const long long threads = static_cast<long long>(a->batch) * pl.Lqp * a->heads * (HD / 8);
-  ANIMA_REQUIRE((threads + 255) / 256 < (1LL << 31), "anima_attention_backward: problem too large");
+  const long long pairs = static_cast<long long>(pl.Lqp) * a->heads;
+  ANIMA_REQUIRE(pairs < (1LL << 31) && a->batch <= 65535, "anima_attention_backward: problem too large");
+  constexpr int kPairs = kPrepRows * 256 / (HD / 8);  // of a block
   ProfScope prof(ctx, "attn.grad", 10.0 * a->batch * a->heads * static_cast<double>(a->Lq) * a->Lk * HD, 0);
   if (!BF16) {
     ANIMA_CUDA(cudaMemsetAsync(const_cast<unsigned*>(pp.top), 0, pl.top_bytes, ctx->stream));
@@ -1013,7 +1022,8 @@ int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, c
     const int st = check_launch("attention_grad_top_kernel");
     if (st) return st;
   }
-  attention_grad_prep_kernel<BF16, HD><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, ctx->stream>>>(pp);
+  attention_grad_prep_kernel<BF16, HD>
+      <<<dim3(static_cast<unsigned>((pairs + kPairs - 1) / kPairs), a->batch), 256, 0, ctx->stream>>>(pp);
   int st = check_launch("attention_grad_prep_kernel");
   if (st) return st;
   const auto fn = attention_grad_kernel<BF16, HD>;
@@ -1153,7 +1163,6 @@ extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_gr
   pp.lddo = g->lddo;
   pp.do_bs = many ? g->do_bstride : 0;
   pp.out_dtype = a->out_dtype;
-  pp.B = a->batch;
   pp.H = a->heads;
   pp.group = pl.group;
   pp.Lq = a->Lq;
@@ -1163,7 +1172,7 @@ extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_gr
   pp.nlse2 = reinterpret_cast<float*>(ws + pl.lse_off);
   pp.ndelta = reinterpret_cast<float*>(ws + pl.delta_off);
   pp.stat = ws + pl.stat_off;
-  pp.scale_log2 = p.scale_log2;
+  pp.inv_scale_log2 = 1.0f / p.scale_log2;
   pp.top = reinterpret_cast<unsigned*>(ws + pl.top_off);
   if (a->dtype == ANIMA_BF16)
     return a->head_dim == 128 ? launch<true, 128>(ctx, g, pl, p, pp, tm) : launch<true, 64>(ctx, g, pl, p, pp, tm);

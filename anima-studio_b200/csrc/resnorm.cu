@@ -99,10 +99,19 @@ __device__ __forceinline__ void unpack(const Raw<V>& r, int dt, float (&v)[V]) {
         v[4 + i] = __uint_as_float(b[i]);
       }
     } else {
+      // (one branch for all eight: a choice for each element would cost more than the row's sums)
+      if (dt == ANIMA_BF16) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = lo16(a[i], dt);
-        v[2 * i + 1] = hi16(a[i], dt);
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = lo16(a[i], ANIMA_BF16);
+          v[2 * i + 1] = hi16(a[i], ANIMA_BF16);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = lo16(a[i], ANIMA_F16);
+          v[2 * i + 1] = hi16(a[i], ANIMA_F16);
+        }
       }
     }
   } else {
@@ -127,8 +136,13 @@ __device__ __forceinline__ void store(void* p, int dt, size_t at, const float (&
       q[0] = make_float4(v[0], v[1], v[2], v[3]);
       q[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
-          make_uint4(pack16(v[0], v[1], dt), pack16(v[2], v[3], dt), pack16(v[4], v[5], dt), pack16(v[6], v[7], dt));
+      uint4* q = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at);
+      if (dt == ANIMA_BF16)
+        *q = make_uint4(pack16(v[0], v[1], ANIMA_BF16), pack16(v[2], v[3], ANIMA_BF16), pack16(v[4], v[5], ANIMA_BF16),
+                        pack16(v[6], v[7], ANIMA_BF16));
+      else
+        *q = make_uint4(pack16(v[0], v[1], ANIMA_F16), pack16(v[2], v[3], ANIMA_F16), pack16(v[4], v[5], ANIMA_F16),
+                        pack16(v[6], v[7], ANIMA_F16));
     }
   } else {
     if (dt == ANIMA_F32)
