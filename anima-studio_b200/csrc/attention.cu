@@ -64,6 +64,7 @@ struct Params {
   int persist;       // whole units, CTA c taking units c, c + grid, ... (grid = SM count)
   int group;         // q heads per k/v head (k/v head = h / group)
   int causal;        // key j visible to query i only when j <= i
+  int heavy_first;   // whole causal units in the order of their length, the longest first
   float* lse;        // TRAIN: [batch][heads][Lq] ln of each row's sum of exponentials
   float* ws;         // [units][PART_FLOATS] partial softmax states of split units
   unsigned* flags;   // [units] tail part written (cleared by the head part)
@@ -161,7 +162,12 @@ __device__ __forceinline__ int build_segments(const Params& p, int4* out) {
     // unit loads its Q and starts its first QK^T while the previous unit's output is written
     const int step = p.persist ? static_cast<int>(gridDim.x) : p.units;
     int n = 0;
-    for (int unit = blockIdx.x; unit < p.units && n < MAX_SEGS; unit += step) {
+    for (int u = blockIdx.x; u < p.units && n < MAX_SEGS; u += step) {
+      int unit = u;
+      if (p.heavy_first) {
+        const int bhs = p.units / p.q_pairs;
+        unit = (u % bhs) * p.q_pairs + p.q_pairs - 1 - u / bhs;
+      }
       const int b = unit / p.q_pairs / p.heads;
       const int kv_len = p.key_len ? min(p.Lk, p.key_len[p.kv_bcast ? 0 : b]) : p.Lk;
       int nblk = kv_len > 0 ? (kv_len + TILE - 1) / TILE : 0;
@@ -1126,6 +1132,11 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratc
     }
     p.stream_k = 1;
     grid = ctx->num_sms;
+  } else if (p.causal && p.q_pairs >= 8 && units > ctx->num_sms) {
+    // long causal units differ in length up to q_pairs-fold: one CTA each, the longest first, so that the
+    // short ones fill the gaps at the end (8192 x 8192 of 16 heads: a fixed share of units per CTA left
+    // one with 1.5 times the mean)
+    p.heavy_first = 1;
   } else if (units > ctx->num_sms && (units + ctx->num_sms - 1) / ctx->num_sms <= attn::MAX_SEGS) {
     // more than one wave of whole units: a persistent grid, one CTA per SM
     p.persist = 1;

@@ -109,8 +109,9 @@ __device__ __forceinline__ void unpack(const Raw<V>& r, int dt, float (&v)[V]) {
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[2 * i] = lo16(a[i], ANIMA_F16);
-          v[2 * i + 1] = hi16(a[i], ANIMA_F16);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
         }
       }
     }
@@ -800,24 +801,26 @@ struct SumParams {
   int per_item[kMaxSums];  // out [items][C], else [C] over all items
 };
 
-// out = the partial rows added in order. A block takes 32 columns of one output row; its 8 warps each
-// add every 8th partial, then the first adds the eight.
-__global__ void __launch_bounds__(256) partial_sum_kernel(const SumParams p) {
-  __shared__ float red[8][32];
+// out = the partial rows added in a fixed order. A block takes 32 columns of one output row; its warps
+// each add every blockDim.y-th partial, then the first adds the warps' sums.
+__global__ void __launch_bounds__(1024) partial_sum_kernel(const SumParams p) {
+  __shared__ float red[32][32];
   const int s = blockIdx.z, item = blockIdx.y;
   if (!p.per_item[s] && item) return;
-  const int c = blockIdx.x * 32 + threadIdx.x;
+  const int c = blockIdx.x * 32 + threadIdx.x, warps = blockDim.y;
   const int n = p.per_item[s] ? p.parts : p.parts * p.items;
-  const float* base = p.part + (static_cast<size_t>(item) * p.parts * p.sums + s) * p.C;
+  const size_t stride = static_cast<size_t>(p.sums) * p.C;
+  const float* base = p.part + (static_cast<size_t>(item) * p.parts * p.sums + s) * p.C + c;
   float t = 0.f;
-  if (c < p.C)
-    for (int i = threadIdx.y; i < n; i += 8) t += base[static_cast<size_t>(i) * p.sums * p.C + c];
+  if (c < p.C) {
+#pragma unroll 4
+    for (int i = threadIdx.y; i < n; i += warps) t += base[i * stride];
+  }
   red[threadIdx.y][threadIdx.x] = t;
   __syncthreads();
   if (threadIdx.y || c >= p.C) return;
   t = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t += red[i][threadIdx.x];
+  for (int i = 0; i < warps; ++i) t += red[i][threadIdx.x];
   p.out[s][static_cast<size_t>(item) * p.C + c] = t;
 }
 
@@ -1058,6 +1061,6 @@ extern "C" int anima_residual_norm_backward(anima_ctx* ctx, const anima_residual
   sp.parts = p.parts * s.Y;
   sp.sums = p.sums;
   sp.C = a->cols;
-  partial_sum_kernel<<<dim3((a->cols + 31) / 32, items, p.sums), dim3(32, 8), 0, ctx->stream>>>(sp);
+  partial_sum_kernel<<<dim3((a->cols + 31) / 32, items, p.sums), dim3(32, sp.parts * items > 296 ? 32 : 8), 0, ctx->stream>>>(sp);
   return check_launch("partial_sum_kernel");
 }
