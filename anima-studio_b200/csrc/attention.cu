@@ -98,7 +98,7 @@ __device__ __forceinline__ void arrive_one_lane(uint64_t* bar) {
 
 // Warp-wide bounded wait: every lane polls, so the common case (phase already complete) has no
 // divergent branch; the result is the AND over the lanes.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned err) {
+__device__ __forceinline__ bool lanes_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned err) {
   const uint32_t a = smem_u32(bar);
   if (__all_sync(0xffffffffu, mbar_test(a, parity))) return true;
   // spin without the suspend hint: the wait is on the critical path
@@ -237,7 +237,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   int* nseg_slot = reinterpret_cast<int*>(tmem_slot + 2);
   int4* segs = reinterpret_cast<int4*>(smem + OFF_SEG);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same for all lanes, and known to be
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -361,45 +362,44 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      const uint32_t id_qk = idesc_f16(TILE, TILE, BF16, false);
-      const uint32_t id_pv = idesc_f16(TILE, HD, BF16, true);
-      const uint32_t sq = smem_u32(smem + OFF_Q);
+    {
+      // the whole warp follows, one lane issues
+      const uint32_t lead = elect_lead();
+      constexpr uint32_t id_qk = idesc_f16(TILE, TILE, BF16, false);
+      constexpr uint32_t id_pv = idesc_f16(TILE, HD, BF16, true);
+      const uint32_t dq = desc_lo(smem_u32(smem + OFF_Q), 16), dk = desc_lo(smem_u32(smem + OFF_K), 16);
+      const uint32_t dv = desc_lo(smem_u32(smem + OFF_V), ATOM);
+      constexpr uint32_t kSlot = TILE_BYTES >> 4;
       auto issue_s = [&](int x, int G) {  // S_x = Q_x K^T for the block in stage G & 1
-        const uint32_t sk = smem_u32(smem + OFF_K + (G & 1) * TILE_BYTES);
-        const uint32_t qx = sq + x * TILE_BYTES;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (k >> 2) * ATOM + (k & 3) * 32;
-          umma_f16(tmem + x * 128, sdesc_sw128(qx + off, 16, 1024), sdesc_sw128(sk + off, 16, 1024), id_qk,
-                   k > 0 ? 1u : 0u);
+          const uint32_t off = ((k >> 2) * ATOM + (k & 3) * 32) >> 4;
+          umma_ss(tmem + x * 128, dq + x * kSlot + off, dk + (G & 1) * kSlot + off, id_qk, k > 0 ? 1u : 0u, lead);
         }
-        umma_commit(&s_full[x]);
+        umma_commit(&s_full[x], lead);
       };
       auto issue_pv = [&](int x, int G, bool first) {  // O_x (+)= P_x V, P from tensor memory
-        const uint32_t sv = smem_u32(smem + OFF_V + (G & 1) * TILE_BYTES);
 #pragma unroll
-        for (int k = 0; k < TILE / 16; ++k) {
-          const uint64_t bd = sdesc_sw128(sv + k * 16 * 128, ATOM, 1024);
-          umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, bd, id_pv, (!first || k > 0) ? 1u : 0u);
-        }
-        umma_commit(&o_done[x]);
+        for (int k = 0; k < TILE / 16; ++k)
+          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, dv + (G & 1) * kSlot + k * (16 * 128 >> 4), id_pv,
+                  (!first || k > 0) ? 1u : 0u, lead);
+        umma_commit(&o_done[x], lead);
       };
       int gb = 0, qn = 0;
       bool ok = true;
       for (int si = 0; ok && si < nseg; ++si) {
         const int nb = segs[si].z - segs[si].y;
         if (nb <= 0) continue;
-        ok = mbar_wait(q_full, qn & 1, abort_flag, kErrTimeoutFull) &&
-             mbar_wait(&k_full[gb & 1], (gb >> 1) & 1, abort_flag, kErrTimeoutFull);
+        ok = warp_wait(q_full, qn & 1, lead, abort_flag, kErrTimeoutFull) &&
+             warp_wait(&k_full[gb & 1], (gb >> 1) & 1, lead, abort_flag, kErrTimeoutFull);
         if (!ok) break;
         ++qn;
         // S(0) of this segment queues behind the previous segment's last PV on the tensor core
         tc_fence_after();
         issue_s(0, gb);
         issue_s(1, gb);
-        umma_commit(&k_empty[gb & 1]);
-        if (nb == 1) umma_commit(q_empty);
+        umma_commit(&k_empty[gb & 1], lead);
+        if (nb == 1) umma_commit(q_empty, lead);
         // Per tile: PV_x(j) as soon as P_x(j) is written, then S_x(j+1) into the same columns (the
         // tensor core runs this thread's MMAs in issue order, so PV_x(j) has read P_x(j) first).
         // The two tiles are serviced alternately: one tile's softmax overlaps the other's MMAs.
@@ -410,23 +410,23 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int st = G & 1;
           const uint32_t ph = (G >> 1) & 1;
           const uint32_t jp = G & 1;
-          if (!mbar_wait(&v_full[st], ph, abort_flag, kErrTimeoutFull)) { ok = false; break; }
+          if (!warp_wait(&v_full[st], ph, lead, abort_flag, kErrTimeoutFull)) { ok = false; break; }
           const bool more = j + 1 < nb;
           const int st1 = (G + 1) & 1;
           for (int x = 0; x < 2; ++x) {
-            if (!mbar_wait(&p_full[x], jp, abort_flag, kErrTimeoutFull)) { ok = false; break; }
+            if (!warp_wait(&p_full[x], jp, lead, abort_flag, kErrTimeoutFull)) { ok = false; break; }
             tc_fence_after();
             issue_pv(x, G, j == 0);
-            if (x == 1) umma_commit(&v_empty[st]);
+            if (x == 1) umma_commit(&v_empty[st], lead);
             if (more) {
-              if (x == 0 && !mbar_wait(&k_full[st1], ((G + 1) >> 1) & 1, abort_flag, kErrTimeoutFull)) {
+              if (x == 0 && !warp_wait(&k_full[st1], ((G + 1) >> 1) & 1, lead, abort_flag, kErrTimeoutFull)) {
                 ok = false;
                 break;
               }
               issue_s(x, G + 1);
               if (x == 1) {
-                umma_commit(&k_empty[st1]);
-                if (j + 2 == nb) umma_commit(q_empty);
+                umma_commit(&k_empty[st1], lead);
+                if (j + 2 == nb) umma_commit(q_empty, lead);
               }
             }
           }
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok) {
         // every MMA this thread issued completes before the CTA frees tensor memory
-        umma_commit(drain);
+        umma_commit(drain, lead);
         const unsigned long long t0 = globaltimer();
         while (!mbar_test(smem_u32(drain), 0)) {
           if (globaltimer() - t0 > kWaitTimeoutNs) {
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int j = 0; j < nb; ++j) {
         const int G = gb + j;
         const uint32_t jp = G & 1;
-        if (ok && !warp_wait(&s_full[x], jp, abort_flag, kErrTimeoutFull)) ok = false;
+        if (ok && !lanes_wait(&s_full[x], jp, abort_flag, kErrTimeoutFull)) ok = false;
         if (!ok) {
           pair_sync();
           continue;
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         l = l * alpha + ((rsp[0].x + rsp[0].y) + (rsp[1].x + rsp[1].y));
         if (rescale) {
           // O holds sum_{i<j} P_i V_i relative to the old max: wait for PV(j-1), then scale in place
-          if (!warp_wait(&o_done[x], jp ^ 1, abort_flag, kErrTimeoutAcc)) {
+          if (!lanes_wait(&o_done[x], jp ^ 1, abort_flag, kErrTimeoutAcc)) {
             ok = false;
             continue;
           }
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       pair_sync();
       const float l_row = l + red_l[(x * 2 + (hf ^ 1)) * 128 + row];
       // the finished O (this half's 64 columns) once the last PV has landed
-      if (!ok || !warp_wait(&o_done[x], (gb - 1) & 1, abort_flag, kErrTimeoutAcc)) {
+      if (!ok || !lanes_wait(&o_done[x], (gb - 1) & 1, abort_flag, kErrTimeoutAcc)) {
         ok = false;
         continue;
       }

@@ -113,83 +113,6 @@ __device__ __forceinline__ int stat_row(int r) { return (r >> 3) * 256 + (r & 7)
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
-// The products' operands. A shared-memory matrix descriptor is a low word, which holds the address, and a
-// high word that only the layout sets; every step of a product is the low word plus a constant.
-__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) {
-  return static_cast<uint32_t>(sdesc_sw128(saddr, lbo_bytes, 1024));
-}
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024, version 1, 128-byte swizzle
-
-// As umma_f16 and umma_f16_ts, for a whole warp: every lane comes here with the same operands and the
-// elected one (lead) issues. The warp's control flow stays uniform, so operands can live in uniform
-// registers and a product costs few issue slots - the sub-partition shares them with busy math warps.
-__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc,
-                                        uint32_t lead, uint32_t hi = kDescHi) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
-      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}\n" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc,
-                                        uint32_t lead) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}\n" ::"r"(d),
-      "r"(a_tmem), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
-      "r"(lead)
-      : "memory");
-}
-
-// A warp's bounded wait. One lane polls: the barrier takes the lanes of a poll one by one, and 32 of them
-// cost 130 to 300 cycles even where the phase had long been complete. The warp agrees on the outcome.
-__device__ __forceinline__ uint32_t mbar_test_lead(uint32_t bar, uint32_t parity, uint32_t lead) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 e, %3, 0;\n\tsetp.ne.b32 p, %3, %3;\n\t"
-      "@e mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(lead)
-      : "memory");
-  return ok;
-}
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t lead, volatile int* abort_flag,
-                                          unsigned err) {
-  const uint32_t a = smem_u32(bar);
-  bool done = __any_sync(0xffffffffu, mbar_test_lead(a, parity, lead));
-  if (!done) {
-    const unsigned long long t0 = globaltimer();
-    for (;;) {
-      // the clock and the flag are looked at once in 64 polls: they would double the time of each
-#pragma unroll 1
-      for (int i = 0; i < 64 && !done; ++i) done = __any_sync(0xffffffffu, mbar_test_lead(a, parity, lead));
-      if (done) break;
-      const bool late = globaltimer() - t0 > kWaitTimeoutNs;
-      if (__any_sync(0xffffffffu, late || *abort_flag)) {
-        if (late) {
-          flag_error(err);
-          *abort_flag = 1;
-        }
-        return false;
-      }
-    }
-  }
-  __syncwarp();  // what the polling lane has seen complete, all have
-  return true;
-}
-
 // The statistics' tiles: rows of 8 in 256 bytes, the second 8 columns 128 bytes on, no swizzle.
 constexpr uint32_t kStatHi = (256u >> 4) | (1u << 14);
 __device__ __forceinline__ uint32_t stat_lo(uint32_t saddr) { return (saddr >> 4) | ((128u >> 4) << 16); }
@@ -333,8 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   // the same for all lanes, and known to be
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kProducerWarp = MATH_WARPS, kMmaWarp = MATH_WARPS + 1;
-  uint32_t lead;  // one lane of the warp: it polls and issues
-  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}\n" : "=r"(lead));
+  const uint32_t lead = elect_lead();
   const Work w = work_of(p);
   const int y0_stages = w.kv ? KV_Y0_STAGES : Y0_STAGES;
 
@@ -466,13 +388,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
         dims_product(t_s, x0, y0);
         add_statistic(t_s, 0, 0);
-        commit(bar.s_full, lead);
+        umma_commit(bar.s_full, lead);
         ok = full(&bar.y1_full[0], 0);
       }
       if (ok) {
         dims_product(t_dp, x1, y1);
         add_statistic(t_dp, 1, 0);
-        commit(bar.dp_full, lead);
+        umma_commit(bar.dp_full, lead);
       }
       if (w.kv) {
         int s = 0;  // stage of block i (both rings have two)
@@ -484,22 +406,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!(ok = full(bar.p_full, i & 1))) break;
           tc_fence_after();
           rows_product(t_acc, t_s, y1 + s * kPlace, i == 0);  // dV
-          commit(&bar.y1_empty[s], lead);
+          umma_commit(&bar.y1_empty[s], lead);
           if (more) {
             if (!(ok = full(&bar.y0_full[s1], ph1))) break;
             dims_product(t_s, x0, y0 + s1 * kPlace);
             add_statistic(t_s, 0, s1);
-            commit(bar.s_full, lead);
+            umma_commit(bar.s_full, lead);
           }
           if (!(ok = full(bar.ds_full, i & 1))) break;
           tc_fence_after();
           rows_product(t_acc2, t_dp, y0 + s * kPlace, i == 0);  // dK
-          commit(&bar.y0_empty[s], lead);
+          umma_commit(&bar.y0_empty[s], lead);
           if (more) {
             if (!(ok = full(&bar.y1_full[s1], ph1))) break;
             dims_product(t_dp, x1, y1 + s1 * kPlace);
             add_statistic(t_dp, 1, s1);
-            commit(bar.dp_full, lead);
+            umma_commit(bar.dp_full, lead);
           }
           s = s1;
           ph = ph1;
@@ -507,32 +429,32 @@ __global__ void __launch_bounds__(THREADS, 1)
       } else {
         int r0 = 0, n0 = 1;  // ring places of K: block i, block i + 1
         uint32_t pn0 = 0;    // the phase of the latter
-        if (ok) commit(&bar.y1_empty[0], lead);
+        if (ok) umma_commit(&bar.y1_empty[0], lead);
         for (int i = 0; ok && i < w.n; ++i) {
           if (i + 1 < w.n) {
             const int s1 = (i + 1) & 1;
             if (!(ok = full(bar.s_free, i & 1) && full(&bar.y0_full[n0], pn0))) break;
             tc_fence_after();
             dims_product(t_s, x0, y0 + n0 * kPlace);
-            commit(bar.s_full, lead);
+            umma_commit(bar.s_full, lead);
             if (++n0 == Y0_STAGES) n0 = 0, pn0 ^= 1;
             if (!(ok = full(&bar.y1_full[s1], ((i + 1) >> 1) & 1))) break;
             dims_product(s1 ? t_dp1 : t_dp, x1, y1 + s1 * kPlace);
-            commit(&bar.dp_full[s1], lead);
-            commit(&bar.y1_empty[s1], lead);
+            umma_commit(&bar.dp_full[s1], lead);
+            umma_commit(&bar.y1_empty[s1], lead);
           }
           if (!(ok = full(bar.ds_full, i & 1))) break;
           tc_fence_after();
           rows_product(t_acc, i & 1 ? t_dp1 : t_dp, y0 + r0 * kPlace, i == 0);  // dQ
-          commit(&bar.y0_empty[r0], lead);
+          umma_commit(&bar.y0_empty[r0], lead);
           if (++r0 == Y0_STAGES) r0 = 0;
         }
       }
       if (ok) {
-        commit(bar.acc_done, lead);
+        umma_commit(bar.acc_done, lead);
       } else {
         // every product this thread issued completes before the block frees tensor memory
-        commit(bar.drain, lead);
+        umma_commit(bar.drain, lead);
         const unsigned long long t0 = globaltimer();
         while (!mbar_test(smem_u32(bar.drain), 0)) {
           if (globaltimer() - t0 > kWaitTimeoutNs) {

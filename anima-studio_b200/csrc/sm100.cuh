@@ -353,6 +353,92 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool b
          | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// ------------------------------------------------------------------ whole-warp issue and waits
+
+// One lane of the warp (all lanes must be here): it polls and issues.
+__device__ __forceinline__ uint32_t elect_lead() {
+  uint32_t lead;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}\n" : "=r"(lead));
+  return lead;
+}
+
+// The products' operands. A shared-memory matrix descriptor is a low word, which holds the address, and a
+// high word that only the layout sets; every step of a product is the low word plus a constant.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) {
+  return static_cast<uint32_t>(sdesc_sw128(saddr, lbo_bytes, 1024));
+}
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024, version 1, 128-byte swizzle
+
+// As umma_f16 and umma_f16_ts, for a whole warp: every lane comes here with the same operands and the
+// elected one (lead) issues. The warp's control flow stays uniform, so operands can live in uniform
+// registers and a product costs few issue slots - the sub-partition shares them with busy math warps.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc,
+                                        uint32_t lead, uint32_t hi = kDescHi) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc,
+                                        uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
+// A warp's bounded wait. One lane polls: the barrier takes the lanes of a poll one by one, and 32 of them
+// cost 130 to 300 cycles even where the phase had long been complete. The warp agrees on the outcome.
+__device__ __forceinline__ uint32_t mbar_test_lead(uint32_t bar, uint32_t parity, uint32_t lead) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 e, %3, 0;\n\tsetp.ne.b32 p, %3, %3;\n\t"
+      "@e mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(lead)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t lead, volatile int* abort_flag,
+                                          unsigned err) {
+  const uint32_t a = smem_u32(bar);
+  bool done = __any_sync(0xffffffffu, mbar_test_lead(a, parity, lead));
+  if (!done) {
+    const unsigned long long t0 = globaltimer();
+    for (;;) {
+      // the clock and the flag are looked at once in 64 polls: they would double the time of each
+#pragma unroll 1
+      for (int i = 0; i < 64 && !done; ++i) done = __any_sync(0xffffffffu, mbar_test_lead(a, parity, lead));
+      if (done) break;
+      const bool late = globaltimer() - t0 > kWaitTimeoutNs;
+      if (__any_sync(0xffffffffu, late || *abort_flag)) {
+        if (late) {
+          flag_error(err);
+          *abort_flag = 1;
+        }
+        return false;
+      }
+    }
+  }
+  __syncwarp();  // what the polling lane has seen complete, all have
+  return true;
+}
+
 __device__ __forceinline__ bool elect_lane0() { return (threadIdx.x & 31) == 0; }
 
 // ------------------------------------------------------------------ small math
