@@ -33,6 +33,12 @@
 // the bound |dS| <= 2 max|dO_i| max|V_j| of the k/v head, so that gradients of any size keep their
 // digits. bf16 has fp32's range and needs neither.
 //
+// delta taken from the rounded output is off by up to half a step of sum |dO O|, next to nothing beside dS's
+// own rounding in a row of many keys, but not in one of few (a causal sequence's first rows, which have its
+// largest gradients; short prompts). Where all keys of a query block lie in one key block - the first block
+// of a causal sequence, all of them up to 128 keys - its q units therefore go first, in a launch of their
+// own, take delta = sum_j P_ij dP_ij from the tile and leave it to the k/v units.
+//
 // Masks: a query row that sees no key has lse = -inf, P = 0 and no gradient. Keys past key_len get
 // dK = dV = 0 whatever they hold: P and dS are selected, not multiplied, to 0, and a q unit clears
 // their rows of K in shared memory (0 x NaN is not 0).
@@ -79,13 +85,15 @@ struct Params {
   const int* key_len;
   float scale, scale_log2;
   const float* nlse2;   // [B][H][Lqp] -lse log2(e) (fp16: + 14), -inf for rows without a key
-  const float* ndelta;  // [B][H][Lqp] -delta
-  const uint8_t* stat;  // [B][H][nqb][lse | delta][STAT_TILE] nlse2 / scale_log2 and ndelta in 16-bit parts
+  float* ndelta;        // [B][H][Lqp] -delta
+  uint8_t* stat;  // [B][H][nqb][lse | delta][STAT_TILE] nlse2 / scale_log2 and ndelta in 16-bit parts
   const unsigned* top;  // fp16: [kv_batch][Hk][2] largest |dO_i|^2 and |V_j|^2, as bits
   void *dq, *dk, *dv;
   long long lddq, lddk, lddv, dq_bs, dk_bs, dv_bs;
   int grad_dtype;
   int kv_units, q_units, nkb, nqb, kv_splits, q_splits;
+  int q_first;  // the first q unit of this launch
+  int single;   // this launch has only q units of a single key block, which compute delta themselves
   float* kv_part;  // [split][unit][dv | dk][D / 4][128] float4, where kv_splits > 1
   float* q_part;   // [split][unit][D / 4][128] float4
 };
@@ -112,6 +120,19 @@ __device__ __forceinline__ int stat_row(int r) { return (r >> 3) * 256 + (r & 7)
 // third of its issue slots.
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
+
+// v as the sum of three 16-bit values (-inf and NaN: the first alone), packed for the first three columns.
+template <bool BF16>
+__device__ __forceinline__ uint2 three_parts(float v) {
+  float part[3];
+  float rest = v;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    part[i] = BF16 ? __bfloat162float(__float2bfloat16_rn(rest)) : __half2float(__float2half_rn(rest));
+    rest = fabsf(part[i]) < INFINITY ? rest - part[i] : 0.f;
+  }
+  return make_uint2(pack2<BF16>(part[0], part[1]), pack2<BF16>(part[2], 0.f));
+}
 
 // The statistics' tiles: rows of 8 in 256 bytes, the second 8 columns 128 bytes on, no swizzle.
 constexpr uint32_t kStatHi = (256u >> 4) | (1u << 14);
@@ -157,6 +178,7 @@ __device__ __forceinline__ Work work_of(const Params& p) {
     id -= kv_ctas;
     w.unit = id / p.q_splits;
     w.split = id - w.unit * p.q_splits;
+    w.unit += p.q_first;
     const int heads = p.B * p.H;
     const int bh = p.causal ? w.unit % heads : w.unit / p.nqb;
     w.blk = p.causal ? p.nqb - 1 - w.unit / heads : w.unit % p.nqb;
@@ -554,13 +576,19 @@ __global__ void __launch_bounds__(THREADS, 1)
       } else {
         const int kb = w.lo + i;
         const size_t at = (static_cast<size_t>(w.b) * p.H + w.h) * p.Lqp + static_cast<size_t>(w.blk) * TILE + row;
-        const f2 nlse2 = dup2(p.nlse2[at]), ndelta = dup2(p.ndelta[at]);
+        const f2 nlse2 = dup2(p.nlse2[at]);
+        f2 ndelta = dup2(p.ndelta[at]);
         // lanes are queries: the row's visible keys of this block end at `end`
         const int left = kv_len - kb * TILE;
         const bool masked = left < TILE || (p.causal && kb == w.blk);
         const int end = p.causal && kb == w.blk ? min(left, row + 1) : left;
         const uint32_t ts = t_s + lane_addr + 32 * qt, td = (i & 1 ? t_dp1 : t_dp) + lane_addr + 32 * qt;
-        if (!(ok = warp_wait(bar.s_full, i & 1, lead, abort_flag, kErrTimeoutFull))) break;
+        // (one iteration in a launch of single blocks, and every math warp meets its barrier once)
+        auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(MATH_WARPS * 32) : "memory"); };
+        if (!(ok = warp_wait(bar.s_full, i & 1, lead, abort_flag, kErrTimeoutFull))) {
+          if (p.single) meet();
+          break;
+        }
         tc_fence_after();
         auto probabilities = [&](const uint32_t(&r)[32]) {
 #pragma unroll
@@ -581,7 +609,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           probabilities(r);
           settle(pr);
         }
-        if (!(ok = warp_wait(&bar.dp_full[i & 1], (i >> 1) & 1, lead, abort_flag, kErrTimeoutFull))) break;
+        if (!(ok = warp_wait(&bar.dp_full[i & 1], (i >> 1) & 1, lead, abort_flag, kErrTimeoutFull))) {
+          if (p.single) meet();
+          break;
+        }
         tc_fence_after();
         auto gradients = [&](auto mask, const uint32_t(&r)[32]) {
           uint32_t pk[16];
@@ -603,6 +634,26 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint32_t r[32];
           tmem_ld32(td, r);
           tmem_ld_wait(r);
+          if (p.single) {
+            float d = 0.f;
+#pragma unroll
+            for (int t = 0; t < 32; ++t)
+              if (32 * qt + t < end) d = fmaf(pr[t], __uint_as_float(r[t]), d);
+            float* red = reinterpret_cast<float*>(smem + OFF_Y0 + 2 * TILE_BYTES);  // a place no load goes to
+            red[qt * TILE + row] = d;
+            meet();
+            d = (red[row] + red[TILE + row]) + (red[2 * TILE + row] + red[3 * TILE + row]);
+            if (!BF16) d *= exp2f(-kP16Shift);
+            ndelta = dup2(-d);
+            if (qt == 0) {
+              p.ndelta[at] = -d;
+              float v = -d;
+              if (!BF16) v /= delta_unit(ds_exponent(p.top, (p.kv_batch > 1 ? w.b : 0) * (p.H / p.group) + w.h / p.group));
+              const uint2 parts = three_parts<BF16>(v);
+              *reinterpret_cast<uint4*>(p.stat + (((static_cast<size_t>(w.b) * p.H + w.h) * p.nqb + w.blk) * 2 + 1) * STAT_TILE +
+                                        stat_row(row)) = make_uint4(parts.x, parts.y, 0u, 0u);
+            }
+          }
           if (masked) gradients(Yes{}, r); else gradients(No{}, r);
         }
         if (left < TILE && p.key_len) {
@@ -687,19 +738,6 @@ struct PrepParams {
   const unsigned* top;
 };
 
-// v as the sum of three 16-bit values (-inf and NaN: the first alone), packed for the first three columns.
-template <bool BF16>
-__device__ __forceinline__ uint2 three_parts(float v) {
-  float part[3];
-  float rest = v;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    part[i] = BF16 ? __bfloat162float(__float2bfloat16_rn(rest)) : __half2float(__float2half_rn(rest));
-    rest = fabsf(part[i]) < INFINITY ? rest - part[i] : 0.f;
-  }
-  return make_uint2(pack2<BF16>(part[0], part[1]), pack2<BF16>(part[2], 0.f));
-}
-
 constexpr int kPrepRows = 2;  // (row, head) pairs of a thread, their loads in flight together
 
 template <bool BF16, int HD>
@@ -763,39 +801,54 @@ __global__ void __launch_bounds__(256) attention_grad_prep_kernel(const PrepPara
   }
 }
 
-// fp16: the largest |dO_i|^2 and |V_j|^2 of each k/v head, over all queries and the keys that count; a
-// warp a row and head. Rows [0, v_rows) of a block's share are V's, the others dO's.
+// fp16: the largest |dO_i|^2 and |V_j|^2 of each k/v head, over all queries and the keys that count. Block
+// row y: a k/v head's V, then a q head's dO; D / 8 threads a row, 16 bytes each, every thread four rows
+// whose loads are in flight together.
 struct TopParams {
   const __half *v, *dout;
   long long ldv, v_bs, lddo, do_bs;
-  int H, group, D, Lq, Lk, kv_batch;
+  int H, group, Lq, Lk, kv_batch;
   const int* key_len;
   unsigned* top;
 };
+constexpr int kTopRows = 4;
+template <int HD>
 __global__ void __launch_bounds__(256) attention_grad_top_kernel(const TopParams p) {
-  const int b = blockIdx.z, lane = threadIdx.x & 31;
-  const int Hk = p.H / p.group;
-  const bool is_v = blockIdx.y < Hk;  // else q head blockIdx.y - Hk
+  constexpr int TPR = HD / 8, ROWS = 256 / TPR;
+  const int b = blockIdx.z, Hk = p.H / p.group;
+  const bool is_v = blockIdx.y < Hk;
   const int h = is_v ? blockIdx.y : blockIdx.y - Hk;
   if (is_v && b >= p.kv_batch) return;
   const int kvb = p.kv_batch > 1 ? b : 0;
   const int len = is_v ? (p.key_len ? min(p.Lk, p.key_len[kvb]) : p.Lk) : p.Lq;
-  const __half* base = (is_v ? p.v + b * p.v_bs : p.dout + b * p.do_bs) + static_cast<long long>(h) * p.D;
+  const __half* base = (is_v ? p.v + b * p.v_bs : p.dout + b * p.do_bs) + h * HD + 8 * (threadIdx.x % TPR);
   const long long ld = is_v ? p.ldv : p.lddo;
+  const int row0 = blockIdx.x * (ROWS * kTopRows) + threadIdx.x / TPR;
+  uint4 w[kTopRows];
+#pragma unroll
+  for (int u = 0; u < kTopRows; ++u) {
+    const int j = row0 + u * ROWS;
+    w[u] = j < len ? *reinterpret_cast<const uint4*>(base + j * ld) : make_uint4(0u, 0u, 0u, 0u);
+  }
   float best = 0.f;
-  for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < len; j += gridDim.x * 8) {
-    const __half2* r = reinterpret_cast<const __half2*>(base + j * ld);
+#pragma unroll
+  for (int u = 0; u < kTopRows; ++u) {
+    const uint32_t q[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
     float n = 0.f;
-    for (int c = lane; c < p.D / 2; c += 32) {
-      const float2 x = __half22float2(r[c]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&q[c]));
       n = fmaf(x.x, x.x, fmaf(x.y, x.y, n));
     }
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) n += __shfl_xor_sync(0xffffffffu, n, s);
+    for (int s = TPR / 2; s > 0; s >>= 1) n += __shfl_xor_sync(0xffffffffu, n, s);
     best = fmaxf(best, n);
   }
+#pragma unroll
+  for (int s = 16; s >= TPR; s >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, s));
   // (bits of values that are not negative are ordered as the values; a maximum hangs on no order)
-  if (lane == 0 && best > 0.f) atomicMax(p.top + 2 * (kvb * Hk + (is_v ? h : h / p.group)) + (is_v ? 1 : 0), __float_as_uint(best));
+  if (threadIdx.x % 32 == 0 && best > 0.f)
+    atomicMax(p.top + 2 * (kvb * Hk + (is_v ? h : h / p.group)) + (is_v ? 1 : 0), __float_as_uint(best));
 }
 
 // The gradients of split units: the splits' partial sums added in order. A thread has four columns of
@@ -933,14 +986,14 @@ int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, c
     tp.do_bs = pp.do_bs;
     tp.H = a->heads;
     tp.group = pl.group;
-    tp.D = HD;
     tp.Lq = a->Lq;
     tp.Lk = a->Lk;
     tp.kv_batch = pl.kv_batch;
     tp.key_len = a->key_len;
     tp.top = const_cast<unsigned*>(pp.top);
-    const int rows = ((a->Lq > a->Lk ? a->Lq : a->Lk) + 31) / 32;
-    attention_grad_top_kernel<<<dim3(rows < 64 ? rows : 64, Hk + a->heads, a->batch), 256, 0, ctx->stream>>>(tp);
+    constexpr int kRows = kTopRows * 256 / (HD / 8);  // of a block
+    const int blocks = ((a->Lq > a->Lk ? a->Lq : a->Lk) + kRows - 1) / kRows;
+    attention_grad_top_kernel<HD><<<dim3(blocks, Hk + a->heads, a->batch), 256, 0, ctx->stream>>>(tp);
     const int st = check_launch("attention_grad_top_kernel");
     if (st) return st;
   }
@@ -951,12 +1004,26 @@ int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, c
   const auto fn = attention_grad_kernel<BF16, HD>;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), SMEM_BYTES);
   if (st) return st;
-  const long long ctas = static_cast<long long>(pl.kv_units) * pl.kv_splits + static_cast<long long>(pl.q_units) * pl.q_splits;
+  int q_units = pl.q_units;
+  if (a->causal || a->Lk <= TILE) {
+    // (in a causal problem the first query blocks are the last units)
+    Params p1 = p;
+    p1.kv_units = 0;
+    p1.q_splits = 1;
+    p1.single = 1;
+    const int n = a->causal ? a->batch * a->heads : q_units;
+    q_units -= n;
+    p1.q_first = q_units;
+    fn<<<n, THREADS, SMEM_BYTES, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], p1);
+    st = check_launch("attention_grad_kernel (single blocks)");
+    if (st) return st;
+  }
+  const long long ctas = static_cast<long long>(pl.kv_units) * pl.kv_splits + static_cast<long long>(q_units) * pl.q_splits;
   ANIMA_REQUIRE(ctas < (1LL << 31), "anima_attention_backward: problem too large");
   fn<<<static_cast<unsigned>(ctas), THREADS, SMEM_BYTES, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], p);
   st = check_launch("attention_grad_kernel");
-  if (st || (pl.kv_splits == 1 && pl.q_splits == 1)) return st;
-  const int tiles = (pl.kv_splits > 1 ? pl.kv_units * 2 : 0) + (pl.q_splits > 1 ? pl.q_units : 0);
+  const int tiles = (pl.kv_splits > 1 ? pl.kv_units * 2 : 0) + (pl.q_splits > 1 ? q_units : 0);
+  if (st || tiles == 0) return st;
   attention_grad_join_kernel<HD><<<dim3(tiles, HD / 4), TILE, 0, ctx->stream>>>(p);
   return check_launch("attention_grad_join_kernel");
 }
