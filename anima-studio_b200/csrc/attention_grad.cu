@@ -141,7 +141,12 @@ __device__ __forceinline__ uint32_t stat_lo(uint32_t saddr) { return (saddr >> 4
 struct Bars {
   uint64_t *x_full, *y0_full, *y1_full, *y0_empty, *y1_empty, *s_full, *s_free, *dp_full, *p_full, *ds_full, *acc_done, *drain;
 };
-constexpr int kBars = 1 + 3 + 2 + 3 + 2 + 1 + 1 + 2 + 1 + 1 + 1 + 1;
+// (ds_full is two barriers, used in turn: a q unit's dP(i + 1) is on its way before dS(i) is waited for, so
+// the math warps can finish dS(i + 1) before the issuing warp has looked at dS(i), and on a single barrier
+// it would then see the next phase of the same parity and wait for good. A k/v unit gives out dP(i + 1)
+// after dS(i) only, and S(i + 1) after P(i), so one p_full and one s_full, dp_full and s_free cannot be
+// passed by.)
+constexpr int kBars = 1 + 3 + 2 + 3 + 2 + 1 + 1 + 2 + 1 + 2 + 1 + 1;
 
 // What a block does: a k/v unit or a q unit, and its range of iterations.
 struct Work {
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
   const Bars bar{bars,      bars + 1,  bars + 4,  bars + 6,  bars + 9,  bars + 11,
-                 bars + 12, bars + 13, bars + 15, bars + 16, bars + 17, bars + 18};
+                 bars + 12, bars + 13, bars + 15, bars + 16, bars + 18, bars + 19};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // the same for all lanes, and known to be
@@ -284,7 +289,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const bool math = bars + i == bar.s_free || bars + i == bar.p_full || bars + i == bar.ds_full;
+      const bool math = bars + i == bar.s_free || bars + i == bar.p_full || bars + i == bar.ds_full ||
+                        bars + i == bar.ds_full + 1;
       mbar_init(bars + i, math ? MATH_WARPS : 1);
     }
     *abort_flag = 0;
@@ -435,7 +441,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             add_statistic(t_s, 0, s1);
             umma_commit(bar.s_full, lead);
           }
-          if (!(ok = full(bar.ds_full, i & 1))) break;
+          if (!(ok = full(&bar.ds_full[i & 1], (i >> 1) & 1))) break;
           tc_fence_after();
           rows_product(t_acc2, t_dp, y0 + s * kPlace, i == 0);  // dK
           umma_commit(&bar.y0_empty[s], lead);
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma_commit(&bar.dp_full[s1], lead);
             umma_commit(&bar.y1_empty[s1], lead);
           }
-          if (!(ok = full(bar.ds_full, i & 1))) break;
+          if (!(ok = full(&bar.ds_full[i & 1], (i >> 1) & 1))) break;
           tc_fence_after();
           rows_product(t_acc, i & 1 ? t_dp1 : t_dp, y0 + r0 * kPlace, i == 0);  // dQ
           umma_commit(&bar.y0_empty[r0], lead);
@@ -572,7 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        arrive_one_lane(bar.ds_full);
+        arrive_one_lane(&bar.ds_full[i & 1]);
       } else {
         const int kb = w.lo + i;
         const size_t at = (static_cast<size_t>(w.b) * p.H + w.h) * p.Lqp + static_cast<size_t>(w.blk) * TILE + row;
@@ -669,7 +675,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        arrive_one_lane(bar.ds_full);
+        arrive_one_lane(&bar.ds_full[i & 1]);
       }
     }
     if (ok && w.n > 0) ok = warp_wait(bar.acc_done, 0, lead, abort_flag, kErrTimeoutAcc);

@@ -24,6 +24,13 @@ def ops():
     return pkg("ops")
 
 
+@pytest.fixture(autouse=True)
+def no_device_error():
+    """No wait of a kernel ran out."""
+    yield
+    pkg("device").Context.get(0).sync()
+
+
 def randn(seed, *shape, dtype=FP, scale=1.0):
     g = torch.Generator(device=DEV).manual_seed(seed)
     return (torch.randn(shape, generator=g, device=DEV) * scale).to(dtype)
@@ -342,3 +349,32 @@ def test_library_refusals(ops):
     out, lse = ops.attention_lse(c.q, c.k, c.v, **c.kw)
     with pytest.raises(err, match="aligned"):
         ops.attention_backward(c.do, c.q, c.k, c.v, out, lse, dq=odd, **c.kw)
+
+
+@pytest.mark.parametrize("B,H,Lq,Lk,lens,causal", [(2, 16, 4096, 512, (512, 325), False), (1, 16, 1024, 1024, None, False),
+                                                    (1, 16, 1500, 1500, None, True)])
+def test_many_passes(ops, B, H, Lq, Lk, lens, causal):
+    """400 passes back to back: the same bits each time, and no wait runs out. (A q unit's dP runs a block
+    ahead of its dS: a barrier that the math warps can pass twice before the issuing warp looks at it
+    would stop a block once in some hundred thousand.)"""
+    c = Case(B, H, 1, 128, Lq, Lk, BF, causal=causal, lens=lens)
+    want = c.run(ops)
+    for i in range(400):
+        got = c.run(ops)
+        if i % 100 == 99:
+            for n in want:
+                assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("Lq,Lk,causal", [(300, 5, False), (70, 128, False), (3, 3, True), (200, 200, True)])
+def test_rows_of_few_keys_keep_their_digits(ops, dtype, D, Lq, Lk, causal):
+    """Where a query block's keys lie in one key block, delta comes from the probabilities: against the
+    64-bit gradients the error is that of rounding dS and the result once each (twice half a step, in
+    the 2-norm), where a delta of the rounded output would add the rounding of sum |dO O|."""
+    c = Case(1, 4, 2, D, Lq, Lk, dtype, causal=causal)
+    got, (val, _) = c.run(ops), c.reference()
+    rows = min(Lq, 128) if causal else Lq
+    g, r = got["dq"][:, :, :rows].double(), val["dq"][:, :, :rows]
+    assert ((g - r).norm() / r.norm()).item() <= 2 * half_step(dtype)

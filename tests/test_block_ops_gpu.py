@@ -20,6 +20,13 @@ def ops():
     return pkg("ops")
 
 
+@pytest.fixture(autouse=True)
+def no_device_error():
+    """No wait of a kernel ran out."""
+    yield
+    pkg("device").Context.get(0).sync()
+
+
 def randn(seed, *shape, dtype=torch.float32, scale=1.0, shift=0.0):
     g = torch.Generator(device=DEV).manual_seed(seed)
     return (torch.randn(shape, generator=g, device=DEV) * scale + shift).to(dtype)
