@@ -1057,8 +1057,9 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratc
   const int kv_batch = kv_bcast ? 1 : a->batch;
   ANIMA_REQUIRE(a->ldo >= static_cast<long long>(a->heads) * a->head_dim && a->ldo % 8 == 0,
                 "anima_attention: bad output stride");
-  ANIMA_REQUIRE(reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && (a->batch == 1 || a->o_bstride % 8 == 0),
-                "anima_attention: the output has to be 16-byte aligned, its batch stride a multiple of 8");
+  ANIMA_REQUIRE(reinterpret_cast<uintptr_t>(a->out) % 16 == 0 &&
+                    (a->batch == 1 || a->o_bstride * (a->out_dtype == ANIMA_F32 ? 4 : 2) % 16 == 0),
+                "anima_attention: the output and its batch stride have to be 16-byte aligned");
 
   // 3D maps (cols, rows, batch) over each operand; the box is 64 columns x 128 rows.
   CUtensorMap tq, tk, tv;

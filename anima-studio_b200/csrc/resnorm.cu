@@ -864,7 +864,7 @@ int count_sums(const anima_residual_norm_args* a) {
 }
 
 int check(const char* fn, const anima_residual_norm_args* a, bool grad) {
-  ANIMA_REQUIRE(a->rows >= 0 && a->cols > 0 && a->cols <= kMaxCols, "%s: %d rows of %d columns (at most %d)", fn,
+  ANIMA_REQUIRE(a->rows >= 0 && a->rows <= 1 << 30 && a->cols > 0 && a->cols <= kMaxCols, "%s: %d rows of %d columns (at most 2^30 of %d)", fn,
                 a->rows, a->cols, kMaxCols);
   ANIMA_REQUIRE(a->rows_per_item > 0 && a->rows % a->rows_per_item == 0, "%s: %d rows are not items of %d rows", fn,
                 a->rows, a->rows_per_item);

@@ -293,7 +293,7 @@ extern "C" int anima_rotary(anima_ctx* ctx, const anima_rotary_args* a) {
   ANIMA_ON_DEVICE(ctx);
   ANIMA_REQUIRE(a->dtype == ANIMA_F32 || a->dtype == ANIMA_BF16 || a->dtype == ANIMA_F16, "anima_rotary: dtype %d",
                 a->dtype);
-  ANIMA_REQUIRE(a->rows >= 0 && a->Hq >= 0 && a->Hk >= 0 && a->Hq + a->Hk > 0 && a->Hq <= 1024 && a->Hk <= 1024,
+  ANIMA_REQUIRE(a->rows >= 0 && a->rows <= 1 << 30 && a->Hq >= 0 && a->Hk >= 0 && a->Hq + a->Hk > 0 && a->Hq <= 1024 && a->Hk <= 1024,
                 "anima_rotary: %d rows, %d and %d heads", a->rows, a->Hq, a->Hk);
   ANIMA_REQUIRE(a->D > 0 && a->D <= 65536 && a->R >= 2 && a->R % 2 == 0 && a->R <= a->D && a->R / 2 <= rotary::kAngles,
                 "anima_rotary: %d rotated of %d dims (an even number, at most the head and %d)", a->R, a->D,

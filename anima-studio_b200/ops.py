@@ -183,7 +183,8 @@ def rotary_freqs(dim: int, theta: float = 10000.0, *, scaling: str | None = None
       "yarn"    pairs that turn more than beta_fast times within original_len stay, those below
                 beta_slow turns are divided by factor, a linear ramp over the turns between; outputs
                 multiplied by 0.1 ln(factor) + 1.
-    No reference counterpart: its RoPE is a table of fixed theta (common.js:26-52)."""
+    Made on the host: once, not inside a stream capture. No reference counterpart: its RoPE is a table of
+    fixed theta (common.js:26-52)."""
     if dim < 2 or dim % 2 or not theta > 0 or not factor > 0:
         raise dev.AnimaError(1, f"rotary_freqs: dim {dim} (even, at least 2), theta {theta}, factor {factor}")
     if scaling not in (None, "linear", "ntk", "yarn"):
@@ -538,6 +539,8 @@ def _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, b
         raise dev.AnimaError(1, f"{fn}: batch {batch}, {Lq} queries, {Lk} keys, {H} heads in groups of {group}")
     if D not in (64, 128):
         raise dev.AnimaError(1, f"{fn}: head_dim {D} (64 or 128)")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise dev.AnimaError(1, f"{fn}: scale {scale}")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise dev.AnimaError(1, f"{fn}: q, k and v are bf16 or fp16, not {q.dtype}")
     C, Ck, dt, at = H * D, H // group * D, q.dtype, q.get_device()
@@ -656,7 +659,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     dev.check(ctx.lib.anima_attention_backward_workspace(ctx.h, C.byref(g), C.byref(need)))
     ws = torch.empty(need.value, dtype=torch.uint8, device=device)
     g.workspace, g.workspace_bytes = ws.data_ptr(), need.value
-    ctx.call("anima_attention_backward", C.byref(g), tag=name, work=10.0 * batch * Lq * Lk * D * H, kernels=2)
+    ctx.call("anima_attention_backward", C.byref(g), tag=name, work=10.0 * batch * Lq * Lk * D * H,
+             kernels=2 + (q.dtype is torch.float16) + (bool(causal) or Lk <= 128))  # (and the join of split units)
     return dq, dk, dv
 
 

@@ -141,6 +141,16 @@ def test_causal_shared_heads(ops, dtype, D, Lq, Lk):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("causal,group,lens", [(True, 1, None), (True, 2, (1500,)), (False, 2, (1201,)), (True, 2, (130,))])
+def test_few_units_are_split_along_their_walk(ops, dtype, D, causal, group, lens):
+    """Two heads of 1500 tokens do not fill the SMs: the units are split and their parts joined, some of
+    them without a block (a causal unit's first keys, keys past key_len)."""
+    c = Case(1, 2, group, D, 1500, 1500, dtype, causal=causal, lens=lens)
+    check(c.run(ops), *c.reference())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [128, 64])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("Lq,Lk,lens", [(200, 333, (333, 129, 1, 0)), (130, 256, (128, 256, 500, -3)), (64, 700, (1, 640, 699, 513))])
 def test_key_lengths(ops, dtype, D, causal, Lq, Lk, lens):

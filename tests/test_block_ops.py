@@ -132,7 +132,8 @@ ATTN_BAD = [
     dict(Lq=0), dict(Lk=0), dict(H=3, group=2), dict(H=0), dict(batch=0), dict(D=96), dict(q=t(20, 128)),
     dict(k=t(24, 64, dtype=torch.float16)), dict(q=t(19, 128, dtype=torch.bfloat16)), dict(k=t(23, 64, dtype=torch.bfloat16)),
     dict(ldq=64), dict(ldk=32), dict(q_off=-8), dict(q_off=8), dict(v_off=64), dict(k_bstride=0), dict(v_bstride=-64),
-    dict(q_bstride=11 * 128), dict(key_len=t(2)), dict(key_len=t(1, dtype=torch.int32)),
+    dict(q_bstride=11 * 128), dict(key_len=t(2)), dict(key_len=t(1, dtype=torch.int32)), dict(scale=-1.0), dict(scale=0.0),
+    dict(scale=float("nan")),
 ]
 
 
