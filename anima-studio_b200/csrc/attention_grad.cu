@@ -28,6 +28,11 @@
 // Tensor memory, k/v unit: S^T [0,128) dP^T [128,256) dV [256,256+D) dK [256+D,256+2D);
 // q unit: S [0,128), dP [128,256) and [384,512), dQ [256,256+D).
 //
+// Bound by the tensor core and the card's power: 4096 x 4096, 16 heads of 128 in bf16 takes 372 us, 925 TFLOP/s
+// of the gradients' 10 Lq Lk D H and 1290 of the 14 that are executed (cuBLAS: 1646 for milliseconds, 1405
+// for seconds); 8192 x 8192 causal with 8 k/v heads 735 us, 4096 x 4096 of 64 dims 287 us (there the
+// exponentials bound it).
+//
 // Roundings. P and dS round to the operands' type before their products (fp32 sums). In fp16 both are
 // moved into its range by powers of two that are undone in fp32: P <= 1 by 2^14; dS by a factor from
 // the bound |dS| <= 2 max|dO_i| max|V_j| of the k/v head, so that gradients of any size keep their

@@ -10,9 +10,10 @@
 //
 // Bound by HBM: each element is read and written once. A thread owns two 16-byte vectors that hold
 // whole pairs (half layout: dims e.. and R/2 + e..; interleaved: 2 adjacent vectors) of one row, in four
-// heads, and issues its eight loads first. Meanwhile the block's threads share the angles of its rows: one
-// sine and cosine each where every thread computing its own 8 would take ten times the instructions
-// (8192 rows of 32 heads of 128 in fp16: 34.3 us so, 24.7 with the angles shared; a copy takes 20.5).
+// heads, and issues its eight loads first. Meanwhile the block's threads share the angles of its rows, one
+// sine and cosine each. 8192 rows of 32 heads of 128 in fp16 take 24.1 us (a device copy 24.8): 34 with
+// 16-bit values converted one by one, which the conversion unit does at a quarter of the rate, 38 to 51
+// with fewer heads a thread; 16381 rows of 24 heads in fp32 take 66 us.
 
 #include "internal.h"
 #include "sm100.cuh"
