@@ -284,7 +284,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t armed = 0;
       auto arm = [&](int i, uint32_t ph) { armed = (armed & ~(3u << (2 * i))) | ((2u | ph) << (2 * i)); };
       int gb = 0, qn = 0, tails = 0;        // key blocks, Q loads and cleared V blocks so far
-      for (int si = 0; si < nseg && !*abort_flag; ++si) {
+      auto aborted = [&]() {
+        const bool a = *abort_flag != 0;
+        return TRAIN ? __any_sync(0xffffffffu, a) != 0 : a;
+      };
+      for (int si = 0; si < nseg && !aborted(); ++si) {
         const int4 sg = segs[si];  // unit, kb0, kb1, kind
         const int qp = sg.x % p.q_pairs, bh = sg.x / p.q_pairs;
         const int h = bh % p.heads, b = bh / p.heads;

@@ -491,9 +491,12 @@ struct Ring {
   uint64_t* full;  // [places]
   volatile int* abort_flag;
   uint32_t row_bytes;
+  uint32_t armed;  // of the fetching thread: bit k place k was used, bit 8 + k the phase of its last row
 
   // One thread: row r to its place (what was there has been read).
-  __device__ __forceinline__ void fetch(int k, size_t r) const {
+  __device__ __forceinline__ void fetch(int k, size_t r) {
+    if (armed >> k & 1u) armed ^= 256u << k;
+    armed |= 1u << k;
     mbar_arrive_expect_tx(&full[k], row_bytes);
     uint8_t* d = smem + k * row_bytes;
 #pragma unroll
@@ -503,7 +506,21 @@ struct Ring {
       d += in[i].bytes;
     }
   }
-  // After a wait that ran out nothing is computed any more, but every thread still meets every barrier.
+  // The fetching thread, before the block ends: after a wait that ran out, copies may be in flight.
+  __device__ __forceinline__ void drain() const {
+    if (!*abort_flag) return;
+    for (int k = 0; k < kMaxPlaces; ++k) {
+      if (!(armed >> k & 1u)) continue;
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_test(smem_u32(&full[k]), armed >> (8 + k) & 1u)) {
+        if (globaltimer() - t0 > kWaitTimeoutNs) {
+          flag_error(kErrTimeoutDrain);
+          break;
+        }
+      }
+    }
+  }
+  // After a wait that ran out nothing is stored any more, but every thread still meets every barrier.
   __device__ __forceinline__ bool wait(int k, uint32_t phase) const {
     return mbar_wait(&full[k], phase, abort_flag, kErrTimeoutFull);
   }
@@ -522,6 +539,7 @@ __device__ __forceinline__ Ring<N> make_ring(const Stream (&in)[N], uint8_t* sme
   r.smem = smem;
   r.full = full;
   r.abort_flag = abort_flag;
+  r.armed = 0;
   if (threadIdx.x == 0) {
     for (int k = 0; k < places; ++k) mbar_init(&full[k], 1);
     *abort_flag = 0;
@@ -604,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, NV == 1 ? 3 : 2) residual_norm_full_
   const Stream in[2] = {{p.x, p.ldx * size_of(p.dtx), p.C * size_of(p.dtx)},
                         {p.y, p.ldy * size_of(p.dty), p.C * size_of(p.dty)}};
   const int places = p.places;
-  const auto ring = make_ring<2>(in, ring_smem, full, &abort_flag, places);
+  auto ring = make_ring<2>(in, ring_smem, full, &abort_flag, places);
   if (threadIdx.x == 0)
     for (int k = 0; k < places; ++k)
       if (w.first + k < w.last) ring.fetch(k, w.row0 + w.first + k);
@@ -659,6 +677,7 @@ __global__ void __launch_bounds__(kThreads, NV == 1 ? 3 : 2) residual_norm_full_
       if (live) store<8>(p.o1, p.dth, r * p.ldo1 + c0 + k * step, x[k]);
     }
   }
+  if (threadIdx.x == 0) ring.drain();
 }
 
 // The backward there. A row's statistics and the sums of the pre-norm's gradient come from one round.
@@ -677,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 2) residual_norm_grad_full_kernel(co
                         {p.y, p.ldy * size_of(p.dty), p.C * size_of(p.dty)},
                         {p.dx, p.lddx * size_of(p.dtx), p.dx ? p.C * size_of(p.dtx) : 0u}};
   const int places = p.places;
-  const auto ring = make_ring<4>(in, ring_smem, full, &abort_flag, places);
+  auto ring = make_ring<4>(in, ring_smem, full, &abort_flag, places);
   const uint32_t off_h = in[0].bytes, off_y = off_h + in[1].bytes, off_d = off_y + in[2].bytes;
   if (threadIdx.x == 0)
     for (int k = 0; k < places; ++k)
@@ -777,6 +796,7 @@ __global__ void __launch_bounds__(kThreads, 2) residual_norm_grad_full_kernel(co
       }
     }
   }
+  if (threadIdx.x == 0) ring.drain();
   if (!p.sums) return;
   float* out = p.part + static_cast<size_t>(blockIdx.x) * p.sums * p.C + c0;
   auto put = [&](int where, const float(&v)[NV][8]) {
