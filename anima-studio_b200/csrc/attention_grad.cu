@@ -28,10 +28,10 @@
 // Tensor memory, k/v unit: S^T [0,128) dP^T [128,256) dV [256,256+D) dK [256+D,256+2D);
 // q unit: S [0,128), dP [128,256) and [384,512), dQ [256,256+D).
 //
-// Bound by the tensor core and the card's power: 4096 x 4096, 16 heads of 128 in bf16 takes 372 us, 925 TFLOP/s
-// of the gradients' 10 Lq Lk D H and 1290 of the 14 that are executed (cuBLAS: 1646 for milliseconds, 1405
-// for seconds); 8192 x 8192 causal with 8 k/v heads 735 us, 4096 x 4096 of 64 dims 287 us (there the
-// exponentials bound it).
+// Bound by the tensor core and the card's power: 4096 x 4096, 16 heads of 128 in bf16 takes 357 to 371 us (two
+// cards), 926 to 962 TFLOP/s of the gradients' 10 Lq Lk D H and 1297 to 1347 of the 14 that are executed
+// (cuBLAS: 1646 for milliseconds, 1405 for seconds); 8192 x 8192 causal with 8 k/v heads 707 to 730 us,
+// 4096 x 4096 of 64 dims 273 to 282 us (there the exponentials bound it).
 //
 // Roundings. P and dS round to the operands' type before their products (fp32 sums). In fp16 both are
 // moved into its range by powers of two that are undone in fp32: P <= 1 by 2^14; dS by a factor from
@@ -85,6 +85,7 @@ constexpr float kLse16 = 128.0f;    // fp16: lse enters the product as 128 x (it
 struct Params {
   int B, H, group, Lq, Lk, Lqp;  // Lqp: Lq rounded up to whole tiles
   int kv_batch;                  // 1 where the items share one K/V
+  int Hk, kv_heads, walk_heads;  // k/v heads; of all K/V items; (item, q head) pairs that share one
   int q_col, k_col, v_col;
   int causal;
   const int* key_len;
@@ -170,23 +171,26 @@ __device__ __forceinline__ Work work_of(const Params& p) {
   w.kv = id < kv_ctas;
   int total;
   if (w.kv) {
-    w.unit = id / p.kv_splits;
+    w.unit = p.kv_splits == 1 ? id : id / p.kv_splits;
     w.split = id - w.unit * p.kv_splits;
-    const int heads = p.kv_units / p.nkb;  // (K/V item, k/v head) pairs
+    const int heads = p.kv_heads;
     // causal: early key blocks are seen by most queries, so they go first; else head by head
     const int bh = p.causal ? w.unit % heads : w.unit / p.nkb;
     w.blk = p.causal ? w.unit / heads : w.unit % p.nkb;
-    const int Hk = p.H / p.group;
-    w.b = bh / Hk;
-    w.h = bh - w.b * Hk;
+    w.b = bh / p.Hk;
+    w.h = bh - w.b * p.Hk;
     const int q0 = p.causal ? w.blk : 0;
     w.per_head = w.blk * TILE < keys_of(p, w.b) ? max(0, p.nqb - q0) : 0;
-    total = w.per_head * p.group * (p.B / p.kv_batch);
-    w.lo = static_cast<int>(static_cast<long long>(total) * w.split / p.kv_splits);
-    w.n = static_cast<int>(static_cast<long long>(total) * (w.split + 1) / p.kv_splits) - w.lo;
+    total = w.per_head * p.walk_heads;
+    w.lo = 0;
+    w.n = total;
+    if (p.kv_splits > 1) {
+      w.lo = static_cast<int>(static_cast<long long>(total) * w.split / p.kv_splits);
+      w.n = static_cast<int>(static_cast<long long>(total) * (w.split + 1) / p.kv_splits) - w.lo;
+    }
   } else {
     id -= kv_ctas;
-    w.unit = id / p.q_splits;
+    w.unit = p.q_splits == 1 ? id : id / p.q_splits;
     w.split = id - w.unit * p.q_splits;
     w.unit += p.q_first;
     const int heads = p.B * p.H;
@@ -196,8 +200,12 @@ __device__ __forceinline__ Work work_of(const Params& p) {
     w.h = bh - w.b * p.H;
     total = (keys_of(p, p.kv_batch > 1 ? w.b : 0) + TILE - 1) / TILE;
     if (p.causal) total = min(total, w.blk + 1);
-    w.lo = total * w.split / p.q_splits;
-    w.n = total * (w.split + 1) / p.q_splits - w.lo;
+    w.lo = 0;
+    w.n = total;
+    if (p.q_splits > 1) {
+      w.lo = total * w.split / p.q_splits;
+      w.n = total * (w.split + 1) / p.q_splits - w.lo;
+    }
     w.per_head = 0;
   }
   return w;
@@ -217,25 +225,12 @@ __device__ __forceinline__ void kv_iteration(const Params& p, const Work& w, int
 // overwrites what another still reads: k-step k (16 of the 128 inner indices, 8 columns) of the A operand.
 __device__ __forceinline__ uint32_t quarter_cols(int k) { return (k >> 1) * 32 + (k & 1) * 8; }
 
-// N neighbouring columns of a gradient's row.
+// N neighbouring columns of an fp32 gradient's row.
 template <int N>
-__device__ __forceinline__ void put(void* out, int dtype, size_t at, const float (&v)[N]) {
-  if (dtype == ANIMA_F32) {
-    float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+__device__ __forceinline__ void put(void* out, size_t at, const float (&v)[N]) {
+  float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
 #pragma unroll
-    for (int t = 0; t < N / 4; ++t) d[t] = make_float4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
-  } else {
-    uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
-    const bool bf = dtype == ANIMA_BF16;
-#pragma unroll
-    for (int t = 0; t < N / 8; ++t) {
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = bf ? pack2<true>(v[8 * t + 2 * e], v[8 * t + 2 * e + 1]) : pack2<false>(v[8 * t + 2 * e], v[8 * t + 2 * e + 1]);
-      d[t] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
+  for (int t = 0; t < N / 4; ++t) d[t] = make_float4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
 }
 
 // 2^x of a pair on the FMA and integer pipes: x = n + f, |f| <= 1/2, by adding 1.5 2^23 (whose sum has n
@@ -275,7 +270,8 @@ template <bool BF16, int HD>
 __global__ void __launch_bounds__(THREADS, 1)
     attention_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                           const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                          const Params p) {
+                          const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ CUtensorMap tm_dk,
+                          const __grid_constant__ CUtensorMap tm_dv, const Params p) {
   constexpr int ATOMS = HD / 64;
   constexpr int BYTES = ATOMS * ATOM;
   extern __shared__ uint8_t smem_raw[];
@@ -292,14 +288,59 @@ __global__ void __launch_bounds__(THREADS, 1)
   const Work w = work_of(p);
   const int y0_stages = w.kv ? KV_Y0_STAGES : Y0_STAGES;
 
-  if (threadIdx.x == 0) {
+  // The loading thread also sets up the barriers and starts the first loads, so that they are on their way
+  // while the others get ready: that took 3900 cycles beside the 7000 that a q unit of four blocks works.
+  const int kvb = p.kv_batch > 1 ? w.b : 0;
+  const int hk = w.kv ? w.h : w.h / p.group;
+  auto load = [&](int off, const CUtensorMap* tm, uint64_t* fb, int col, int row, int item) {
+#pragma unroll
+    for (int t = 0; t < ATOMS; ++t) tma_load_3d(smem + off + t * ATOM, tm, fb, col + 64 * t, row, item);
+  };
+  auto load_y0 = [&](int i, int place, int b, int h, int qb) {
+    uint64_t* fb = &bar.y0_full[place];
+    if (w.kv) {
+      // the statistics come and go with Q: its place is freed last
+      mbar_arrive_expect_tx(fb, BYTES + 2 * STAT_TILE);
+      load(OFF_Y0 + place * TILE_BYTES, &tm_q, fb, p.q_col + h * HD, qb * TILE, b);
+      bulk_load_1d(smem + OFF_STAT + place * 2 * STAT_TILE,
+                   p.stat + ((static_cast<size_t>(b) * p.H + h) * p.nqb + qb) * (2 * STAT_TILE), 2 * STAT_TILE, fb);
+    } else {
+      mbar_arrive_expect_tx(fb, BYTES);
+      load(OFF_Y0 + place * TILE_BYTES, &tm_k, fb, p.k_col + hk * HD, (w.lo + i) * TILE, kvb);
+    }
+  };
+  auto load_y1 = [&](int i, int place, int b, int h, int qb) {
+    uint64_t* fb = &bar.y1_full[place];
+    mbar_arrive_expect_tx(fb, BYTES);
+    if (w.kv) {
+      load(OFF_Y1 + place * TILE_BYTES, &tm_do, fb, h * HD, qb * TILE, b);
+    } else {
+      load(OFF_Y1 + place * TILE_BYTES, &tm_v, fb, p.v_col + hk * HD, (w.lo + i) * TILE, kvb);
+    }
+  };
+  if (warp == kProducerWarp && lane == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const bool math = bars + i == bar.s_free || bars + i == bar.p_full || bars + i == bar.ds_full ||
-                        bars + i == bar.ds_full + 1;
+      const bool math = i == 12 || (i >= 15 && i <= 17);  // s_free, p_full, ds_full
       mbar_init(bars + i, math ? MATH_WARPS : 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
+    fence_proxy_async_smem();
+    if (w.n > 0) {
+      int b = 0, h = 0, qb = 0;
+      if (w.kv) kv_iteration(p, w, 0, b, h, qb);
+      mbar_arrive_expect_tx(bar.x_full, 2 * BYTES);
+      if (w.kv) {
+        load(OFF_X, &tm_k, bar.x_full, p.k_col + hk * HD, w.blk * TILE, kvb);
+        load_y0(0, 0, b, h, qb);
+        load(OFF_X + TILE_BYTES, &tm_v, bar.x_full, p.v_col + hk * HD, w.blk * TILE, kvb);
+      } else {
+        load(OFF_X, &tm_q, bar.x_full, p.q_col + w.h * HD, w.blk * TILE, w.b);
+        load_y0(0, 0, b, h, qb);
+        load(OFF_X + TILE_BYTES, &tm_do, bar.x_full, w.h * HD, w.blk * TILE, w.b);
+      }
+      load_y1(0, 0, b, h, qb);
+    }
   }
   if (w.kv && threadIdx.x < 2 * TILE) {  // the constant columns: 1 (or fp16's unit) three times, then zeros
     const int which = threadIdx.x / TILE;
@@ -322,50 +363,19 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == kProducerWarp) {
     if (lane == 0 && w.n > 0) {
-      // what is in flight: for each full barrier, armed and the parity of its last arm
-      uint32_t armed = 0;
+      // what is in flight: for each full barrier (x, y0[3], y1[2]), armed and the parity of its last arm
+      uint32_t armed = 2u | 2u << 2 | 2u << 8;
       auto arm = [&](int i, uint32_t ph) { armed = (armed & ~(3u << (2 * i))) | ((2u | ph) << (2 * i)); };
-      auto load = [&](int off, const CUtensorMap* tm, uint64_t* fb, int col, int row, int item) {
-#pragma unroll
-        for (int t = 0; t < ATOMS; ++t) tma_load_3d(smem + off + t * ATOM, tm, fb, col + 64 * t, row, item);
-      };
-      const int kvb = p.kv_batch > 1 ? w.b : 0;
-      const int hk = w.kv ? w.h : w.h / p.group;
-      const int kc = p.k_col + hk * HD, vc = p.v_col + hk * HD;
-      mbar_arrive_expect_tx(bar.x_full, 2 * BYTES);
-      if (w.kv) {
-        load(OFF_X, &tm_k, bar.x_full, kc, w.blk * TILE, kvb);
-        load(OFF_X + TILE_BYTES, &tm_v, bar.x_full, vc, w.blk * TILE, kvb);
-      } else {
-        load(OFF_X, &tm_q, bar.x_full, p.q_col + w.h * HD, w.blk * TILE, w.b);
-        load(OFF_X + TILE_BYTES, &tm_do, bar.x_full, w.h * HD, w.blk * TILE, w.b);
-      }
-      arm(0, 0);
-      int s0 = 0, s1 = 0;
+      int s0 = 1, s1 = 1;  // block 0 is on its way
       uint32_t ph0 = 0, ph1 = 0;
-      for (int i = 0; i < w.n; ++i) {
+      for (int i = 1; i < w.n; ++i) {
         int b = 0, h = 0, qb = 0;
         if (w.kv) kv_iteration(p, w, i, b, h, qb);
-        const size_t stat = ((static_cast<size_t>(b) * p.H + h) * p.nqb + qb) * (2 * STAT_TILE);
         if (!mbar_wait(&bar.y0_empty[s0], ph0 ^ 1, abort_flag, kErrTimeoutEmpty)) break;
-        if (w.kv) {
-          // the statistics come and go with Q: its place is freed last
-          mbar_arrive_expect_tx(&bar.y0_full[s0], BYTES + 2 * STAT_TILE);
-          load(OFF_Y0 + s0 * TILE_BYTES, &tm_q, &bar.y0_full[s0], p.q_col + h * HD, qb * TILE, b);
-          bulk_load_1d(smem + OFF_STAT + s0 * 2 * STAT_TILE, p.stat + stat, 2 * STAT_TILE, &bar.y0_full[s0]);
-        } else {
-          mbar_arrive_expect_tx(&bar.y0_full[s0], BYTES);
-          load(OFF_Y0 + s0 * TILE_BYTES, &tm_k, &bar.y0_full[s0], kc, (w.lo + i) * TILE, kvb);
-        }
+        load_y0(i, s0, b, h, qb);
         arm(1 + s0, ph0);
         if (!mbar_wait(&bar.y1_empty[s1], ph1 ^ 1, abort_flag, kErrTimeoutEmpty)) break;
-        if (w.kv) {
-          mbar_arrive_expect_tx(&bar.y1_full[s1], BYTES);
-          load(OFF_Y1 + s1 * TILE_BYTES, &tm_do, &bar.y1_full[s1], h * HD, qb * TILE, b);
-        } else {
-          mbar_arrive_expect_tx(&bar.y1_full[s1], BYTES);
-          load(OFF_Y1 + s1 * TILE_BYTES, &tm_v, &bar.y1_full[s1], vc, (w.lo + i) * TILE, kvb);
-        }
+        load_y1(i, s1, b, h, qb);
         arm(4 + s1, ph1);
         if (++s0 == y0_stages) s0 = 0, ph0 ^= 1;
         if (++s1 == Y1_STAGES) s1 = 0, ph1 ^= 1;
@@ -713,14 +723,32 @@ __global__ void __launch_bounds__(THREADS, 1)
           float4* d = reinterpret_cast<float4*>(w.kv ? p.kv_part : p.q_part) + (slot * (HD / 4) + c0 / 4) * TILE + row;
 #pragma unroll
           for (int t = 0; t < NC / 4; ++t) d[t * TILE] = make_float4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
+        } else if (p.grad_dtype != ANIMA_F32) {
+          // a warp's 32 x NC piece through shared memory (the unit's own tiles are done with) to a TMA store,
+          // which leaves out the rows behind the last: stored from registers, 16 bytes of 32 rows at a time,
+          // a tile took 3500 cycles
+          uint8_t* piece = smem + OFF_X + (a * MATH_WARPS + warp) * (32 * NC * 2);
+          uint4* d = reinterpret_cast<uint4*>(piece + lane * NC * 2);
+#pragma unroll
+          for (int t = 0; t < NC / 8; ++t)
+            d[t] = make_uint4(pack2<BF16>(v[8 * t], v[8 * t + 1]), pack2<BF16>(v[8 * t + 2], v[8 * t + 3]),
+                              pack2<BF16>(v[8 * t + 4], v[8 * t + 5]), pack2<BF16>(v[8 * t + 6], v[8 * t + 7]));
+          fence_proxy_async_smem();
+          __syncwarp();
+          const int r0 = w.blk * TILE + quad * 32;
+          if (lead && r0 < (w.kv ? p.Lk : p.Lq)) {
+            tma_store_3d(w.kv ? (a ? &tm_dk : &tm_dv) : &tm_dq, piece, w.h * HD + c0, r0, w.b);
+            bulk_commit();
+          }
         } else if (w.kv) {
           if (r < p.Lk)
-            put<NC>(a ? p.dk : p.dv, p.grad_dtype,
+            put<NC>(a ? p.dk : p.dv,
                     (a ? w.b * p.dk_bs + r * p.lddk : w.b * p.dv_bs + r * p.lddv) + static_cast<size_t>(w.h) * HD + c0, v);
         } else if (r < p.Lq) {
-          put<NC>(p.dq, p.grad_dtype, w.b * p.dq_bs + r * p.lddq + static_cast<size_t>(w.h) * HD + c0, v);
+          put<NC>(p.dq, w.b * p.dq_bs + r * p.lddq + static_cast<size_t>(w.h) * HD + c0, v);
         }
       }
+      if (lead) bulk_wait_all();  // shared memory stays until the stores have read it, and they are done
     }
   }
   tc_fence_before();
@@ -978,7 +1006,7 @@ int check(const char* fn, const anima_attention_grad_args* g) {
 
 template <bool BF16, int HD>
 int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, const Params& p, const PrepParams& pp,
-           const CUtensorMap (&tm)[4]) {
+           const CUtensorMap (&tm)[7]) {
   const anima_attention_args* a = &g->fwd;
   const long long pairs = static_cast<long long>(pl.Lqp) * a->heads;
   ANIMA_REQUIRE(pairs < (1LL << 31) && a->batch <= 65535, "anima_attention_backward: problem too large");
@@ -1025,13 +1053,13 @@ int launch(anima_ctx* ctx, const anima_attention_grad_args* g, const Plan& pl, c
     const int n = a->causal ? a->batch * a->heads : q_units;
     q_units -= n;
     p1.q_first = q_units;
-    fn<<<n, THREADS, SMEM_BYTES, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], p1);
+    fn<<<n, THREADS, SMEM_BYTES, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], tm[6], p1);
     st = check_launch("attention_grad_kernel (single blocks)");
     if (st) return st;
   }
   const long long ctas = static_cast<long long>(pl.kv_units) * pl.kv_splits + static_cast<long long>(q_units) * pl.q_splits;
   ANIMA_REQUIRE(ctas < (1LL << 31), "anima_attention_backward: problem too large");
-  fn<<<static_cast<unsigned>(ctas), THREADS, SMEM_BYTES, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], p);
+  fn<<<static_cast<unsigned>(ctas), THREADS, SMEM_BYTES, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], tm[6], p);
   st = check_launch("attention_grad_kernel");
   const int tiles = (pl.kv_splits > 1 ? pl.kv_units * 2 : 0) + (pl.q_splits > 1 ? q_units : 0);
   if (st || tiles == 0) return st;
@@ -1096,7 +1124,7 @@ extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_gr
   ANIMA_REQUIRE(g->workspace && g->workspace_bytes >= pl.bytes && reinterpret_cast<uintptr_t>(g->workspace) % 256 == 0,
                 "anima_attention_backward: a workspace of %zu bytes (256-byte aligned) is needed, %zu are given", pl.bytes,
                 g->workspace ? g->workspace_bytes : 0);
-  CUtensorMap tm[4];
+  CUtensorMap tm[7] = {};
   const CUtensorMapDataType dt =
       a->dtype == ANIMA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint32_t box[3] = {64, anima::attn::TILE, 1};
@@ -1115,6 +1143,23 @@ extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_gr
     st = make_tmap(&tm[i], dt, 3, m.p, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (st) return st;
   }
+  if (g->grad_dtype != ANIMA_F32) {  // dq, dk, dv: a warp's piece of a tile
+    const uint32_t piece[3] = {static_cast<uint32_t>(a->head_dim) / 4, 32, 1};
+    const struct {
+      const void* p;
+      long long ld, bs, cols;
+      int L, batch;
+    } outs[3] = {{g->dq, g->lddq, g->dq_bstride, cq, a->Lq, a->batch},
+                 {g->dk, g->lddk, g->dk_bstride, ck, a->Lk, pl.kv_batch},
+                 {g->dv, g->lddv, g->dv_bstride, ck, a->Lk, pl.kv_batch}};
+    for (int i = 0; i < 3; ++i) {
+      const auto& m = outs[i];
+      const uint64_t dims[3] = {static_cast<uint64_t>(m.cols), static_cast<uint64_t>(m.L), static_cast<uint64_t>(m.batch)};
+      const uint64_t str[2] = {static_cast<uint64_t>(m.ld) * 2, static_cast<uint64_t>(m.batch > 1 ? m.bs : m.ld * m.L) * 2};
+      st = make_tmap(&tm[4 + i], dt, 3, m.p, dims, str, piece, CU_TENSOR_MAP_SWIZZLE_NONE);
+      if (st) return st;
+    }
+  }
   unsigned char* ws = static_cast<unsigned char*>(g->workspace);
   const float scale = a->scale > 0.f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim));
   Params p{};
@@ -1125,6 +1170,9 @@ extern "C" int anima_attention_backward(anima_ctx* ctx, const anima_attention_gr
   p.Lk = a->Lk;
   p.Lqp = pl.Lqp;
   p.kv_batch = pl.kv_batch;
+  p.Hk = a->heads / pl.group;
+  p.kv_heads = pl.kv_batch * p.Hk;
+  p.walk_heads = pl.group * (a->batch / pl.kv_batch);
   p.q_col = a->q_off;
   p.k_col = a->k_off;
   p.v_col = a->v_off;
