@@ -388,3 +388,21 @@ def test_rows_of_few_keys_keep_their_digits(ops, dtype, D, Lq, Lk, causal):
     rows = min(Lq, 128) if causal else Lq
     g, r = got["dq"][:, :, :rows].double(), val["dq"][:, :, :rows]
     assert ((g - r).norm() / r.norm()).item() <= 2 * half_step(dtype)
+
+
+@pytest.mark.parametrize("grad_dtype", [BF, FP])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("Lq,Lk,causal", [(1, 33, False), (161, 95, False), (223, 223, True)])
+def test_rows_behind_the_last_stay(ops, D, Lq, Lk, causal, grad_dtype):
+    """Items of odd lengths lie end to end: a tile's rows past an item's end belong to the next item, or lie
+    behind the last one, and its columns beside the heads'."""
+    c = Case(3, 4, 2, D, Lq, Lk, BF, causal=causal, lens=[Lk, 0, max(1, Lk - 40)])
+    bufs = [torch.full((3 * L + 130, n * D + 8), 7.0, dtype=grad_dtype, device=DEV) for L, n in ((Lq, 4), (Lk, 2), (Lk, 2))]
+    d = [b[:, :b.shape[1] - 8] for b in bufs]
+    out, lse = ops.attention_lse(c.q, c.k, c.v, **c.kw)
+    ops.attention_backward(c.do, c.q, c.k, c.v, out, lse, dq=d[0], dk=d[1], dv=d[2], **c.kw)
+    val, tol = c.reference(grad_dtype=grad_dtype)
+    got = {n: c.heads(t[:3 * L].contiguous(), L) for n, t, L in zip(("dq", "dk", "dv"), d, (Lq, Lk, Lk))}
+    check(got, val, tol, ("dq", "dk", "dv"))
+    for b, L in zip(bufs, (Lq, Lk, Lk)):
+        assert bool((b[3 * L:] == 7).all() and (b[:, -8:] == 7).all())
