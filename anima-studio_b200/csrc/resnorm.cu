@@ -168,8 +168,10 @@ __device__ __forceinline__ void param(const float* p, size_t at, float none, flo
   }
 }
 
-// Sums of K values over the T threads of a row, to all of them. `buf` alternates between calls, so one
-// barrier a call is enough: a value is read before its thread can reach the barrier after next.
+// Sums of K values over the T threads of a row, to all of them. `buf` alternates between the calls on `red`,
+// so one barrier a call is enough: a value is read before its thread can reach the barrier after next, behind
+// which its place is written again. That needs all calls on one array to have places of one size, so
+// row_moments has an array and a `buf` of its own.
 template <int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float* red, int& buf) {
 #pragma unroll
@@ -300,7 +302,7 @@ __device__ __forceinline__ void merge_lanes(Moments& m, int lanes, float n) {
 constexpr int kRedMoments = 2 * 2 * (kThreads / 32);  // [2 buffers][warps][2 sets]
 
 // The moments of K sets, n values a thread, over the row's threads, to all of them (GRAD0: the first set
-// has a gradient). One barrier, as in row_sum.
+// has a gradient). One barrier, as in row_sum, and so K is the same in all calls on one array.
 template <int K, bool GRAD0>
 __device__ __forceinline__ void row_moments(Moments (&m)[K], float n, float4* red, int& buf) {
   auto step = [&](int lanes) {
@@ -685,9 +687,10 @@ template <int NV, bool MODS, bool WEIGHTS>
 __global__ void __launch_bounds__(kThreads, 2) residual_norm_grad_full_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t ring_smem[];
   __shared__ float4 red[kRedMoments];
+  __shared__ float red2[kRedFloats];  // of row_sum
   __shared__ uint64_t full[kMaxPlaces];
   __shared__ int abort_flag;
-  int buf = 0;
+  int buf = 0, buf2 = 0;
   const int step = blockDim.x * 8, c0 = threadIdx.x * 8;
   const Share w = share_of(p);
   const float inv_c = 1.0f / static_cast<float>(p.C);
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 2) residual_norm_grad_full_kernel(co
       if (p.post == kNone && live) store<8>(p.o1, p.dty, r * p.ldo1 + c0 + k * step, d[k]);
     }
     if (p.post != kNone) {
-      row_sum(s2, reinterpret_cast<float*>(red), buf);
+      row_sum(s2, red2, buf2);
       const float m0 = p.post == kLayer ? s2[0] * inv_c : 0.f, m1 = s2[1] * inv_c;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {

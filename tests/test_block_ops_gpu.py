@@ -397,3 +397,37 @@ def test_block_ops_captured_and_on_another_stream(ops):
     torch.cuda.synchronize()
     for a, b in zip(side, want):
         assert torch.equal(a, b)
+
+
+# Blocks of several rows: as many as the ring has places and more, so that places are filled again, phases
+# turn, column sums gather and the row sums' shared memory is used again and again. The last block of an item
+# has fewer rows than the others.
+MANY_ROWS = [(4593, 1024, 1531, "rms", "rms", torch.bfloat16, torch.bfloat16, torch.bfloat16),
+             (16382, 512, 8191, "layer", "layer", torch.float32, torch.float32, torch.float32),
+             (8191, 2048, 8191, None, "layer", torch.float32, torch.float16, torch.float16),
+             (8190, 2048, 2730, "layer", "rms", torch.float32, torch.bfloat16, torch.bfloat16),
+             (2503, 4096, 2503, "rms", "layer", torch.float32, torch.float32, torch.float32),  # a ring of two places
+             (20001, 256, 6667, "rms", "layer", torch.bfloat16, torch.bfloat16, torch.float16)]
+
+
+@pytest.mark.parametrize("rows,C,L,post,pre,xd,yd,hd", MANY_ROWS)
+def test_residual_norm_blocks_of_many_rows(ops, rows, C, L, post, pre, xd, yd, hd):
+    t, c = make_norm(rows, C, L, post, pre, True, xd, yd, hd, seed=90)
+    kw = kwargs(t, c)
+
+    def run():
+        x, h = ops.residual_norm(t["x"], t["y"], out_dtype=hd, **kw)
+        return [x, h, *(g for g in ops.residual_norm_backward(t["dh"], t["dx_out"], t["x"], t["y"], **kw) if g is not None)]
+
+    want = run()
+    rx, rh = norm_ref({n: (v.double() if v is not None else None) for n, v in t.items()}, c)
+    assert rel(want[0], rx) <= half_step(xd) + 64 * U and rel(want[1], rh) <= half_step(hd) + 64 * U
+    got = ops.residual_norm_backward(t["dh"], t["dx_out"], t["x"], t["y"], **kw)
+    check_grads(got, grad_refs(t, c), rows)
+    dx, dy = t["dx_out"].clone(), t["y"].clone()
+    here = ops.residual_norm_backward(t["dh"], dx, t["x"], dy, dx=dx, dy=dy, **kw)
+    for a, b in zip(got, here):
+        assert (a is None and b is None) or torch.equal(a, b)
+    for _ in range(200):
+        for a, b in zip(want, run()):
+            assert torch.equal(a, b)
