@@ -233,7 +233,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 class Context:
-    """One anima_ctx per CUDA device; every call is issued on torch's current stream."""
+    """One anima_ctx per CUDA device; every call is issued on torch's current stream. The device's
+    threads share it: binding the stream and the call on it are one step under its lock, and nothing
+    about the stream is remembered from one call to the next."""
 
     _per_device: dict = {}
     launches = 0  # kernels this process enqueued through the library (all devices)
@@ -247,7 +249,7 @@ class Context:
         with torch.cuda.device(device):
             check(self.lib.anima_ctx_create(device, C.byref(h)))
         self.h = h
-        self.stream = None  # the one bound last
+        self.lock = threading.RLock()
 
     @classmethod
     def get(cls, device=None) -> "Context":
@@ -265,34 +267,39 @@ class Context:
         check(self.lib.anima_ctx_set_attention_split(self.h, int(mode)))
 
     def bind_stream(self):
-        stream = _raw_stream(self.device)
-        if stream != self.stream:
-            check(self.lib.anima_ctx_set_stream(self.h, C.c_void_p(stream)))
-            self.stream = stream
+        """Bind torch's current stream; the caller holds the lock until its call is made."""
+        check(self.lib.anima_ctx_set_stream(self.h, _raw_stream(self.device)))
         return self.h
 
     def call(self, name: str, *args, tag: str | None = None, work: float = 0.0, kernels: int = 1):
         """Run entry point `name` on torch's current stream; `kernels` = library kernels it enqueues."""
-        h = self.bind_stream()
         kt = KernelTimer.active
         if kt is not None and name in kt.names:
             e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             e0.record()
-            check(getattr(self.lib, name)(h, *args))
+            with self.lock:
+                check(getattr(self.lib, name)(self.bind_stream(), *args))
             e1.record()
             kt.events.append((name, tag, e0, e1, work))
         else:
-            check(getattr(self.lib, name)(h, *args))
+            with self.lock:
+                check(getattr(self.lib, name)(self.bind_stream(), *args))
         if name in LAUNCHING:
             Context.launches += kernels
 
     def sync(self):
         """gpu.sync: wait for the stream and raise on a device-side fault or timed-out wait."""
-        check(self.lib.anima_sync(self.bind_stream()))
+        try:
+            torch.cuda.current_stream(self.device).synchronize()  # other threads launch meanwhile
+        except RuntimeError:
+            pass  # the library reports it
+        with self.lock:
+            check(self.lib.anima_sync(self.bind_stream()))
 
     def profile_report(self) -> str:
         buf = C.create_string_buffer(1 << 16)
-        check(self.lib.anima_profile_report(self.bind_stream(), buf, len(buf)))
+        with self.lock:
+            check(self.lib.anima_profile_report(self.bind_stream(), buf, len(buf)))
         return buf.value.decode()
 
 

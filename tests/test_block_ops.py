@@ -5,6 +5,7 @@ import math
 import os
 import shutil
 import subprocess
+import threading
 
 import pytest
 import torch
@@ -162,3 +163,68 @@ def test_attention_backward_refuses(ops, err, change):
     with pytest.raises(err) as e:
         ops.attention_backward(**{**kw, **change})
     assert e.value.status == 1
+
+
+# ----------------------------------------------------------------------------- the context's stream
+
+class StreamLib:
+    """A stand-in for the library: which stream each call would have run on."""
+
+    def __init__(self):
+        self.bound, self.ran, self.at_bind = None, [], None
+
+    def anima_ctx_set_stream(self, h, stream):
+        self.bound = getattr(stream, "value", stream)
+        if self.at_bind:
+            self.at_bind(self.bound)
+        return 0
+
+    def anima_zero(self, h, name):
+        self.ran.append((name, self.bound))
+        return 0
+
+
+@pytest.fixture
+def shared_context(monkeypatch):
+    dev = pkg("device")
+    ctx = dev.Context.__new__(dev.Context)
+    ctx.lib, ctx.device, ctx.h, ctx.lock = StreamLib(), 0, None, threading.RLock()
+    here = threading.local()
+    monkeypatch.setattr(dev, "_raw_stream", lambda device: here.stream)
+    return ctx, here
+
+
+def test_threads_that_share_a_context_keep_their_streams(shared_context):
+    """Another thread's call in the middle of one (between the binding of its stream and what follows)
+    moves neither that call nor the thread's later ones to the other's stream."""
+    ctx, here = shared_context
+    done = threading.Event()
+
+    def other():
+        here.stream = 22
+        ctx.call("anima_zero", "b")
+        done.set()
+
+    def in_the_middle(stream):
+        if stream == 11:
+            ctx.lib.at_bind = None
+            threading.Thread(target=other, daemon=True).start()
+            done.wait(0.5)  # as far as it gets
+
+    ctx.lib.at_bind = in_the_middle
+    here.stream = 11
+    ctx.call("anima_zero", "a")
+    assert done.wait(10)
+    for i in range(3):
+        ctx.call("anima_zero", "a")
+    assert sorted(set(ctx.lib.ran)) == [("a", 11), ("b", 22)]
+
+
+def test_a_stream_set_behind_the_context_does_not_stay(shared_context):
+    """A host that calls anima_ctx_set_stream itself: the next operator is on torch's current stream again."""
+    ctx, here = shared_context
+    here.stream = 11
+    ctx.call("anima_zero", "a")
+    ctx.lib.anima_ctx_set_stream(ctx.h, 99)
+    ctx.call("anima_zero", "a")
+    assert ctx.lib.ran == [("a", 11), ("a", 11)]

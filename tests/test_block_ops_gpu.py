@@ -3,6 +3,8 @@
 Tolerances count roundings: u = 2^-24 is half a step of fp32, and an output of type t is off by at
 most eps(t) / 2 of its value more."""
 
+import threading
+
 import pytest
 import torch
 
@@ -431,3 +433,30 @@ def test_residual_norm_blocks_of_many_rows(ops, rows, C, L, post, pre, xd, yd, h
     for _ in range(200):
         for a, b in zip(want, run()):
             assert torch.equal(a, b)
+
+
+def test_two_threads_on_streams_of_their_own(ops):
+    """Both share the device's context. Each works on inputs that its own stream has just written, so a call
+    on the other's stream would find the old ones."""
+    inv, _ = ops.rotary_freqs(128)
+    x = [randn(100 + i, 2048, 16 * 128, dtype=torch.bfloat16) for i in range(2)]
+    want = [ops.rotary(t, None, inv, Hq=16, D=128)[0] for t in x]
+    wrong, errors = [0, 0], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(200):
+                    t = torch.zeros_like(x[i])
+                    t.copy_(x[i])
+                    wrong[i] += int(not torch.equal(ops.rotary(t, None, inv, Hq=16, D=128)[0], want[i]))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and wrong == [0, 0]
