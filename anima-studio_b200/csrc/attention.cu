@@ -1024,6 +1024,16 @@ constexpr size_t callers_bytes(int sms) {
   return callers_flag_bytes(sms) + static_cast<size_t>(sms) * attn::PART_FLOATS * sizeof(float);
 }
 
+// The softmax scales that training takes (0 or less: the default). The backward pass computes lse / scale, in
+// fp16 with 2^31 as its end: log2 of 2^30 keys (less P's shift of 14) over 2^-24 log2(e) takes less than 2^28 of
+// it, the rest is q.k's.
+int check_scale(const char* fn, const anima_attention_args* a) {
+  const float least = a->dtype == ANIMA_F16 ? 0x1p-24f : 0x1p-100f;
+  ANIMA_REQUIRE(a->scale <= 0.f || (a->scale >= least && a->scale <= 0x1p64f),
+                "%s: softmax scale %g (%g to %g)", fn, a->scale, least, 0x1p64f);
+  return ANIMA_OK;
+}
+
 // lse: row statistics wanted (then head_dim 64 takes the tensor cores too, and nothing else runs).
 int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratch& scratch, float* lse) {
   const bool static_ws = scratch.static_ws;
@@ -1037,6 +1047,8 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratc
   if (lse) {
     ANIMA_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "anima_attention_lse: head_dim %d (64 or 128)", a->head_dim);
     ANIMA_REQUIRE(a->heads % group == 0, "anima_attention_lse: %d heads do not form groups of %d", a->heads, group);
+    const int st = check_scale("anima_attention_lse", a);
+    if (st) return st;
   }
   if (!lse && attention_planes_ok(a)) return attention_planes(ctx, a);  // the VAE's wide single head
   if (!lse && (a->head_dim != 128 || a->dtype == ANIMA_F32 || a->heads % group != 0)) {

@@ -24,7 +24,8 @@
 // A k/v unit's lse and delta belong to columns, the same for all lanes. Loading them costs dearly there
 // (beside products that read both operands from shared memory, 8 16-byte loads a warp took 5700 cycles
 // for 190), so the tensor core adds them: S^T and dP^T get one more step of 16 inner indices, a constant
-// column times each value's 16-bit parts (three of them: value = hi + mid + low to 2^-24 of it).
+// column times each value's 16-bit parts, three of them: in bf16 value = hi + mid + low to 2^-24 of it; in
+// fp16, whose range is short, lse / scale = 2^15 hi + 2^5 mid + low, up to 2^31 and to 2^-33 of it or 2^-25.
 // Tensor memory, k/v unit: S^T [0,128) dP^T [128,256) dV [256,256+D) dK [256+D,256+2D);
 // q unit: S [0,128), dP [128,256) and [384,512), dQ [256,256+D).
 //
@@ -80,7 +81,11 @@ constexpr int OFF_BAR = OFF_Y1 + Y1_STAGES * TILE_BYTES;
 constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
 static_assert(SMEM_BYTES <= 232448, "fits a block's shared memory");
 constexpr float kP16Shift = 14.0f;  // fp16: P is held as 2^14 P
-constexpr float kLse16 = 128.0f;    // fp16: lse enters the product as 128 x (its 128th)
+// fp16: the units of the parts that lse / scale enters the product in. The first is the largest power of two
+// that fp16 holds; what it leaves, at most 2^-11 of 2^31, is within fp16 in units of 2^5; what that leaves, at
+// most 2^9, in units of 1. (One unit of 128 for all three ended at 2^23: with softmax scales around 1e-6, or
+// q.k past 8e6, P became 0 or inf.)
+__device__ constexpr float kLse16[3] = {32768.0f, 32.0f, 1.0f};
 
 struct Params {
   int B, H, group, Lq, Lk, Lqp;  // Lqp: Lq rounded up to whole tiles
@@ -92,7 +97,7 @@ struct Params {
   float scale, scale_log2;
   const float* nlse2;   // [B][H][Lqp] -lse log2(e) (fp16: + 14), -inf for rows without a key
   float* ndelta;        // [B][H][Lqp] -delta
-  uint8_t* stat;  // [B][H][nqb][lse | delta][STAT_TILE] nlse2 / scale_log2 and ndelta in 16-bit parts
+  uint8_t* stat;        // [B][H][nqb][lse | delta][STAT_TILE] nlse2 / scale_log2 and ndelta in 16-bit parts
   const unsigned* top;  // fp16: [kv_batch][Hk][2] largest |dO_i|^2 and |V_j|^2, as bits
   void *dq, *dk, *dv;
   long long lddq, lddk, lddv, dq_bs, dk_bs, dv_bs;
@@ -127,15 +132,18 @@ __device__ __forceinline__ int stat_row(int r) { return (r >> 3) * 256 + (r & 7)
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
-// v as the sum of three 16-bit values (-inf and NaN: the first alone), packed for the first three columns.
+// v as the sum of three 16-bit values, each times its unit, a power of two (-inf and NaN: the first alone),
+// packed for the first three columns.
 template <bool BF16>
-__device__ __forceinline__ uint2 three_parts(float v) {
+__device__ __forceinline__ uint2 three_parts(float v, float u0 = 1.f, float u1 = 1.f, float u2 = 1.f) {
+  const float unit[3] = {u0, u1, u2};
   float part[3];
   float rest = v;
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    part[i] = BF16 ? __bfloat162float(__float2bfloat16_rn(rest)) : __half2float(__float2half_rn(rest));
-    rest = fabsf(part[i]) < INFINITY ? rest - part[i] : 0.f;
+    const float t = rest / unit[i];
+    part[i] = BF16 ? __bfloat162float(__float2bfloat16_rn(t)) : __half2float(__float2half_rn(t));
+    rest = fabsf(part[i]) < INFINITY ? fmaf(-unit[i], part[i], rest) : 0.f;
   }
   return make_uint2(pack2<BF16>(part[0], part[1]), pack2<BF16>(part[2], 0.f));
 }
@@ -342,12 +350,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       load_y1(0, 0, b, h, qb);
     }
   }
-  if (w.kv && threadIdx.x < 2 * TILE) {  // the constant columns: 1 (or fp16's unit) three times, then zeros
+  if (w.kv && threadIdx.x < 2 * TILE) {  // the constant columns: 1 (or fp16's units) three times, then zeros
     const int which = threadIdx.x / TILE;
     uint8_t* row = smem + OFF_ONES + which * STAT_TILE + stat_row(threadIdx.x % TILE);
-    float one = 1.f;
-    if (!BF16) one = which ? delta_unit(ds_exponent(p.top, w.b * (p.H / p.group) + w.h)) : kLse16;
-    *reinterpret_cast<uint4*>(row) = make_uint4(pack2<BF16>(one, one), pack2<BF16>(one, 0.f), 0u, 0u);
+    uint32_t first = pack2<BF16>(1.f, 1.f), third = pack2<BF16>(1.f, 0.f);
+    if (!BF16) {
+      const float d = delta_unit(ds_exponent(p.top, w.b * (p.H / p.group) + w.h));
+      first = which ? pack2<BF16>(d, d) : pack2<BF16>(kLse16[0], kLse16[1]);
+      third = pack2<BF16>(which ? d : kLse16[2], 0.f);
+    }
+    *reinterpret_cast<uint4*>(row) = make_uint4(first, third, 0u, 0u);
     *reinterpret_cast<uint4*>(row + 128) = make_uint4(0u, 0u, 0u, 0u);
     fence_proxy_async_smem();
   }
@@ -828,12 +840,15 @@ __global__ void __launch_bounds__(256) attention_grad_prep_kernel(const PrepPara
       uint8_t* tile = p.stat + ((bh * (p.Lqp / TILE) + row[u] / TILE) * 2 + which) * STAT_TILE + stat_row(row[u] % TILE) + half * 128;
       uint2 parts = make_uint2(0u, 0u);
       if (!half) {
-        float v = nl * p.inv_scale_log2 * (BF16 ? 1.f : 1.f / kLse16);
         if (which) {
-          v = -d;
+          float v = -d;
           if (!BF16) v /= delta_unit(ds_exponent(p.top, (p.kv_batch > 1 ? b : 0) * (p.H / p.group) + h[u] / p.group));
+          parts = three_parts<BF16>(v);
+        } else if (BF16) {
+          parts = three_parts<BF16>(nl * p.inv_scale_log2);
+        } else {
+          parts = three_parts<BF16>(nl * p.inv_scale_log2, kLse16[0], kLse16[1], kLse16[2]);
         }
-        parts = three_parts<BF16>(v);
       }
       *reinterpret_cast<uint4*>(tile) = make_uint4(parts.x, parts.y, 0u, 0u);
     }
@@ -999,6 +1014,8 @@ int check(const char* fn, const anima_attention_grad_args* g) {
   ANIMA_REQUIRE(a->dtype == ANIMA_BF16 || a->dtype == ANIMA_F16, "%s: q/k/v dtype must be bf16 or f16", fn);
   ANIMA_REQUIRE(a->heads % (a->group > 1 ? a->group : 1) == 0, "%s: %d heads do not form groups of %d", fn, a->heads,
                 a->group);
+  const int st = check_scale(fn, a);
+  if (st) return st;
   ANIMA_REQUIRE(a->batch == 1 || (a->k_bstride == 0 && a->v_bstride == 0) || (a->k_bstride > 0 && a->v_bstride > 0),
                 "%s: k and v batch strides must both be zero (shared) or both positive", fn);
   return ANIMA_OK;

@@ -539,10 +539,10 @@ def _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, b
         raise dev.AnimaError(1, f"{fn}: batch {batch}, {Lq} queries, {Lk} keys, {H} heads in groups of {group}")
     if D not in (64, 128):
         raise dev.AnimaError(1, f"{fn}: head_dim {D} (64 or 128)")
-    if scale is not None and not 0.0 < scale < math.inf:
-        raise dev.AnimaError(1, f"{fn}: scale {scale}")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise dev.AnimaError(1, f"{fn}: q, k and v are bf16 or fp16, not {q.dtype}")
+    if scale is not None and not (2.0 ** -24 if q.dtype is torch.float16 else 2.0 ** -100) <= scale <= 2.0 ** 64:
+        raise dev.AnimaError(1, f"{fn}: scale {scale} (2^-24 in fp16, 2^-100 in bf16, to 2^64)")
     C, Ck, dt, at = H * D, H // group * D, q.dtype, q.get_device()
     kv_items = 1 if batch > 1 and k_bstride == 0 and v_bstride == 0 else batch
     ldq, ldk, ldv = ldq or C, ldk or Ck, ldv or Ck
@@ -593,8 +593,8 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, Lq: int,
                   causal: bool = False, name: str | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """attention() for training: the same arguments (bf16 or fp16 q/k/v, D 64 or 128), and beside the
     output [batch * Lq, H D] the row statistics lse [batch, H, Lq] that attention_backward needs: ln of
-    each query's sum of exponentials, -inf (with an output of zeros) where it sees no key. k and v may
-    hold anything, NaN included, past key_len. Its workspace comes from torch's allocator, so calls on
+    each query's sum of exponentials, -inf (with an output of zeros) where it sees no key. scale: 2^-24
+    (bf16: 2^-100) to 2^64. k and v may hold anything, NaN included, past key_len. Its workspace comes from torch's allocator, so calls on
     several streams and captured graphs share nothing."""
     fn = "attention_lse"
     if out is None:

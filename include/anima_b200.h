@@ -312,7 +312,8 @@ int anima_attention_noalloc(anima_ctx* ctx, const anima_attention_args* a);
  *
  * anima_attention_lse: anima_attention that also writes lse [batch, heads, Lq] (fp32), the natural
  * logarithm of each row's sum of exponentials over its visible keys, -inf where it sees none (its output
- * row is 0). head_dim 64 or 128, bf16/fp16 q/k/v, on the tensor cores; same arguments otherwise. What
+ * row is 0). head_dim 64 or 128, bf16/fp16 q/k/v, on the tensor cores; same arguments otherwise, with a
+ * softmax scale of 2^-24 (bf16: 2^-100) to 2^64, or 0 for the default. What
  * lies in k and v behind key_len may be anything, NaN included. workspace: device memory of the caller
  * (256-byte aligned) of anima_attention_lse_workspace bytes (0 for most shapes), free again when the
  * call's work is done; nothing is shared between calls. */
@@ -328,7 +329,9 @@ int anima_attention_lse(anima_ctx* ctx, const anima_attention_args* a, float* ls
  * all. Rows of keys past key_len get zeros. dq, dk, dv: head h at columns h * head_dim from the pointer,
  * rows and items their strides apart (so slices of one q|k|v gradient will do); they must not overlap
  * the inputs. P and dS are rounded to q's type, sums are fp32; no atomics on the gradients, so the same
- * inputs give the same bits. All tensors 16-byte aligned with strides that are multiples of 8 elements.
+ * inputs give the same bits. Probabilities come from lse in fp32: |lse| above 10^4 costs them digits (2^-24
+ * |lse|), and in fp16 |q.k| has to stay below 2^30 before the scale. All tensors 16-byte aligned with
+ * strides that are multiples of 8 elements.
  * workspace: as above, of anima_attention_backward_workspace bytes. */
 typedef struct {
   anima_attention_args fwd;

@@ -5,6 +5,7 @@ half a step of the operands' type: P, dS and every output round once to that typ
 each), and delta is taken from the rounded output (h of sum |dO O|). What is in fp32 (scores, exponents,
 sums of up to a few thousand terms) stays below F = 2^-16 of the magnitudes that are summed."""
 
+import ctypes
 import math
 
 import pytest
@@ -406,3 +407,34 @@ def test_rows_behind_the_last_stay(ops, D, Lq, Lk, causal, grad_dtype):
     check(got, val, tol, ("dq", "dk", "dv"))
     for b, L in zip(bufs, (Lq, Lk, Lk)):
         assert bool((b[3 * L:] == 7).all() and (b[:, -8:] == 7).all())
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("dtype,scale,sharp", [
+    (HF, 2.0 ** -24, 1.0), (HF, 1e-7, 1.0), (HF, 1e-6, 1.0), (HF, 3e-5, 1.0), (HF, 2e-7, 700.0), (HF, 2.0 ** -24, 1500.0),
+    (BF, 2.0 ** -100, 1.0), (BF, 1e-30, 1.0), (BF, 1e-7, 700.0)])
+def test_small_scales(ops, D, dtype, scale, sharp):
+    """lse / scale, which enters a product in 16-bit parts, is up to 10^8 times the scores' differences, and
+    with large q and k as large as they are. Beside the bounds of each element, the 2-norm: P and dS round
+    once (half a step each, random), delta and out are in fp32."""
+    c = Case(2, 4, 2, D, 200, 300, dtype, lens=(300, 129), sharp=sharp)
+    c.kw["scale"] = scale
+    got = c.run(ops, dict(out_dtype=FP), dict(grad_dtype=FP))
+    val, tol = c.reference(scale=scale, out_dtype=FP, grad_dtype=FP)
+    check(got, val, tol)
+    for n in ("dq", "dk", "dv"):
+        assert ((got[n].double() - val[n]).norm() / val[n].norm()).item() < 2 * half_step(dtype), n
+
+
+def test_the_library_refuses_scales(ops):
+    dev = pkg("device")
+    c = Case(1, 2, 1, 64, 32, 32, HF)
+    ctx, need = dev.Context.get(0), ctypes.c_size_t()
+    for scale, dtype in ((math.nan, BF), (math.inf, BF), (2.0 ** -25, HF), (2.0 ** -101, BF), (2.0 ** 65, HF)):
+        g = dev.AttentionGradArgs()
+        g.fwd.batch, g.fwd.heads, g.fwd.head_dim, g.fwd.Lq, g.fwd.Lk = 1, 2, 64, 32, 32
+        g.fwd.dtype, g.fwd.scale = dev.DTYPE_CODE[dtype], scale
+        with pytest.raises(dev.AnimaError, match="scale"):
+            dev.check(ctx.lib.anima_attention_backward_workspace(ctx.h, ctypes.byref(g), ctypes.byref(need)))
+    out, lse = ops.attention_lse(c.q, c.k, c.v, **c.kw, scale=2.0 ** -24)
+    assert lse.isfinite().all()

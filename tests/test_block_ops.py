@@ -228,3 +228,17 @@ def test_a_stream_set_behind_the_context_does_not_stay(shared_context):
     ctx.lib.anima_ctx_set_stream(ctx.h, 99)
     ctx.call("anima_zero", "a")
     assert ctx.lib.ran == [("a", 11), ("a", 11)]
+
+
+# ----------------------------------------------------------------------------- ranges
+
+@pytest.mark.parametrize("dtype,scale", [(torch.float16, 2.0 ** -25), (torch.float16, 1e-9), (torch.bfloat16, 2.0 ** -101),
+                                         (torch.bfloat16, 1e-46), (torch.float16, 2.0 ** 65), (torch.bfloat16, 1e39),
+                                         (torch.bfloat16, math.inf)])
+def test_attention_refuses_scales_out_of_range(ops, err, dtype, scale):
+    """1e-46 is 0 in the kernels' fp32, which stands for the default, and 1e39 is infinite."""
+    kw = {n: (v.to(dtype) if isinstance(v, torch.Tensor) else v) for n, v in attn_kw().items()}
+    with pytest.raises(err, match="scale"):
+        ops.attention_lse(**kw, scale=scale)
+    with pytest.raises(err, match="scale"):
+        ops.attention_backward(t(20, 128, dtype=dtype), out=t(20, 128, dtype=dtype), lse=t(2, 2, 10), **kw, scale=scale)
