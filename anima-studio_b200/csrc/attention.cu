@@ -1149,10 +1149,14 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratc
     }
     p.stream_k = 1;
     grid = ctx->num_sms;
-  } else if (p.causal && p.q_pairs >= 8 && units > ctx->num_sms) {
+  } else if (p.causal && p.q_pairs >= 8 && units > ctx->num_sms && 2LL * a->Lk >= a->Lq) {
     // long causal units differ in length up to q_pairs-fold: one CTA each, the longest first, so that the
-    // short ones fill the gaps at the end (8192 x 8192 of 16 heads: a fixed share of units per CTA left
-    // one with 1.5 times the mean)
+    // short ones fill the gaps at the end, where a fixed share of units per CTA left one with 1.5 times the
+    // mean. Against the persistent grid below, 16 heads, 2048 to 16384 queries and as many keys: 0.62 to 0.90
+    // of its time (8192: 274 us for 385); half as many keys: 0.77 to 1.00; a quarter: 0.92 to 1.13; an eighth:
+    // 1.05 to 1.27, for most units are then equally short and want their set-up overlapped. What key_len
+    // leaves of the keys is not known here: 4 items of 2048 with 2048, 512, 300 and 77 of them take 0.92, all
+    // with a sixteenth of 8192 1.23.
     p.heavy_first = 1;
   } else if (units > ctx->num_sms && (units + ctx->num_sms - 1) / ctx->num_sms <= attn::MAX_SEGS) {
     // more than one wave of whole units: a persistent grid, one CTA per SM

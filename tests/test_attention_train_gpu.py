@@ -438,3 +438,24 @@ def test_the_library_refuses_scales(ops):
             dev.check(ctx.lib.anima_attention_backward_workspace(ctx.h, ctypes.byref(g), ctypes.byref(need)))
     out, lse = ops.attention_lse(c.q, c.k, c.v, **c.kw, scale=2.0 ** -24)
     assert lse.isfinite().all()
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("Lk,lens", [(2048, (2048, 1333)), (1030, (1030, 0)), (300, None)])
+def test_long_causal_schedule(ops, D, Lk, lens):
+    """More causal units than SMs, of eight query tiles' pairs a head: one CTA each with the longest first, or (few
+    keys) a persistent grid. Both have the bits of each head alone, whose units are in neither."""
+    B, H, L = 2, 16, 2048
+    c = Case(B, H, 1, D, L, Lk, BF, causal=True, lens=lens)
+    out, lse = ops.attention_lse(c.q, c.k, c.v, **c.kw)
+    if D == 128:
+        assert torch.equal(ops.attention(c.q, c.k, c.v, **c.kw), out)
+    for b in range(B):
+        for h in (0, 5, 15):
+            q, k, v = (c.heads(t, n)[b, h].contiguous() for t, n in ((c.q, L), (c.k, Lk), (c.v, Lk)))
+            o1, l1 = ops.attention_lse(q, k, v, Lq=L, Lk=Lk, H=1, D=D, causal=True,
+                                       key_len=c.lens[b:b + 1] if lens else None)
+            assert torch.equal(c.heads(out, L)[b, h], o1) and torch.equal(lse[b, h], l1[0, 0])
+    one = [c.heads(t, n)[:, 3:4].double() for t, n in ((c.q, L), (c.k, Lk), (c.v, Lk), (c.do, L))]
+    val, tol = reference(*one, causal=True, lens=c.lens, dtype=BF)
+    check({"out": c.heads(out, L)[:, 3:4], "lse": lse[:, 3:4]}, val, tol, ("out", "lse"))
