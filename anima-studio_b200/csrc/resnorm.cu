@@ -823,22 +823,26 @@ struct SumParams {
   int items, parts, sums, C;
   float* out[kMaxSums];
   int per_item[kMaxSums];  // out [items][C], else [C] over all items
+  unsigned end[kMaxSums];  // the block behind the sum's last
 };
 
-// out = the partial rows added in a fixed order. A block takes 32 columns of one output row; its warps
-// each add every blockDim.y-th partial, then the first adds the warps' sums.
+// out = the partial rows added in a fixed order. A block takes 32 columns of one output row (the sums' rows one
+// after another: an item is no grid axis of its own, which would end at 65535); its warps each add every
+// blockDim.y-th partial, then the first adds the warps' sums.
 __global__ void __launch_bounds__(1024) partial_sum_kernel(const SumParams p) {
   __shared__ float red[32][32];
-  const int s = blockIdx.z, item = blockIdx.y;
-  if (!p.per_item[s] && item) return;
-  const int c = blockIdx.x * 32 + threadIdx.x, warps = blockDim.y;
-  const int n = p.per_item[s] ? p.parts : p.parts * p.items;
+  int s = 0;
+  while (blockIdx.x >= p.end[s]) ++s;
+  const unsigned at = blockIdx.x - (s ? p.end[s - 1] : 0u), column_blocks = (p.C + 31) / 32;
+  const unsigned item = at / column_blocks;
+  const int c = (at - item * column_blocks) * 32 + threadIdx.x, warps = blockDim.y;
+  const size_t n = static_cast<size_t>(p.parts) * (p.per_item[s] ? 1 : p.items);
   const size_t stride = static_cast<size_t>(p.sums) * p.C;
   const float* base = p.part + (static_cast<size_t>(item) * p.parts * p.sums + s) * p.C + c;
   float t = 0.f;
   if (c < p.C) {
 #pragma unroll 4
-    for (int i = threadIdx.y; i < n; i += warps) t += base[i * stride];
+    for (size_t i = threadIdx.y; i < n; i += warps) t += base[i * stride];
   }
   red[threadIdx.y][threadIdx.x] = t;
   __syncthreads();
@@ -1074,7 +1078,12 @@ extern "C" int anima_residual_norm_backward(anima_ctx* ctx, const anima_residual
     st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), 2 * kMaxCols * 16);
     if (st) return st;
   }
-  ANIMA_REQUIRE(static_cast<long long>(items) * p.parts < (1LL << 31) && items <= 65535,
+  long long blocks = 0;  // of the sums
+  for (int i = 0; i < k; ++i) {
+    blocks += static_cast<long long>((a->cols + 31) / 32) * (sp.per_item[i] ? items : 1);
+    sp.end[i] = static_cast<unsigned>(blocks);
+  }
+  ANIMA_REQUIRE(static_cast<long long>(items) * p.parts < (1LL << 31) && blocks < (1LL << 31),
                 "anima_residual_norm_backward: %d items are too many", items);
   ProfScope prof(ctx, "residual_norm.grad", 0, static_cast<double>(a->rows) * a->cols * 20);
   fn<<<items * p.parts, dim3(s.T, s.Y), smem, ctx->stream>>>(p);
@@ -1085,6 +1094,8 @@ extern "C" int anima_residual_norm_backward(anima_ctx* ctx, const anima_residual
   sp.parts = p.parts * s.Y;
   sp.sums = p.sums;
   sp.C = a->cols;
-  partial_sum_kernel<<<dim3((a->cols + 31) / 32, items, p.sums), dim3(32, sp.parts * items > 296 ? 32 : 8), 0, ctx->stream>>>(sp);
+  // (32 warps for a sum over more partials than two blocks an SM leave: with 8 each would add dozens in turn)
+  const bool many = static_cast<long long>(sp.parts) * items > 2LL * ctx->num_sms;
+  partial_sum_kernel<<<static_cast<unsigned>(blocks), dim3(32, many ? 32 : 8), 0, ctx->stream>>>(sp);
   return check_launch("partial_sum_kernel");
 }

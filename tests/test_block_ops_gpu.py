@@ -460,3 +460,25 @@ def test_two_threads_on_streams_of_their_own(ops):
     for t in threads:
         t.join()
     assert not errors and wrong == [0, 0]
+
+
+@pytest.mark.parametrize("rows,C,L", [(65536, 8, 1), (70001, 33, 1), (131074, 64, 2)])
+def test_residual_norm_of_many_items(ops, rows, C, L):
+    """A modulation for each row or two, more of them than a grid axis has blocks, beside sums over all."""
+    t, c = make_norm(rows, C, L, "rms", "rms", True, torch.float32, torch.float32, torch.float32, seed=110)
+    x, h = ops.residual_norm(t["x"], t["y"], **kwargs(t, c))
+    rx, rh = norm_ref({n: (v.double() if v is not None else None) for n, v in t.items()}, c)
+    assert rel(x, rx) <= 64 * U and rel(h, rh) <= 64 * U
+    got = ops.residual_norm_backward(t["dh"], t["dx_out"], t["x"], t["y"], **kwargs(t, c))
+    ref = grad_refs(t, c)
+    check_grads(got, ref, rows)
+    # each item for itself: some 20 roundings of every term, and the terms' own sums of magnitudes
+    p = {n: v.double() for n, v in t.items() if v is not None}
+    item = torch.arange(rows, device=DEV) // L
+    r = 1 / (p["x"].square().mean(1, keepdim=True) + c["eps"]).sqrt()
+    n, u = p["x"] * r, normalise(p["y"], "rms", c["eps"]) * p["post_w"]
+    g = p["dh"] * (1 + p["scale"][item]) * p["pre_w"]
+    G = p["dx_out"].abs() + r * (g.abs() + n.abs() * (g * n).abs().mean(1, keepdim=True))
+    for name, mag in (("gate", c["alpha"] * G * u.abs()), ("scale", (p["dh"] * n * p["pre_w"]).abs()), ("shift", p["dh"].abs())):
+        mag = mag.view(-1, L, C).sum(1)
+        assert bool(((getattr(got, "d" + name).double() - ref[name]).abs() <= 64 * U * mag).all()), name
