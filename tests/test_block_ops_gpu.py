@@ -482,3 +482,24 @@ def test_residual_norm_of_many_items(ops, rows, C, L):
     for name, mag in (("gate", c["alpha"] * G * u.abs()), ("scale", (p["dh"] * n * p["pre_w"]).abs()), ("shift", p["dh"].abs())):
         mag = mag.view(-1, L, C).sum(1)
         assert bool(((getattr(got, "d" + name).double() - ref[name]).abs() <= 64 * U * mag).all()), name
+
+
+def test_residual_norm_rows_out_of_range(ops):
+    """Infinities, NaN and squares past fp32 stay in their rows, forward and backward, in the forms for whole and
+    for other widths alike: a row whose squares overflow has the norm 0 (its x_out stays), as 1 / sqrt(inf) says."""
+    for C in (1024, 1000):
+        t, c = make_norm(16, C, 16, None, "rms", False, torch.float32, torch.float32, torch.float32, seed=120)
+        kw = kwargs(t, c)
+        t["y"].zero_()
+        x0, h0 = ops.residual_norm(t["x"], t["y"], **kw)
+        g0 = ops.residual_norm_backward(t["dh"], t["dx_out"], t["x"], t["y"], **kw)
+        x = t["x"].clone()
+        x[3], x[7, 5], x[9, 11] = 1e25, float("inf"), float("nan")
+        x1, h1 = ops.residual_norm(x, t["y"], **kw)
+        g1 = ops.residual_norm_backward(t["dh"], t["dx_out"], x, t["y"], **kw)
+        keep = torch.tensor([r not in (3, 7, 9) for r in range(16)], device=DEV)
+        for a, b in ((x0, x1), (h0, h1), (g0.dx, g1.dx), (g0.dy, g1.dy)):
+            assert torch.equal(a[keep], b[keep])
+        assert bool((h1[3] == 0).all() and torch.equal(x1[3], x[3]) and torch.equal(g1.dx[3], t["dx_out"][3]))
+        others = torch.arange(C, device=DEV) != 5
+        assert bool(h1[7, 5].isnan() and (h1[7, others] == 0).all() and h1[9].isnan().all())
