@@ -349,20 +349,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         gb += nb;
       }
-      if (*abort_flag) {
-        // let every copy this thread started land before the CTA exits
-        for (int i = 0; i < 6; ++i) {
-          const uint32_t a = (armed >> (2 * i)) & 3u;
-          if (!(a & 2u)) continue;
-          uint64_t* fb = i == 5 ? v_tail : bars + (i < 3 ? i : i + 2);  // q_full, k_full[0..1], v_full[0..1], v_tail
-          const unsigned long long t0 = globaltimer();
-          while (!mbar_test(smem_u32(fb), a & 1u)) {
-            if (globaltimer() - t0 > kWaitTimeoutNs) {
-              flag_error(kErrTimeoutDrain);
-              break;
-            }
-          }
-        }
+      // every copy this thread started lands before the CTA exits: another warp's wait can run out after the
+      // last of them was issued (on the way all are waited for anyway)
+      for (int i = 0; i < 6; ++i) {
+        const uint32_t a = (armed >> (2 * i)) & 3u;
+        // q_full, k_full[0..1], v_full[0..1], v_tail
+        if (a & 2u) mbar_settle(i == 5 ? v_tail : bars + (i < 3 ? i : i + 2), a & 1u);
       }
     }
   } else if (warp == kMmaWarp) {
@@ -437,17 +429,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         gb += nb;
       }
-      if (!ok) {
-        // every MMA this thread issued completes before the CTA frees tensor memory
-        umma_commit(drain, lead);
-        const unsigned long long t0 = globaltimer();
-        while (!mbar_test(smem_u32(drain), 0)) {
-          if (globaltimer() - t0 > kWaitTimeoutNs) {
-            flag_error(kErrTimeoutDrain);
-            break;
-          }
-        }
-      }
+      // every MMA this warp issued completes before the CTA frees tensor memory, whether a wait of this warp
+      // ran out or one of the softmax warps'
+      umma_commit(drain, lead);
+      mbar_settle(drain, 0);
     }
   } else {
     // softmax: tile x, lane quadrant `quad` (rows quad * 32 + lane), key-column half hf

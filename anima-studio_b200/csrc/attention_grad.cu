@@ -392,19 +392,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (++s0 == y0_stages) s0 = 0, ph0 ^= 1;
         if (++s1 == Y1_STAGES) s1 = 0, ph1 ^= 1;
       }
-      if (*abort_flag) {
-        // let every copy this thread started land before the block exits
-        for (int i = 0; i < 6; ++i) {
-          const uint32_t a = (armed >> (2 * i)) & 3u;
-          if (!(a & 2u)) continue;
-          const unsigned long long t0 = globaltimer();
-          while (!mbar_test(smem_u32(bars + i), a & 1u)) {
-            if (globaltimer() - t0 > kWaitTimeoutNs) {
-              flag_error(kErrTimeoutDrain);
-              break;
-            }
-          }
-        }
+      // every copy this thread started lands before the block exits: another warp's wait can run out after
+      // the last of them was issued (on the way all are waited for anyway)
+      for (int i = 0; i < 6; ++i) {
+        const uint32_t a = (armed >> (2 * i)) & 3u;
+        if (a & 2u) mbar_settle(bars + i, a & 1u);
       }
     }
   } else if (warp == kMmaWarp) {
@@ -505,19 +497,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (++r0 == Y0_STAGES) r0 = 0;
         }
       }
-      if (ok) {
-        umma_commit(bar.acc_done, lead);
-      } else {
-        // every product this thread issued completes before the block frees tensor memory
-        umma_commit(bar.drain, lead);
-        const unsigned long long t0 = globaltimer();
-        while (!mbar_test(smem_u32(bar.drain), 0)) {
-          if (globaltimer() - t0 > kWaitTimeoutNs) {
-            flag_error(kErrTimeoutDrain);
-            break;
-          }
-        }
-      }
+      // every product this warp issued completes before the block frees tensor memory, whether a wait of
+      // this warp ran out or one of the math warps'
+      uint64_t* done = ok ? bar.acc_done : bar.drain;
+      umma_commit(done, lead);
+      mbar_settle(done, 0);
     }
   } else {
     const int qt = warp >> 2, quad = warp & 3;

@@ -110,6 +110,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   return mbar_wait_for(bar, parity, abort_flag, err, kWaitTimeoutNs);
 }
 
+// Before a role leaves: the copies or products that complete this phase are done (bounded, and whatever
+// the abort flag says), so that the block does not exit under them.
+__device__ __forceinline__ void mbar_settle(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_test(a, parity)) return;
+  const unsigned long long t0 = globaltimer();
+  while (!mbar_test_sleep(a, parity)) {
+    if (globaltimer() - t0 > kWaitTimeoutNs) {
+      flag_error(kErrTimeoutDrain);
+      return;
+    }
+  }
+}
+
 // ------------------------------------------------------------------ TMA (no multicast anywhere)
 
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
