@@ -74,6 +74,8 @@ def _rows(fn: str, name: str, t: torch.Tensor, rows: int, cols: int, dtype=None,
     shape, st, dt = t.shape, t.stride(), t.dtype
     if len(shape) != 2 or shape[0] != rows or (shape[1] != cols if exact else shape[1] < cols):
         raise dev.AnimaError(1, f"{fn}: {name} is {tuple(shape)}, expected [{rows}, {cols}]")
+    if rows > _MOST or cols > _MOST:
+        raise dev.AnimaError(1, f"{fn}: {name} is [{rows}, {cols}], sizes end at 2^30")
     if st[1] != 1 and shape[1] > 1:
         raise dev.AnimaError(1, f"{fn}: {name} needs contiguous rows (strides {st})")
     if dt not in _FLOATS or (dtype is not None and dt is not dtype):
@@ -83,6 +85,7 @@ def _rows(fn: str, name: str, t: torch.Tensor, rows: int, cols: int, dtype=None,
     return st[0] if rows > 1 else shape[1]  # a single row's stride says nothing
 
 
+_MOST = 2 ** 30  # sizes beyond are refused here: ctypes would cut a C int's upper bits off without a word
 _FLOATS = frozenset((torch.float32, torch.bfloat16, torch.float16))
 
 
@@ -217,8 +220,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, *, H
     at offset + r % rows_per_item (default: all rows are one item). inverse: the transposed rotation,
     for gradients. Returns (out_q, out_k), new tensors unless given; out_q may be q itself."""
     rows, dt, at, R = q.shape[0], q.dtype, q.get_device(), inv_freq.shape[0] * 2
+    if R > _MOST:
+        raise dev.AnimaError(1, f"rotary: {R} rotated dims")
     a = dev.RotaryArgs(dtype=dev.DTYPE_CODE.get(dt, -1), rows=rows, D=D, R=R, Hq=Hq, mscale=mscale, offset=offset,
-                       rows_per_item=rows_per_item or max(rows, 1), interleaved=interleaved, inverse=inverse)
+                       rows_per_item=min(rows_per_item or rows, rows) or 1, interleaved=interleaved, inverse=inverse)
     a.ldq = _rows("rotary", "q", q, rows, Hq * D)
     if out_q is None:
         out_q, a.ldoq = torch.empty((rows, Hq * D), dtype=dt, device=q.device), Hq * D
@@ -253,6 +258,8 @@ def _residual_norm_args(fn, x, y, alpha, gate, post, post_w, pre, pre_w, scale, 
         raise dev.AnimaError(1, f"{fn}: x has to be a 2-D tensor of rows")
     (rows, cols), at = x.shape, x.get_device()
     L = rows_per_item or max(rows, 1)
+    if L < 0 or rows % L:
+        raise dev.AnimaError(1, f"{fn}: {rows} rows are not items of {L} rows")
     items = rows // L
     a = dev.ResidualNormArgs(rows=rows, cols=cols, rows_per_item=L, post=NORM_KIND[post], pre=NORM_KIND[pre], alpha=alpha,
                              eps=eps)
@@ -537,6 +544,9 @@ def _train_args(fn, q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, q_off, k_off, v_off, b
     number of k/v items (1 where the batch shares one K/V) and the k/v columns."""
     if Lq <= 0 or Lk <= 0 or H <= 0 or batch <= 0 or group <= 0 or H % group:
         raise dev.AnimaError(1, f"{fn}: batch {batch}, {Lq} queries, {Lk} keys, {H} heads in groups of {group}")
+    if max(Lq, Lk, H, batch, q_off, k_off, v_off) > _MOST:
+        raise dev.AnimaError(1, f"{fn}: sizes and column offsets end at 2^30 (batch {batch}, {Lq} queries, {Lk} keys, {H} "
+                                f"heads, columns {q_off}, {k_off}, {v_off})")
     if D not in (64, 128):
         raise dev.AnimaError(1, f"{fn}: head_dim {D} (64 or 128)")
     if q.dtype not in (torch.bfloat16, torch.float16):

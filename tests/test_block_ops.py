@@ -242,3 +242,53 @@ def test_attention_refuses_scales_out_of_range(ops, err, dtype, scale):
         ops.attention_lse(**kw, scale=scale)
     with pytest.raises(err, match="scale"):
         ops.attention_backward(t(20, 128, dtype=dtype), out=t(20, 128, dtype=dtype), lse=t(2, 2, 10), **kw, scale=scale)
+
+
+FAR = 2 ** 32  # a C int would keep the rest: 5 rows of 2^32 + 5
+
+
+def far(rows, cols, dtype=torch.float32):
+    return torch.empty(rows, cols, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("rows,cols", [(FAR + 5, 64), (2 ** 30 + 1, 64), (5, FAR + 64)])
+def test_sizes_that_a_c_int_cuts_off_are_refused(ops, err, rows, cols):
+    inv = torch.empty(8, dtype=torch.float64, device="meta")
+    x = far(rows, cols)
+    for call in (lambda: ops.rotary(x, None, inv, Hq=1, D=cols), lambda: ops.residual_norm(x, x),
+                 lambda: ops.residual_norm_backward(x, x, x, x)):
+        with pytest.raises(err) as e:
+            call()
+        assert e.value.status == 1
+    with pytest.raises(err) as e:
+        ops.rotary(far(4, 64), None, torch.empty(FAR // 2 + 8, dtype=torch.float64, device="meta"), Hq=1, D=64)
+    assert e.value.status == 1
+
+
+@pytest.mark.parametrize("change", [dict(Lq=FAR + 10), dict(Lk=FAR + 12), dict(batch=FAR + 2), dict(H=FAR + 2),
+                                    dict(q_off=FAR), dict(k_off=FAR), dict(v_off=FAR + 8), dict(H=FAR + 2, group=FAR + 2)])
+def test_attention_sizes_that_a_c_int_cuts_off_are_refused(ops, err, change):
+    kw = {n: (far(2 ** 34, 128, torch.bfloat16) if isinstance(v, torch.Tensor) else v) for n, v in attn_kw().items()}
+    kw |= dict(q_bstride=8, k_bstride=8, v_bstride=8, ldq=2 ** 33, ldk=2 ** 33, ldv=2 ** 33)
+    with pytest.raises(err) as e:
+        ops.attention_lse(**{**kw, **change}, out=far(2 ** 37, 128, torch.bfloat16))
+    assert e.value.status == 1 and "2^30" in str(e.value)
+
+
+def test_rows_per_item_past_a_c_int(ops, monkeypatch):
+    """More rows an item than there are: one item, as the longest count that is kept whole says."""
+    dev, seen = pkg("device"), []
+
+    class Fake:
+        def call(self, name, args, **kw):
+            seen.append(args._obj.rows_per_item)
+
+    monkeypatch.setattr(ops, "ctx_for", lambda t: Fake())
+    inv = t(8, dtype=torch.float64)
+    for n in (None, 3, 6, FAR + 2, 2 ** 31):
+        ops.rotary(t(6, 16), None, inv, Hq=1, D=16, rows_per_item=n)
+    assert seen == [6, 3, 6, 6, 6]
+    for n in (4, FAR + 2, -3):
+        with pytest.raises(dev.AnimaError) as e:
+            ops.residual_norm(t(6, 16), t(6, 16), rows_per_item=n)
+        assert e.value.status == 1
