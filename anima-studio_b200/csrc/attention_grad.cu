@@ -243,7 +243,9 @@ __device__ __forceinline__ void put(void* out, size_t at, const float (&v)[N]) {
 
 // 2^x of a pair on the FMA and integer pipes: x = n + f, |f| <= 1/2, by adding 1.5 2^23 (whose sum has n
 // in its low bits), 2^f by a polynomial of degree 4 (least largest relative error, 2.6e-6), times 2^n put
-// together from n's bits. x below -127 gives 0, NaN stays NaN.
+// together from n's bits (the reduction of Cody and Waite, Software Manual for the Elementary Functions, 1980).
+// To share a softmax's exponentials between the special-function unit and the FMA pipe is a published idea
+// for attention on this architecture, not this code's own. x below -127 gives 0, NaN stays NaN.
 __device__ __forceinline__ f2 exp2_fma(f2 x) {
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));

@@ -11,11 +11,14 @@
 // The statistics are computed again from y and x' (a row is in registers anyway), so the forward saves
 // nothing.
 //
-// Both passes are bound by HBM. A row is held in registers by T = C / V threads (V = 8 columns a
-// thread, or 1 where the columns or alignments are odd); the row's sums are warp shuffles and one
-// exchange through shared memory a round. Where the threads hold 8 columns each and none is idle (C = 256,
-// 512, 1024, 2048), mean, squares about the mean and products with the gradient come from one round: the
-// threads' own moments about their own means are merged pairwise, which loses no digits to a large mean.
+// Both passes are bound by HBM in fp32 and at 2048 columns (forward 82%, backward 90% of the copy rate); a
+// backward of 1024 columns in 16 bits with a post norm is not: 4593 rows take 22.7 us for 8.6, with 767
+// instructions a warp and row, 60% of the issue slots and 19% of DRAM's rate. A row is held in registers by
+// T = C / V threads (V = 8 columns a thread, or 1 where the columns or alignments are odd); the row's sums are
+// warp shuffles and one exchange through shared memory a round. Where the threads hold 8 columns each (4096: 16)
+// and none is idle (C = 256, 512, 1024, 2048, 4096), mean, squares about the mean and products with the gradient
+// come from one round: the threads' own moments about their own means are merged pairwise, which loses no
+// digits to a large mean. The other widths take two to four dependent rounds a row, with no row in flight ahead.
 // The backward's column sums stay in registers over the rows
 // of a block, each block writes one partial row of sums and a second kernel adds the partials in a
 // fixed order: no atomics, the same inputs give the same bits.
@@ -870,19 +873,21 @@ Shape shape_of(int C, bool vec) {
   return s;
 }
 
-// Rows of one item that a block takes, with as many blocks as the SMs hold at once (`threads` of them an
-// SM), or one row each where there are not as many rows.
+// Rows of one item that a block takes, with as many blocks as `threads` of them an SM make, or one row each
+// where there are not as many rows. Up to 2048 columns the SMs hold them all at once. At 4096 they do not: the
+// forward's registers let two blocks of its three in (a wave and a half), and two places of four fp32 streams,
+// 128 KB, one block of the backward's two.
 void parts_of(const Shape& s, int items, int L, int sms, int threads, int& parts, int& part_rows) {
   const int blocks = threads / (s.T * s.Y) < 16 ? threads / (s.T * s.Y) : 16;
-  const int want = blocks * sms / items > 1 ? blocks * sms / items : 1;  // (one wave: a block more would double it)
+  const int want = blocks * sms / items > 1 ? blocks * sms / items : 1;  // (a block past a whole wave would double it)
   const int most = (L + s.Y - 1) / s.Y;
   parts = want < most ? want : most;
   part_rows = ((L + parts - 1) / parts + s.Y - 1) / s.Y * s.Y;
   parts = (L + part_rows - 1) / part_rows;
 }
-constexpr int kGradThreads = 512, kForwardThreads = 768;  // an SM, by the kernels' launch bounds
+constexpr int kGradThreads = 512, kForwardThreads = 768;  // an SM, by the launch bounds up to 2048 columns
 
-// Places of a ring: three, or two where three would leave an SM with fewer blocks.
+// Places of a ring: three, or two where three would leave an SM with fewer blocks than that.
 int places_of(const Shape& s, int threads, int row_bytes) { return kMaxPlaces * row_bytes * (threads / s.T) <= 208 * 1024 ? kMaxPlaces : 2; }
 int size_of_host(int dt) { return dt == ANIMA_F32 ? 4 : 2; }
 

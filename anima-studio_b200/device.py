@@ -268,7 +268,9 @@ class Context:
 
     def bind_stream(self):
         """Bind torch's current stream; the caller holds the lock until its call is made."""
-        check(self.lib.anima_ctx_set_stream(self.h, _raw_stream(self.device)))
+        status = self.lib.anima_ctx_set_stream(self.h, _raw_stream(self.device))
+        if status:
+            check(status)
         return self.h
 
     def call(self, name: str, *args, tag: str | None = None, work: float = 0.0, kernels: int = 1):
@@ -283,7 +285,9 @@ class Context:
             kt.events.append((name, tag, e0, e1, work))
         else:
             with self.lock:
-                check(getattr(self.lib, name)(self.bind_stream(), *args))
+                status = getattr(self.lib, name)(self.bind_stream(), *args)
+            if status:
+                check(status)
         if name in LAUNCHING:
             Context.launches += kernels
 

@@ -604,7 +604,7 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, Lq: int,
     """attention() for training: the same arguments (bf16 or fp16 q/k/v, D 64 or 128), and beside the
     output [batch * Lq, H D] the row statistics lse [batch, H, Lq] that attention_backward needs: ln of
     each query's sum of exponentials, -inf (with an output of zeros) where it sees no key. scale: 2^-24
-    (bf16: 2^-100) to 2^64. k and v may hold anything, NaN included, past key_len. Its workspace comes from torch's allocator, so calls on
+    (bf16: 2^-100) to 2^64; in fp16 |q.k| below 2^30 before it. k and v may hold anything, NaN included, past key_len. Its workspace comes from torch's allocator, so calls on
     several streams and captured graphs share nothing."""
     fn = "attention_lse"
     if out is None:
