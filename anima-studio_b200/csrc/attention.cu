@@ -1138,7 +1138,7 @@ int attention_launch(anima_ctx* ctx, const anima_attention_args* a, const Scratc
     // long causal units differ in length up to q_pairs-fold: one CTA each, the longest first, so that the
     // short ones fill the gaps at the end, where a fixed share of units per CTA left one with 1.5 times the
     // mean. Against the persistent grid below, 16 heads, 2048 to 16384 queries and as many keys: 0.62 to 0.90
-    // of its time (8192: 274 us for 385); half as many keys: 0.77 to 1.00; a quarter: 0.92 to 1.13; an eighth:
+    // of its time (8192: 274 us for 385); half as many keys: 0.77 to 1.00; a quarter: 0.90 to 1.13; an eighth:
     // 1.05 to 1.27, for most units are then equally short and want their set-up overlapped. What key_len
     // leaves of the keys is not known here: 4 items of 2048 with 2048, 512, 300 and 77 of them take 0.92, all
     // with a sixteenth of 8192 1.23.
