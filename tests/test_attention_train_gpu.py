@@ -459,3 +459,27 @@ def test_long_causal_schedule(ops, D, Lk, lens):
     one = [c.heads(t, n)[:, 3:4].double() for t, n in ((c.q, L), (c.k, Lk), (c.v, Lk), (c.do, L))]
     val, tol = reference(*one, causal=True, lens=c.lens, dtype=BF)
     check({"out": c.heads(out, L)[:, 3:4], "lse": lse[:, 3:4]}, val, tol, ("out", "lse"))
+
+
+@pytest.mark.parametrize("dtype,D,causal", [(BF, 64, False), (HF, 64, True), (HF, 128, False)])
+def test_more_items_than_a_grid_axis_has_blocks(ops, dtype, D, causal):
+    """Windows of a few tokens, each an item of its own."""
+    B, Lq, Lk = 66001, 3, 3 if causal else 5
+    lens = [(i * 7) % (Lk + 1) for i in range(B)]
+    c = Case(B, 1, 1, D, Lq, Lk, dtype, causal=causal, lens=lens)
+    check(c.run(ops), *c.reference())
+
+
+def test_more_items_share_keys_than_a_grid_axis_has_blocks(ops):
+    B, Lq, Lk, D = 66001, 2, 5, 64
+    c = Case(B, 1, 1, D, Lq, Lk, HF, gscale=0.03)
+    for t in (c.k, c.v):
+        t.view(B, Lk, -1)[1:] = t.view(B, Lk, -1)[0]
+    val, tol = c.reference()
+    k, v, kw = c.k[:Lk].contiguous(), c.v[:Lk].contiguous(), {**c.kw, "k_bstride": 0, "v_bstride": 0}
+    out, lse = ops.attention_lse(c.q, k, v, **kw)
+    dq, dk, dv = ops.attention_backward(c.do, c.q, k, v, out, lse, **kw)
+    check({"out": c.heads(out, Lq), "lse": lse, "dq": c.heads(dq, Lq)}, val, tol, ("out", "lse", "dq"))
+    for n, g in (("dk", dk), ("dv", dv)):
+        r = val[n].sum(0)
+        assert bool(((g.view(Lk, 1, D).transpose(0, 1).double() - r).abs() <= tol[n].sum(0) + half_step(HF) * r.abs()).all()), n
